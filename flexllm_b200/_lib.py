@@ -98,6 +98,12 @@ SIGNATURES = {
     "flexllm_attn_window_bias": [_P, _P, _I, _I, _P, _P],
     "flexllm_attn_window_workspace": [_P, _I, _I],
     "flexllm_attn_window": [_I, _P, _I, _P, _P, _P, _P, _P, _F, _P, _P, _I, _P, _I, _I, _I, _P, _L, _P, _SZ, _P],
+    "flexllm_kv_cache_pages": [_P, _I, _P],
+    "flexllm_qk_norm_rope": [_I, _P, _I, _P, _L, _P, _P, _F, _P, _I, _P, _P, _P, _I, _I, _P, _P, _P, _I, _I, _I, _I, _P, _L, _P],
+    "flexllm_attn_packed": [_I, _P, _I, _F, _P, _L, _P, _P, _P, _I, _I, _I, _I, _P, _L, _P],
+    "flexllm_attn_tree": [_I, _P, _I, _F, _P, _L, _P, _P, _P, _P, _I, _I, _I, _I, _P, _L, _P],
+    "flexllm_kv_keep": [_I, _P, _I, _P, _I, _P, _I, _P, _P, _I, _I, _P],
+    "flexllm_linear_w4": [_I, _P, _L, _P, _P, _I, _P, _I, _P, _I, _I, _I, _P, _L, _I, _P],
     "flexllm_hmt_create": [_P, _P, _P, _I, _P, _P, _P],
     "flexllm_hmt_destroy": [_P],
     "flexllm_hmt_prefill": [_P, _P, _I, _P, _P, _P],
@@ -133,6 +139,10 @@ class DecoderConfig(C.Structure):
 
 class KvShape(C.Structure):
     _fields_ = [("hkv", _I), ("kdim", _I), ("vdim", _I)]
+
+
+class KvPages(C.Structure):
+    _fields_ = [("k", _P), ("v", _P), ("n_pages", _I), ("hkv", _I), ("kdim", _I), ("vdim", _I)]
 
 
 class AttnWindowShape(C.Structure):

@@ -768,6 +768,13 @@ extern "C" int flexllm_kv_cache_reset(flexllm_kv_cache* c, void* stream) {
     return FLEXLLM_OK;
 }
 
+extern "C" int flexllm_kv_cache_pages(flexllm_kv_cache* c, int layer, flexllm_kv_pages* out) {
+    FLEXLLM_REQUIRE(c && out && c->elem_bytes != 1 && layer >= 0 && layer < c->layers);
+    const flexllm_kv_shape& s = c->shape[layer];
+    *out = {c->k + c->k_off[layer], c->v + c->v_off[layer], c->n_pages, s.hkv, s.kdim, s.vdim};
+    return FLEXLLM_OK;
+}
+
 extern "C" int flexllm_kv_cache_pools(flexllm_kv_cache* c, int layer, int8_t** k, float** ks, int8_t** v, float** vs) {
     FLEXLLM_REQUIRE(c && layer >= 0 && layer < c->layers);
     if (c->elem_bytes != 1) {

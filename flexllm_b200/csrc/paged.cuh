@@ -1,0 +1,79 @@
+// What the operators over packed sequences and the floating-point paged cache share: sequence b of a call has the packed rows
+// cu[b] .. cu[b+1] - 1, at cache positions ctx[b] .., in pages of 64 tokens, K [page][G][64][dk], V transposed [page][G][dv][64].
+// cu, ctx and the page table are device memory that the host never sees: values out of range are clamped (a page id: page 0; entries
+// that no position needs are not looked at) and reported through the device's error word, so that no access leaves its buffer.
+#pragma once
+#include "float_common.cuh"
+
+namespace flexllm {
+
+constexpr int kPage = 64;
+
+struct PackedSeqs {
+    const int32_t *cu, *ctx, *page_table;
+    int max_pages, max_ctx, B, T, n_pages;
+    int max_new;                           // most rows of one sequence
+    int* error_flag;
+};
+struct SeqRows { int row0, n, ctx; };      // first packed row, rows, tokens already in the cache
+
+__device__ __forceinline__ void data_error(int* flag) { if (flag) atomicOr(flag, 2); }
+
+__device__ __forceinline__ SeqRows seq_rows(const PackedSeqs& p, int b) {
+    const int c0 = p.cu[b], c1 = p.cu[b + 1], x0 = p.ctx[b];
+    SeqRows s;
+    s.row0 = min(max(c0, 0), p.T);
+    s.n = min(max(c1, s.row0), p.T) - s.row0;
+    s.n = min(min(s.n, p.max_new), p.max_ctx + 1);
+    s.ctx = min(max(x0, 0), p.max_ctx + 1 - s.n);
+    if (s.row0 != c0 || s.n != c1 - c0 || (s.n > 0 && s.ctx != x0)) data_error(p.error_flag);
+    return s;
+}
+__device__ __forceinline__ int page_of(const PackedSeqs& p, int b, int i) {
+    const int page = p.page_table[(long)b * p.max_pages + i];
+    if ((unsigned)page < (unsigned)p.n_pages) return page;
+    data_error(p.error_flag);
+    return 0;
+}
+
+// Unit `u` of a call whose sequences have count(rows) units each, counted from the last unit of the last sequence (in causal attention the
+// longest first). One whole warp; b < 0: no such unit.
+struct Unit { int b, i; SeqRows s; };
+template <class Count> __device__ __forceinline__ Unit find_unit(const PackedSeqs& p, int u, Count count) {
+    const int lane = threadIdx.x & 31;
+    Unit r;
+    r.b = -1; r.i = 0; r.s.row0 = r.s.n = r.s.ctx = 0;
+    int base = 0;
+    for (int b0 = 0; b0 < p.B; b0 += 32) {
+        const int b = p.B - 1 - b0 - lane;
+        SeqRows s = {0, 0, 0};
+        if (b >= 0) s = seq_rows(p, b);
+        const int c = s.n > 0 ? count(s) : 0;
+        int incl = c;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int t = __shfl_up_sync(0xffffffffu, incl, o);
+            if (lane >= o) incl += t;
+        }
+        const unsigned hit = __ballot_sync(0xffffffffu, u < base + incl);
+        if (hit) {
+            const int src = __ffs(hit) - 1;
+            r.b = __shfl_sync(0xffffffffu, b, src);
+            r.i = base + __shfl_sync(0xffffffffu, incl, src) - 1 - u;
+            r.s.row0 = __shfl_sync(0xffffffffu, s.row0, src);
+            r.s.n = __shfl_sync(0xffffffffu, s.n, src);
+            r.s.ctx = __shfl_sync(0xffffffffu, s.ctx, src);
+            return r;
+        }
+        base += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    return r;
+}
+
+// The host's checks of those arguments.
+inline bool packed_ok(const PackedSeqs& p) {
+    return p.cu && p.ctx && p.page_table && p.B > 0 && p.T >= 0 && p.max_pages > 0 && p.n_pages > 0 && p.max_ctx >= 0 &&
+           (long)p.max_ctx < (long)p.max_pages * kPage;
+}
+
+}  // namespace flexllm

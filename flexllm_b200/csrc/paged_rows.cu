@@ -1,0 +1,296 @@
+// Rows of packed sequences on their way into the floating-point paged cache, and within it:
+//   qk_norm_rope  norm of every q and k head, rotation, q to a dense tensor, k and v to the pages
+//   kv_keep       the entries of an accepted path moved together
+#include "paged.cuh"
+
+namespace flexllm {
+
+namespace {
+
+// Norm and rotation.  y = x / sqrt(mean x^2 + eps) * gain;  pair p < rot/2 turns elements p and p + rot/2 by the angle whose cosine and sine
+// the tables hold at [pos[axis of p]][p]; elements from rot on stay. All in fp32, rounded once.
+// HBM bound: every row is read and written once, the tables' rows come from L2. A group of L lanes holds a head: lane c the pairs
+// 4 c .. 4 c + 3 (two vectors of four elements, so that both halves of a pair meet in one thread), the lanes behind them eight of the unrotated
+// elements each. A warp stays with one token, so that its table entries are read once for the heads that it takes.
+struct RopeArgs {
+    PackedSeqs seq;
+    int H, G, dk, dv, rot;
+    const void* proj; long ldp;
+    const float *q_gain, *k_gain;
+    float eps;
+    const int32_t* pos; int axes, sec_end[4];      // pairs below sec_end[a] (and not below sec_end[a - 1]) turn by axis a's position
+    const float *cos_t, *sin_t; int table_len;
+    void *k, *v;
+    void* q; long ldq;
+    int chunks, qk_ctas, v_units;
+};
+constexpr int kRopeHeads = 8;             // heads of one warp
+
+template <class T, int L> __device__ __forceinline__ void rope_warp(const RopeArgs& a, long w) {
+    const int lane = threadIdx.x & 31, c = lane % L, sub = lane / L;
+    const int t = (int)(w / a.chunks), h0 = (int)(w % a.chunks) * kRopeHeads;
+    if (t >= a.seq.T) return;
+    // the sequence of the row: the last one that starts at or before it and has rows
+    int lo = 0, hi = a.seq.B - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (a.seq.cu[mid] <= t) lo = mid; else hi = mid - 1;
+    }
+    const SeqRows s = seq_rows(a.seq, lo);
+    if (t < s.row0 || t >= s.row0 + s.n) return;
+    const int at = s.ctx + t - s.row0;
+    const int half = a.rot >> 1, nrot = half >> 2;
+    const bool turns = c < nrot, rest = !turns && a.rot + (c - nrot) * 8 < a.dk;
+    const int e0 = turns ? 4 * c : a.rot + (c - nrot) * 8, e1 = turns ? e0 + half : e0 + 4;
+    float co[4], si[4];
+    if (turns) {
+#pragma unroll
+        for (int p = 0; p < 4; p++) {
+            int axis = 0;
+            while (axis < a.axes - 1 && e0 + p >= a.sec_end[axis]) axis++;
+            int row = a.pos[(long)axis * a.seq.T + t];
+            if ((unsigned)row >= (unsigned)a.table_len) { data_error(a.seq.error_flag); row = row < 0 ? 0 : a.table_len - 1; }
+            co[p] = a.cos_t[(long)row * half + e0 + p]; si[p] = a.sin_t[(long)row * half + e0 + p];
+        }
+    }
+    const T* src = (const T*)a.proj + (long)t * a.ldp;
+    const long page = page_of(a.seq, lo, at / kPage);
+#pragma unroll
+    for (int j = 0; j < kRopeHeads * L / 32; j++) {
+        const int h = h0 + j * (32 / L) + sub;
+        const bool on = h < a.H + a.G && (turns || rest);
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
+        if (on) { x = load4(src + (long)h * a.dk + e0); y = load4(src + (long)h * a.dk + e1); }
+        const float* gain = h < a.H ? a.q_gain : a.k_gain;
+        float ss = x.x * x.x + x.y * x.y + x.z * x.z + x.w * x.w + y.x * y.x + y.y * y.y + y.z * y.z + y.w * y.w;
+#pragma unroll
+        for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        if (!on) continue;
+        if (gain) {
+            const float r = 1.0f / sqrtf(ss / (float)a.dk + a.eps);
+            const float4 gx = load4(gain + e0), gy = load4(gain + e1);
+            x = make_float4(x.x * r * gx.x, x.y * r * gx.y, x.z * r * gx.z, x.w * r * gx.w);
+            y = make_float4(y.x * r * gy.x, y.y * r * gy.y, y.z * r * gy.z, y.w * r * gy.w);
+        }
+        if (turns) {
+            const float4 u = x;
+            x = make_float4(u.x * co[0] - y.x * si[0], u.y * co[1] - y.y * si[1], u.z * co[2] - y.z * si[2], u.w * co[3] - y.w * si[3]);
+            y = make_float4(y.x * co[0] + u.x * si[0], y.y * co[1] + u.y * si[1], y.z * co[2] + u.z * si[2], y.w * co[3] + u.w * si[3]);
+        }
+        T* dst = h < a.H ? (T*)a.q + (long)t * a.ldq + (long)h * a.dk
+                         : (T*)a.k + ((page * a.G + (h - a.H)) * kPage + (at & (kPage - 1))) * a.dk;
+        store4(dst + e0, x);
+        store4(dst + e1, y);
+    }
+}
+
+// 16 bytes of consecutive slots of a V^T row
+template <class T> struct Slots;
+template <> struct Slots<bf16> { static constexpr int N = 8; };
+template <> struct Slots<float> { static constexpr int N = 4; };
+
+// CTAs below qk_ctas: eight warps of the above. Then one (page of a sequence, key/value head) each: the page's new value rows through shared
+// memory into its columns, whole 16-byte pieces where the call fills them.
+template <class T, int L> __global__ void __launch_bounds__(256) qk_norm_rope_kernel(const __grid_constant__ RopeArgs a) {
+    extern __shared__ __align__(16) uint8_t raw[];
+    __shared__ Unit unit_sm;
+    pdl_sync();
+    if ((int)blockIdx.x < a.qk_ctas) {
+        rope_warp<T, L>(a, (long)blockIdx.x * 8 + (threadIdx.x >> 5));
+        return;
+    }
+    const int id = blockIdx.x - a.qk_ctas, g = id % a.G, tid = threadIdx.x;
+    if (tid < 32) {
+        const Unit u = find_unit(a.seq, id / a.G, [](const SeqRows& s) { return (s.ctx + s.n - 1) / kPage - s.ctx / kPage + 1; });
+        if (tid == 0) unit_sm = u;
+    }
+    __syncthreads();
+    if (unit_sm.b < 0) return;
+    const SeqRows s = unit_sm.s;
+    const int pg = s.ctx / kPage + unit_sm.i;
+    const int lo = max(s.ctx, pg * kPage) - pg * kPage, hi = min(s.ctx + s.n - pg * kPage, kPage);      // slots [lo, hi)
+    constexpr int N = Slots<T>::N;
+    const int pitch = a.dv + 4 / (int)sizeof(T);          // elements: consecutive rows one word apart
+    T* tile = reinterpret_cast<T*>(raw);                  // [slot][pitch]
+    const T* src = (const T*)a.proj + (long)(s.row0 + pg * kPage - s.ctx) * a.ldp + (long)(a.H + a.G) * a.dk + (long)g * a.dv;
+    const int vec = a.dv / N;
+    for (int e = tid; e < (hi - lo) * vec; e += 256) {
+        const int t = lo + e / vec, d = (e % vec) * N;
+        const uint4 w = *reinterpret_cast<const uint4*>(src + (long)t * a.ldp + d);
+        uint32_t* dst = reinterpret_cast<uint32_t*>(tile + (long)t * pitch + d);
+        dst[0] = w.x; dst[1] = w.y; dst[2] = w.z; dst[3] = w.w;
+    }
+    const long page = page_of(a.seq, unit_sm.b, pg);
+    __syncthreads();
+    T* vp = (T*)a.v + (page * a.G + g) * (long)a.dv * kPage;
+    constexpr int PIECES = kPage / N;
+    for (int e = tid; e < a.dv * PIECES; e += 256) {
+        const int d = e / PIECES, t0 = (e % PIECES) * N;
+        if (t0 + N <= lo || t0 >= hi) continue;
+        __align__(16) T x[N];
+#pragma unroll
+        for (int i = 0; i < N; i++) x[i] = t0 + i >= lo && t0 + i < hi ? tile[(long)(t0 + i) * pitch + d] : from_f<T>(0.0f);
+        T* dst = vp + (long)d * kPage + t0;
+        if (t0 >= lo && t0 + N <= hi) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(x);
+        else
+#pragma unroll
+            for (int i = 0; i < N; i++)
+                if (t0 + i >= lo && t0 + i < hi) dst[i] = x[i];
+    }
+}
+
+template <class T, int L> int launch_rope(RopeArgs& a, cudaStream_t st) {
+    a.chunks = (a.H + a.G + kRopeHeads - 1) / kRopeHeads;
+    const long qk = ((long)a.seq.T * a.chunks + 7) / 8;
+    // a sequence's rows touch at most two pages more than they would fill
+    const long units = (long)a.seq.T / kPage + 2L * (a.seq.B < a.seq.T ? a.seq.B : a.seq.T);
+    if (qk + units * a.G > 0x7fffffffL) return FLEXLLM_ENOTSUP;
+    a.qk_ctas = (int)qk;
+    const size_t smem = (size_t)kPage * (a.dv * sizeof(T) + 4);
+    auto kern = qk_norm_rope_kernel<T, L>;
+    TRY_RC(allow_shared(kern, smem));
+    launch_k(kern, dim3((unsigned)(qk + units * a.G)), dim3(256), smem, st, a);
+    return launch_status();
+}
+template <class T> int run_rope(RopeArgs& a, cudaStream_t st) {
+    if (a.dk <= 64) return launch_rope<T, 8>(a, st);
+    if (a.dk <= 128) return launch_rope<T, 16>(a, st);
+    return launch_rope<T, 32>(a, st);
+}
+
+// new[ctx + i] = old[ctx + keep[i]], i < count: one CTA per (sequence, key/value head, layer). All old entries are in shared memory before the
+// first new one is written, so the indices may come in any order. Latency bound: a few KB per CTA; entries that stay are not touched.
+struct KeepLayer { void *k, *v; int hkv, dk, dv, n_pages; };
+constexpr int kKeepLayers = 64;
+struct KeepArgs {
+    PackedSeqs seq;                        // cu unused
+    const int32_t *keep, *count;
+    int most;
+    KeepLayer layer[kKeepLayers];
+};
+template <class T> __global__ void __launch_bounds__(256) kv_keep_kernel(const __grid_constant__ KeepArgs a) {
+    extern __shared__ __align__(16) uint8_t raw[];
+    __shared__ int src_page[64], src_slot[64], dst_page[64], dst_slot[64], n_moves;
+    const KeepLayer& y = a.layer[blockIdx.z];
+    const int b = blockIdx.x, g = blockIdx.y, tid = threadIdx.x;
+    pdl_sync();
+    if (g >= y.hkv) return;
+    if (tid == 0) n_moves = 0;
+    __syncthreads();
+    int count = a.count[b], ctx = a.seq.ctx[b];
+    if (count < 0 || count > a.most) { if (tid == 0) data_error(a.seq.error_flag); count = min(max(count, 0), a.most); }
+    if (tid < count) {
+        PackedSeqs p = a.seq;
+        p.n_pages = y.n_pages;
+        const int from = a.keep[(long)b * a.most + tid], s = ctx + from, d = ctx + tid;
+        if (ctx < 0 || from < 0 || from >= 64 || s > a.seq.max_ctx || d > a.seq.max_ctx) data_error(a.seq.error_flag);      // such an entry is not moved
+        else if (s != d) {
+            const int sp = page_of(p, b, s / kPage), dp = page_of(p, b, d / kPage), m = atomicAdd(&n_moves, 1);
+            src_page[m] = sp; src_slot[m] = s & (kPage - 1);
+            dst_page[m] = dp; dst_slot[m] = d & (kPage - 1);
+        }
+    }
+    __syncthreads();
+    const int n = n_moves;
+    T* ks = reinterpret_cast<T*>(raw);                    // [n][dk]
+    T* vs = ks + (long)n * y.dk;                          // [dv][n]
+    auto k_at = [&](int page, int slot) { return (T*)y.k + (((long)page * y.hkv + g) * kPage + slot) * y.dk; };
+    auto v_at = [&](int page, int slot) { return (T*)y.v + ((long)page * y.hkv + g) * y.dv * kPage + slot; };
+    const int vec = y.dk * (int)sizeof(T) / 16;
+    for (int e = tid; e < n * vec; e += 256) {
+        const int i = e / vec, c = e % vec;
+        reinterpret_cast<uint4*>(ks + (long)i * y.dk)[c] = reinterpret_cast<const uint4*>(k_at(src_page[i], src_slot[i]))[c];
+    }
+    for (int e = tid; e < n * y.dv; e += 256) {
+        const int d = e / n, i = e - d * n;
+        vs[e] = v_at(src_page[i], src_slot[i])[(long)d * kPage];
+    }
+    __syncthreads();
+    for (int e = tid; e < n * vec; e += 256) {
+        const int i = e / vec, c = e % vec;
+        reinterpret_cast<uint4*>(k_at(dst_page[i], dst_slot[i]))[c] = reinterpret_cast<const uint4*>(ks + (long)i * y.dk)[c];
+    }
+    for (int e = tid; e < n * y.dv; e += 256) {
+        const int d = e / n, i = e - d * n;
+        v_at(dst_page[i], dst_slot[i])[(long)d * kPage] = vs[e];
+    }
+}
+
+template <class T> int run_keep(const KeepArgs& a, int layers, int heads, int widest, cudaStream_t st) {
+    const size_t smem = (size_t)a.most * widest * sizeof(T);
+    auto kern = kv_keep_kernel<T>;
+    TRY_RC(allow_shared(kern, smem));
+    launch_k(kern, dim3(a.seq.B, heads, layers), dim3(256), smem, st, a);
+    return launch_status();
+}
+
+bool pages_ok(const flexllm_kv_pages* kv) {
+    return kv && kv->k && kv->v && aligned(kv->k, 16) && aligned(kv->v, 16) && kv->n_pages > 0 && kv->hkv > 0 && kv->kdim > 0 && kv->vdim > 0;
+}
+bool dims_ok(const flexllm_kv_pages* kv) { return kv->kdim % 8 == 0 && kv->vdim % 8 == 0 && kv->kdim <= 256 && kv->vdim <= 256; }
+
+}  // namespace
+
+}  // namespace flexllm
+
+using namespace flexllm;
+
+extern "C" int flexllm_qk_norm_rope(int dtype, const flexllm_kv_pages* kv, int heads, const void* proj, long ldp, const float* q_gain, const float* k_gain,
+                                    float eps, const int32_t* pos, int axes, const int* sections_host, const float* cos_t, const float* sin_t, int rot,
+                                    int table_len, const int32_t* cu, const int32_t* ctx, const int32_t* page_table, int max_pages, int max_ctx, int B,
+                                    int T, void* q, long ldq, void* stream) {
+    FLEXLLM_REQUIRE(dtype == FLEXLLM_F32 || dtype == FLEXLLM_BF16);
+    FLEXLLM_REQUIRE(pages_ok(kv) && heads > 0 && eps >= 0.0f);
+    RopeArgs a = {};
+    a.seq = {cu, ctx, page_table, max_pages, max_ctx, B, T, kv->n_pages, 0x7fffffff, nullptr};
+    a.H = heads; a.G = kv->hkv; a.dk = kv->kdim; a.dv = kv->vdim; a.rot = rot;
+    const long per16 = dtype == FLEXLLM_BF16 ? 8 : 4;
+    FLEXLLM_REQUIRE(packed_ok(a.seq) && ldp >= (long)(a.H + a.G) * a.dk + (long)a.G * a.dv && ldq >= (long)a.H * a.dk && ldp % per16 == 0 && ldq % per16 == 0);
+    FLEXLLM_REQUIRE(rot >= 0 && rot <= a.dk && axes >= 1 && axes <= 4 && (axes == 1 || sections_host) && (rot == 0 || (cos_t && sin_t && table_len > 0)));
+    if (!dims_ok(kv) || rot % 8) return FLEXLLM_ENOTSUP;
+    int end = 0;
+    for (int i = 0; i < axes; i++) {
+        const int n = axes == 1 ? rot / 2 : sections_host[i];
+        FLEXLLM_REQUIRE(n >= 0 && n <= rot / 2 - end);
+        end += n;
+        a.sec_end[i] = end;
+    }
+    FLEXLLM_REQUIRE(end == rot / 2);
+    if (T == 0) return FLEXLLM_OK;
+    FLEXLLM_REQUIRE(proj && q && (rot == 0 || pos) && aligned(proj, 16) && aligned(q, 16) && aligned(q_gain, 16) && aligned(k_gain, 16));
+    a.proj = proj; a.ldp = ldp; a.q_gain = q_gain; a.k_gain = k_gain; a.eps = eps; a.pos = pos; a.axes = axes;
+    a.cos_t = cos_t; a.sin_t = sin_t; a.table_len = table_len; a.k = kv->k; a.v = kv->v; a.q = q; a.ldq = ldq;
+    a.seq.error_flag = device_error_flag();
+    const SetUpEarly early;
+    return dtype == FLEXLLM_BF16 ? run_rope<bf16>(a, (cudaStream_t)stream) : run_rope<float>(a, (cudaStream_t)stream);
+}
+
+extern "C" int flexllm_kv_keep(int dtype, const flexllm_kv_pages* layers_host, int layers, const int32_t* page_table, int max_pages, const int32_t* ctx,
+                               int max_ctx, const int32_t* keep, const int32_t* count, int most, int B, void* stream) {
+    FLEXLLM_REQUIRE(dtype == FLEXLLM_F32 || dtype == FLEXLLM_BF16);
+    FLEXLLM_REQUIRE(layers_host && layers > 0 && most >= 0 && B > 0 && B <= 0x7fffffff && page_table && ctx && max_pages > 0 && max_ctx >= 0 &&
+                    (long)max_ctx < (long)max_pages * kPage);
+    if (most > 64) return FLEXLLM_ENOTSUP;
+    for (int i = 0; i < layers; i++) {
+        FLEXLLM_REQUIRE(pages_ok(layers_host + i));
+        if (!dims_ok(layers_host + i) || layers_host[i].hkv > 65535) return FLEXLLM_ENOTSUP;
+    }
+    if (most == 0) return FLEXLLM_OK;
+    FLEXLLM_REQUIRE(keep && count);
+    const SetUpEarly early;
+    for (int l0 = 0; l0 < layers; l0 += kKeepLayers) {
+        const int n = layers - l0 < kKeepLayers ? layers - l0 : kKeepLayers;
+        KeepArgs a = {};
+        a.seq = {nullptr, ctx, page_table, max_pages, max_ctx, B, 0, 0, 0, device_error_flag()};
+        a.keep = keep; a.count = count; a.most = most;
+        int heads = 0, widest = 0;
+        for (int i = 0; i < n; i++) {
+            const flexllm_kv_pages& p = layers_host[l0 + i];
+            a.layer[i] = {p.k, p.v, p.hkv, p.kdim, p.vdim, p.n_pages};
+            heads = p.hkv > heads ? p.hkv : heads;
+            widest = p.kdim + p.vdim > widest ? p.kdim + p.vdim : widest;
+        }
+        TRY_RC(dtype == FLEXLLM_BF16 ? run_keep<bf16>(a, n, heads, widest, (cudaStream_t)stream) : run_keep<float>(a, n, heads, widest, (cudaStream_t)stream));
+    }
+    return FLEXLLM_OK;
+}

@@ -374,6 +374,187 @@ class WindowAttention:
         return out
 
 
+# ------------------------------------------------------------------------------ packed sequences over the paged cache
+# Sequence b of a call has the packed rows cu[b] .. cu[b+1] - 1 at the cache positions ctx[b] .. of the pages page_table[b]. Pages are tensors
+# k_pages [n_pages,kv heads,64,dim] and v_pages [n_pages,kv heads,vdim,64] (bf16 or fp32, like the rows): the caller's, or a layer of a PagedKV.
+# cu [B+1], ctx [B] and page_table [B,max_pages] are int32. max_ctx: largest cache position of the call (default: what the table covers).
+# Calls run on the tensors' device, on its current stream.
+_DTYPE = {torch.bfloat16: _lib.BF16, torch.float32: _lib.F32}
+
+
+def _same(like, dtype, *tensors):
+    """The tensors (None: none) are dense, of the type, and where `like` is."""
+    for t in tensors:
+        if t is not None and not (t.dtype is dtype and t.device == like.device and t.is_contiguous()):
+            raise ValueError("flexllm_b200: expected a contiguous %s tensor on %s, got %s on %s, strides %s" % (dtype, like.device, t.dtype, t.device, t.stride()))
+
+
+def _call_on(device, name, *args):
+    if device.index == torch.cuda.current_device():
+        return _call(name, *args)
+    with torch.cuda.device(device):
+        _call(name, *args)
+
+
+def _rows(t, dtype_of=None):
+    """Data pointer and row stride of [T, ...] with dense rows, CUDA, bf16 or fp32."""
+    if not t.is_cuda or t.dtype not in _DTYPE or (dtype_of is not None and (t.dtype is not dtype_of.dtype or t.device != dtype_of.device)):
+        raise ValueError("flexllm_b200: expected CUDA rows of bfloat16 or float32, all alike and on one device")
+    if t.dim() == 3 and t.numel() and (t.stride(2) != 1 or t.stride(1) != t.shape[2]) or t.dim() == 2 and t.numel() and t.stride(1) != 1 or t.dim() not in (2, 3):
+        raise ValueError("flexllm_b200: rows have to be dense, got strides %s" % (t.stride(),))
+    width = t.shape[1] if t.dim() == 2 else t.shape[1] * t.shape[2]
+    return t.data_ptr(), t.stride(0) if t.shape[0] > 1 else width
+
+
+def _pages(k_pages, v_pages, like):
+    _same(like, like.dtype, k_pages, v_pages)
+    n, g, page, dim = k_pages.shape
+    if page != 64 or v_pages.shape[:2] != k_pages.shape[:2] or v_pages.shape[3] != 64:
+        raise ValueError("flexllm_b200: pages are K [n,heads,64,dim] and V [n,heads,vdim,64], got %s and %s" % (tuple(k_pages.shape), tuple(v_pages.shape)))
+    return _lib.KvPages(k_pages.data_ptr(), v_pages.data_ptr(), n, g, dim, v_pages.shape[2])
+
+
+def _packed(like, page_table, cu, ctx, max_ctx):
+    _same(like, torch.int32, page_table, cu, ctx)
+    B, max_pages = page_table.shape
+    if cu.numel() != B + 1 or ctx.numel() != B:
+        raise ValueError("flexllm_b200: %d sequences in the page table, cu has %d and ctx %d entries" % (B, cu.numel(), ctx.numel()))
+    return max_pages, max_pages * 64 - 1 if max_ctx is None else max_ctx, B
+
+
+class PagedKV:
+    """A floating-point paged cache owned by the library: shapes [(kv heads, dim, vdim)] per layer. k[l] and v[l] are its pages as tensors."""
+
+    def __init__(self, n_pages, shapes, dtype=torch.bfloat16, device="cuda"):
+        self._h = C.c_void_p()
+        dev = torch.empty(0, device=device).device
+        size = 2 if dtype == torch.bfloat16 else 4
+        kv = (_lib.KvShape * len(shapes))(*[_lib.KvShape(*s) for s in shapes])
+        with torch.cuda.device(dev):
+            _check("flexllm_kv_cache_create_float", lib().flexllm_kv_cache_create_float(C.byref(self._h), len(shapes), n_pages, kv, 64, size))
+        self.k, self.v = [], []
+        for layer, (g, dim, vdim) in enumerate(shapes):
+            p = _lib.KvPages()
+            _check("flexllm_kv_cache_pages", lib().flexllm_kv_cache_pages(self._h, layer, C.byref(p)))
+            self.k.append(_wrap(p.k, (n_pages, g, 64, dim), dtype, dev))
+            self.v.append(_wrap(p.v, (n_pages, g, vdim, 64), dtype, dev))
+
+    def close(self):
+        if self._h:
+            self.k, self.v = [], []
+            lib().flexllm_kv_cache_destroy(self._h)
+            self._h = C.c_void_p()
+
+
+def _wrap(ptr, shape, dtype, device):
+    """Device memory of the library as a tensor (bfloat16 has no type string: as int16, seen as bfloat16)."""
+    class _H:
+        pass
+    h = _H()
+    h.__cuda_array_interface__ = {"shape": tuple(shape), "typestr": "<i2" if dtype == torch.bfloat16 else "<f4", "data": (ptr, False), "version": 2}
+    t = torch.as_tensor(h, device=device)
+    return t.view(torch.bfloat16) if dtype == torch.bfloat16 else t
+
+
+def qk_norm_rope(proj, heads, pos, cos_t, sin_t, k_pages, v_pages, page_table, cu, ctx, q_gain=None, k_gain=None, eps=1e-6, sections=None, max_ctx=None,
+                 out=None):
+    """proj [T, q heads | k heads | v heads]: q and k normed head by head (q_gain, k_gain [dim] fp32; None: not), turned by the tables cos_t, sin_t
+    [P, rot/2] fp32 at the positions pos [T] or [axes,T] int32 (sections: pairs of each axis), k and v appended to the pages. Returns q [T, heads*dim]."""
+    p, ldp = _rows(proj)
+    T = proj.shape[0]
+    kv = _pages(k_pages, v_pages, proj)
+    max_pages, max_ctx, B = _packed(proj, page_table, cu, ctx, max_ctx)
+    _same(proj, torch.float32, cos_t, sin_t, q_gain, k_gain)
+    _same(proj, torch.int32, pos)
+    axes = pos.shape[0] if pos.dim() == 2 else 1
+    if proj.shape[1] != (heads + kv.hkv) * kv.kdim + kv.hkv * kv.vdim or pos.numel() != axes * T or (axes > 1 and (sections is None or len(sections) != axes)):
+        raise ValueError("flexllm_b200: qk_norm_rope: the widths of proj, pos and sections do not fit %d heads" % heads)
+    if cos_t.dim() != 2 or cos_t.shape != sin_t.shape or any(x is not None and x.numel() != kv.kdim for x in (q_gain, k_gain)):
+        raise ValueError("flexllm_b200: qk_norm_rope: tables are [P, rot/2], gains [dim]")
+    q = torch.empty((T, heads * kv.kdim), dtype=proj.dtype, device=proj.device) if out is None else out
+    qp, ldq = _rows(q, proj)
+    if q.dim() != 2 or q.shape[0] != T or q.shape[1] != heads * kv.kdim:
+        raise ValueError("flexllm_b200: out has to be [%d,%d]" % (T, heads * kv.kdim))
+    sec = None if sections is None else (C.c_int * axes)(*sections)
+    _call_on(proj.device, "flexllm_qk_norm_rope", _DTYPE[proj.dtype], C.byref(kv), heads, p, ldp, _ptr(q_gain), _ptr(k_gain), eps, pos.data_ptr(), axes, sec,
+             cos_t.data_ptr(), sin_t.data_ptr(), 2 * cos_t.shape[1], cos_t.shape[0], cu.data_ptr(), ctx.data_ptr(), page_table.data_ptr(), max_pages, max_ctx,
+             B, T, qp, ldq)
+    return q
+
+
+def _attn_paged(name, q, mask, k_pages, v_pages, page_table, cu, ctx, scale, max_ctx, out):
+    p, ldq = _rows(q)
+    if q.dim() != 3:
+        raise ValueError("flexllm_b200: q is [T,heads,dim]")
+    T, heads, dim = q.shape
+    kv = _pages(k_pages, v_pages, q)
+    max_pages, max_ctx, B = _packed(q, page_table, cu, ctx, max_ctx)
+    if kv.kdim != dim:
+        raise ValueError("flexllm_b200: heads of %d over pages of %d" % (dim, kv.kdim))
+    if out is None:
+        out = torch.empty((T, heads * kv.vdim), dtype=q.dtype, device=q.device)
+    o, ldo = _rows(out, q)
+    if out.dim() != 2 or out.shape[0] != T or out.shape[1] != heads * kv.vdim:
+        raise ValueError("flexllm_b200: out has to be [%d,%d]" % (T, heads * kv.vdim))
+    _call_on(q.device, name, _DTYPE[q.dtype], C.byref(kv), heads, dim ** -0.5 if scale is None else scale, p, ldq, *mask, cu.data_ptr(), ctx.data_ptr(),
+             page_table.data_ptr(), max_pages, max_ctx, B, T, o, ldo)
+    return out
+
+
+def attn_packed(q, k_pages, v_pages, page_table, cu, ctx, scale=None, max_ctx=None, out=None):
+    """Causal attention of packed rows q [T,heads,dim] (dense rows, any row stride of whole 16 bytes) over their sequences' pages, which hold the new
+    keys and values already: row i of sequence b sees the positions 0 .. ctx[b] + i. scale: 1/sqrt(dim). Returns [T, heads*vdim]; rows of `out` from
+    cu[B] on are left alone."""
+    return _attn_paged("flexllm_attn_packed", q, (), k_pages, v_pages, page_table, cu, ctx, scale, max_ctx, out)
+
+
+def attn_tree(q, mask, k_pages, v_pages, page_table, cu, ctx, scale=None, max_ctx=None, out=None):
+    """Attention of trees of up to 64 drafted tokens per sequence: a row sees the ctx[b] cached positions and the new tokens whose bit is set in
+    mask [T] int64 (bit j: token j of the sequence). Everything else as in attn_packed."""
+    _same(q, torch.int64, mask)
+    if mask.numel() != q.shape[0]:
+        raise ValueError("flexllm_b200: attn_tree: %d rows, %d masks" % (q.shape[0], mask.numel()))
+    return _attn_paged("flexllm_attn_tree", q, (mask.data_ptr(),), k_pages, v_pages, page_table, cu, ctx, scale, max_ctx, out)
+
+
+def kv_keep(layers, page_table, ctx, keep, count, max_ctx=None):
+    """The accepted tokens of every tree moved together in all layers [(k_pages, v_pages), ...]: the entries at ctx[b] + keep[b,i] become those at
+    ctx[b] + i for i < count[b]. keep [B,most] int32 in [0,64), count [B] int32."""
+    if not layers:
+        raise ValueError("flexllm_b200: kv_keep: no layers")
+    k0 = layers[0][0]
+    if not k0.is_cuda or k0.dtype not in _DTYPE:
+        raise ValueError("flexllm_b200: expected CUDA pages of bfloat16 or float32")
+    kv = (_lib.KvPages * len(layers))(*[_pages(k, v, k0) for k, v in layers])
+    _same(k0, torch.int32, page_table, ctx, keep, count)
+    B, max_pages = page_table.shape
+    if ctx.numel() != B or count.numel() != B or keep.dim() != 2 or keep.shape[0] != B:
+        raise ValueError("flexllm_b200: kv_keep: page_table, ctx, keep and count are for different numbers of sequences")
+    _call_on(k0.device, "flexllm_kv_keep", _DTYPE[k0.dtype], kv, len(layers), page_table.data_ptr(), max_pages, ctx.data_ptr(),
+             max_pages * 64 - 1 if max_ctx is None else max_ctx, keep.data_ptr(), count.data_ptr(), keep.shape[1], B)
+
+
+def linear_w4(x, w, scale, zero=None, bias=None, out_f32=False, out=None):
+    """x [M,K] (bf16 or fp32) times 4-bit weights w [N,K/2] uint8 (low nibble: even column), scale [N,K/group] bf16 or fp32, zero points zero [N,K/group]
+    uint8 (None: 8), bias [N] fp32. Returns [M,N] of x's type, or fp32."""
+    p, lda = _rows(x)
+    (M, K), N = x.shape, w.shape[0]
+    if scale.dtype not in _DTYPE or scale.dim() != 2 or scale.shape[0] != N or scale.shape[1] == 0 or K % scale.shape[1] or w.shape[1] * 2 != K:
+        raise ValueError("flexllm_b200: linear_w4: w [N,K/2] and scale [N,K/group] do not fit x [M,K]")
+    if zero is not None and zero.shape != scale.shape or bias is not None and bias.numel() != N:
+        raise ValueError("flexllm_b200: linear_w4: zero is [N,K/group], bias [N]")
+    _same(x, torch.uint8, w, zero)
+    _same(x, scale.dtype, scale)
+    _same(x, torch.float32, bias)
+    y = torch.empty((M, N), dtype=torch.float32 if out_f32 else x.dtype, device=x.device) if out is None else out
+    if y.dim() != 2 or y.shape[0] != M or y.shape[1] != N or y.dtype is not (torch.float32 if out_f32 else x.dtype):
+        raise ValueError("flexllm_b200: linear_w4: out has to be [%d,%d] %s" % (M, N, torch.float32 if out_f32 else x.dtype))
+    yp, ldy = _rows(y)
+    _call_on(x.device, "flexllm_linear_w4", _DTYPE[x.dtype], p, lda, w.data_ptr(), scale.data_ptr(), _DTYPE[scale.dtype], _ptr(zero), K // scale.shape[1],
+             _ptr(bias), M, N, K, yp, ldy, 1 if out_f32 else 0)
+    return y
+
+
 # ------------------------------------------------------------------------------ MHA_i8xi8
 def MHA_i8xi8_Prefilling(q, qs, k, ks, v, vs, cos_t, sin_t, a_s, want_oacc=False):
     """Prefill GQA attention. q [B,S,HQ,64] s8, qs [B,S,HQ]; k,v [B,S,HKV,64], ks,vs [B,S,HKV];

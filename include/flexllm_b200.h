@@ -455,6 +455,56 @@ FLEXLLM_API int flexllm_attn_window(int dtype, flexllm_kv_cache* c, int layer, c
                                     long ldo, void* workspace, size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * Packed sequences over a floating-point paged cache (no counterpart in the reference): what a layer runs between its projections when a step
+ * serves prompts of different lengths, or trees of drafted tokens (speculative decoding).
+ * A call has T packed rows; sequence b < B has the rows cu[b] .. cu[b+1] - 1 (cu [B+1], cu[0] = 0; a sequence may have none, rows from cu[B] on are
+ * left alone) at the cache positions ctx[b] .. of its pages page_table[b][0 ..] (max_pages per sequence; entries behind its last position are
+ * not looked at). max_ctx: largest position of the call, < 64 * max_pages. cu, ctx, page_table, pos, keep and count are device memory;
+ * values out of range are clamped and reported by flexllm_device_status() (FLEXLLM_EDEVDATA). Element type FLEXLLM_BF16 or FLEXLLM_F32 for
+ * rows and pages alike; scores, norms, weights and sums are fp32. kdim and vdim multiples of 8 up to 256 (else FLEXLLM_ENOTSUP).
+ * ------------------------------------------------------------------------------------------- */
+/* One layer's pages of 64 tokens, K [n_pages][hkv][64][kdim] and V [n_pages][hkv][vdim][64], 16-byte aligned: memory of the caller, or a layer of a
+ * cache made by flexllm_kv_cache_create_float, which flexllm_kv_cache_pages describes. */
+typedef struct { void *k, *v; int n_pages, hkv, kdim, vdim; } flexllm_kv_pages;
+FLEXLLM_API int flexllm_kv_cache_pages(flexllm_kv_cache* c, int layer, flexllm_kv_pages* out);
+
+/* Norm of q and k head by head, rotation, append:
+ *   y = x / sqrt(mean x^2 + eps) * gain  (q_gain, k_gain [kdim] fp32, either NULL: no norm for that side)
+ *   pair p < rot/2 turns y[p] and y[p + rot/2] by the angle with cosine cos_t[pos_a][p] and sine sin_t[pos_a][p], a the axis of the pair
+ * proj [T][ldp]: q heads | k heads | v heads. pos [axes][T]: positions of the rows (time, height, width, ...), 1 to 4 axes; sections_host[axes]: pairs
+ * that follow each axis, in order, adding up to rot/2 (NULL with one axis). cos_t, sin_t [table_len][rot/2] fp32; rot a multiple of 8 up to
+ * kdim (0: no rotation), the elements behind it only normed. q [T][ldq] receives the q heads, the pages the keys and values. Row strides are
+ * multiples of 16 bytes, pointers 16-byte aligned. */
+FLEXLLM_API int flexllm_qk_norm_rope(int dtype, const flexllm_kv_pages* kv, int heads, const void* proj, long ldp, const float* q_gain, const float* k_gain,
+                                     float eps, const int32_t* pos, int axes, const int* sections_host, const float* cos_t, const float* sin_t, int rot,
+                                     int table_len, const int32_t* cu, const int32_t* ctx, const int32_t* page_table, int max_pages, int max_ctx, int B,
+                                     int T, void* q, long ldq, void* stream);
+
+/* Causal attention of the packed rows over their sequences' pages, which hold the keys and values of all their positions (the new ones
+ * included): row i of sequence b sees the positions 0 .. ctx[b] + i. heads a multiple of hkv. q [T][ldq] (heads side by side, row stride a
+ * multiple of 16 bytes), out [T][ldo]. What a row does not see has no influence on it, not finite values included. */
+FLEXLLM_API int flexllm_attn_packed(int dtype, const flexllm_kv_pages* kv, int heads, float scale, const void* q, long ldq, const int32_t* cu,
+                                    const int32_t* ctx, const int32_t* page_table, int max_pages, int max_ctx, int B, int T, void* out, long ldo,
+                                    void* stream);
+/* The same for trees of up to 64 drafted tokens per sequence: a row sees the ctx[b] cached positions and, of its sequence's new tokens, those whose bit
+ * is set in mask[row] (bit j: token j; a token that sees itself has its own bit set). A row that sees nothing is zero. */
+FLEXLLM_API int flexllm_attn_tree(int dtype, const flexllm_kv_pages* kv, int heads, float scale, const void* q, long ldq, const uint64_t* mask,
+                                  const int32_t* cu, const int32_t* ctx, const int32_t* page_table, int max_pages, int max_ctx, int B, int T, void* out,
+                                  long ldo, void* stream);
+/* The accepted tokens of every tree moved together, in all `layers` layers: the entries at ctx[b] + keep[b][i] become those at ctx[b] + i,
+ * i < count[b] <= most <= 64, keep [B][most] in [0, 64) in any order. An entry out of range stays where it is and is reported. */
+FLEXLLM_API int flexllm_kv_keep(int dtype, const flexllm_kv_pages* layers_host, int layers, const int32_t* page_table, int max_pages, const int32_t* ctx,
+                                int max_ctx, const int32_t* keep, const int32_t* count, int most, int B, void* stream);
+
+/* Product with 4-bit weights: y[m][n] = sum_k a[m][k] (q[n][k] - z[n][k/group]) s[n][k/group] (+ bias[n]).
+ * a [M][lda] of type dtype, lda a multiple of 8 and >= K; w [N][K/2]: element k of a row in the low (k even) or high nibble of byte k/2; scale [N][K/group]
+ * of type scale_dtype (FLEXLLM_BF16 or FLEXLLM_F32); zero [N][K/group] one value of 0 .. 15 per byte, NULL: 8 throughout; bias [N] fp32 or NULL.
+ * group a multiple of 32 that divides K. y [M][ldy] of type dtype, or fp32 (y_f32). Made for few tokens, where the weights' bytes are the cost;
+ * any M is taken, 64 tokens at a time. Nothing is rounded to fewer than 32 bits but y. */
+FLEXLLM_API int flexllm_linear_w4(int dtype, const void* a, long lda, const uint8_t* w, const void* scale, int scale_dtype, const uint8_t* zero, int group,
+                                  const float* bias, int M, int N, int K, void* y, long ldy, int y_f32, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
  * HMT long-context plug-in (Modules/HMT.h; HMT_SpinQuant_Llama_32_1B/): the prompt is processed in segments of seg_len
  * tokens through the same prefill path; per segment a summary pass over [T, first sum_len tokens, T] queries a ring of
  * mem_num memory vectors by fp32 cross-attention (Q = Wq S, keys Wk M, dec_Softmax with scale sqrt(hidden)) for the
