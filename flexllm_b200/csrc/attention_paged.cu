@@ -23,10 +23,8 @@ __device__ __forceinline__ void copy16(float* dst, const float* src) {
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-__device__ __forceinline__ void put4(float* dst, const float* src) { copy16(dst, src); }
-__device__ __forceinline__ void put4(float* dst, const bf16* src) { store4(dst, load4(src)); }
 
-template <class T, int RT, int NV>
+template <int RT, int NV>
 __global__ void __launch_bounds__(256) attn_paged_simt_kernel(const __grid_constant__ SimtArgs sa, int n_split) {
     constexpr int RR = RT / 16;           // rows per thread
     extern __shared__ __align__(16) float sm[];
@@ -69,28 +67,28 @@ __global__ void __launch_bounds__(256) attn_paged_simt_kernel(const __grid_const
     for (int e = tid; e < RT * (a.dk / 4); e += 256) {
         const int row = e / (a.dk / 4), c = (e - row * (a.dk / 4)) * 4, i = i0 + row / sa.RC;
         const bool on = row < sa.TQ * sa.RC && i < s.n && row % sa.RC < heads;
-        if (on) put4(q_sm + row * DP + c, (const T*)a.q + (long)(s.row0 + i) * a.ldq + (long)(h0 + row % sa.RC) * a.dk + c);
+        if (on) copy16(q_sm + row * DP + c, (const float*)a.q + (long)(s.row0 + i) * a.ldq + (long)(h0 + row % sa.RC) * a.dk + c);
         else store4(q_sm + row * DP + c, make_float4(0.0f, 0.0f, 0.0f, 0.0f));
     }
     auto load_k = [&](int t) {
-        const T* kp = (const T*)a.k + ((long)page_of(a.seq, b, t) * a.G + g) * kPage * a.dk;
+        const float* kp = (const float*)a.k + ((long)page_of(a.seq, b, t) * a.G + g) * kPage * a.dk;
         for (int e = tid; e < kPage * (a.dk / 4); e += 256) {
             const int key = e / (a.dk / 4), c = (e - key * (a.dk / 4)) * 4;
-            put4(k_sm + key * DP + c, kp + (long)key * a.dk + c);
+            copy16(k_sm + key * DP + c, kp + (long)key * a.dk + c);
         }
         copies_commit();
     };
     // keys from `end` on were never written: zeros in their place, so that a weight of zero stays without effect
     auto load_v = [&](int t) {
-        const T* vp = (const T*)a.v + ((long)page_of(a.seq, b, t) * a.G + g) * a.dv * kPage;
+        const float* vp = (const float*)a.v + ((long)page_of(a.seq, b, t) * a.G + g) * a.dv * kPage;
         const int left = end - t * kPage;
         for (int e = tid; e < a.dv * (kPage / 4); e += 256) {
             const int d = e / (kPage / 4), c = (e % (kPage / 4)) * 4;
-            const T* src = vp + (long)d * kPage + c;
+            const float* src = vp + (long)d * kPage + c;
             float* dst = v_sm + d * PPITCH + c;
-            if (c + 4 <= left) put4(dst, src);
+            if (c + 4 <= left) copy16(dst, src);
             else
-                for (int x = 0; x < 4; x++) dst[x] = c + x < left ? to_f(src[x]) : 0.0f;
+                for (int x = 0; x < 4; x++) dst[x] = c + x < left ? src[x] : 0.0f;
         }
         copies_commit();
     };
@@ -208,22 +206,22 @@ __global__ void __launch_bounds__(256) attn_paged_simt_kernel(const __grid_const
         }
         v = sum == 0.0f ? 0.0f : v / sum;
         if (not_finite(v)) atomicOr(&redo_sm[row >> 5], 1u << (row & 31));
-        ((T*)a.out)[(long)(s.row0 + i0 + row / sa.RC) * a.ldo + (long)(h0 + row % sa.RC) * a.dv + d] = from_f<T>(v);
+        ((float*)a.out)[(long)(s.row0 + i0 + row / sa.RC) * a.ldo + (long)(h0 + row % sa.RC) * a.dv + d] = v;
     }
     if (n_split > 1) cluster_sync(); else __syncthreads();
     if (redo_sm[0] | redo_sm[1])
         for (int row = tid >> 5; row < rows; row += 8)
-            if (redo_sm[row >> 5] >> (row & 31) & 1) attn_row_by_key<T>(a, b, s, i0 + row / sa.RC, h0 + row % sa.RC);
+            if (redo_sm[row >> 5] >> (row & 31) & 1) attn_row_by_key<float>(a, b, s, i0 + row / sa.RC, h0 + row % sa.RC);
 }
 
-template <class T, int RT, int NV> int launch_simt(const SimtArgs& sa, int tiles, int splits, cudaStream_t st) {
+template <int RT, int NV> int launch_simt(const SimtArgs& sa, int tiles, int splits, cudaStream_t st) {
     const size_t smem = simt_floats(RT, sa.a.dk, NV * 16) * 4;
-    auto kern = attn_paged_simt_kernel<T, RT, NV>;
+    auto kern = attn_paged_simt_kernel<RT, NV>;
     TRY_RC(allow_shared(kern, smem));
     launch_cluster(kern, dim3(tiles * splits, sa.a.G * sa.HC), dim3(256), splits, smem, st, sa, splits);
     return launch_status();
 }
-template <class T, int RT> int run_simt(const PagedAttn& a, cudaStream_t st) {
+template <int RT> int run_simt(const PagedAttn& a, cudaStream_t st) {
     SimtArgs sa;
     const int R = a.H / a.G;
     sa.a = a;
@@ -231,19 +229,17 @@ template <class T, int RT> int run_simt(const PagedAttn& a, cudaStream_t st) {
     const long tiles = a.seq.T / sa.TQ + (a.seq.B < a.seq.T ? a.seq.B : a.seq.T);
     const int splits = key_splits(tiles * a.G * sa.HC, (a.seq.max_ctx + kPage) / kPage, 2);
     if (tiles * splits > 0x7fffffffL || a.G * sa.HC > 65535) return FLEXLLM_ENOTSUP;
-    if (a.dv <= 64) return launch_simt<T, RT, 4>(sa, (int)tiles, splits, st);
-    if (a.dv <= 128) return launch_simt<T, RT, 8>(sa, (int)tiles, splits, st);
-    return launch_simt<T, RT, 16>(sa, (int)tiles, splits, st);
+    if (a.dv <= 64) return launch_simt<RT, 4>(sa, (int)tiles, splits, st);
+    if (a.dv <= 128) return launch_simt<RT, 8>(sa, (int)tiles, splits, st);
+    return launch_simt<RT, 16>(sa, (int)tiles, splits, st);
 }
 
 }  // namespace
 
-template <class T> int attn_paged_simt(const PagedAttn& a, cudaStream_t st) {
+int attn_paged_simt(const PagedAttn& a, cudaStream_t st) {
     const long rows = (long)(a.seq.T / a.seq.B) * (a.H / a.G);          // of an average sequence and a key/value head
-    return rows <= 16 ? run_simt<T, 16>(a, st) : run_simt<T, 64>(a, st);
+    return rows <= 16 ? run_simt<16>(a, st) : run_simt<64>(a, st);
 }
-template int attn_paged_simt<float>(const PagedAttn&, cudaStream_t);
-template int attn_paged_simt<bf16>(const PagedAttn&, cudaStream_t);
 
 namespace {
 int attn_paged(int dtype, const flexllm_kv_pages* kv, int heads, float scale, const void* q, long ldq, const uint64_t* mask, const int32_t* cu,
@@ -255,13 +251,13 @@ int attn_paged(int dtype, const flexllm_kv_pages* kv, int heads, float scale, co
     a.H = heads; a.G = kv->hkv; a.dk = kv->kdim; a.dv = kv->vdim;
     a.scale = scale; a.q = q; a.ldq = ldq; a.mask = (const unsigned long long*)mask; a.k = kv->k; a.v = kv->v; a.out = out; a.ldo = ldo;
     const long per16 = dtype == FLEXLLM_BF16 ? 8 : 4;                   // elements of 16 bytes
-    FLEXLLM_REQUIRE(packed_ok(a.seq) && ldq >= (long)heads * a.dk && ldo >= (long)heads * a.dv && ldq % per16 == 0 && scale == scale);
+    FLEXLLM_REQUIRE(packed_ok(a.seq) && ldq >= (long)heads * a.dk && ldo >= (long)heads * a.dv && ldq % per16 == 0 && scale >= 0.0f && scale <= 1e30f);
     if (a.dk % 8 || a.dv % 8 || a.dk > 256 || a.dv > 256) return FLEXLLM_ENOTSUP;
     if (T == 0) return FLEXLLM_OK;
     FLEXLLM_REQUIRE(q && out && aligned(q, 16) && aligned(kv->k, 16) && aligned(kv->v, 16) && aligned(out, dtype == FLEXLLM_BF16 ? 2 : 4));
     a.seq.error_flag = device_error_flag();
     const SetUpEarly early;
-    return dtype == FLEXLLM_BF16 ? attn_paged_simt<bf16>(a, (cudaStream_t)stream) : attn_paged_simt<float>(a, (cudaStream_t)stream);
+    return dtype == FLEXLLM_BF16 ? attn_paged_tc(a, (cudaStream_t)stream) : attn_paged_simt(a, (cudaStream_t)stream);
 }
 }  // namespace
 

@@ -64,6 +64,7 @@ template <class T> __device__ __noinline__ void attn_row_by_key(const PagedAttn&
     for (int e = 0; e < 8; e++)
         if (lane + 32 * e < a.dv) out[lane + 32 * e] = from_f<T>(l == 0.0f ? 0.0f : o[e] / l);
 }
+__device__ __forceinline__ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 __device__ __forceinline__ bool not_finite(float v) { return !(fabsf(v) <= 3.402823466e38f); }
 
 // CTAs of a cluster among which a tile's keys are cut, for `tiles` (tile, head) pairs of up to `pages` key pages each: while there are SMs
@@ -74,6 +75,7 @@ inline int key_splits(long tiles, int pages, int least) {
     return s;
 }
 
-template <class T> int attn_paged_simt(const PagedAttn& a, cudaStream_t st);
+int attn_paged_simt(const PagedAttn& a, cudaStream_t st);      // fp32
+int attn_paged_tc(const PagedAttn& a, cudaStream_t st);        // bf16, scale >= 0
 
 }  // namespace flexllm

@@ -87,12 +87,12 @@ int make_tmap_3d_u8(CUtensorMap* out, const void* base, uint64_t rows, uint64_t 
 }
 
 int make_tmap_rows3_u8(CUtensorMap* out, const void* base, uint64_t outer, uint64_t mid, uint64_t row_bytes, uint32_t box_outer,
-                       uint32_t box_mid) {
+                       uint32_t box_mid, uint64_t outer_bytes) {
     EncodeTiledFn fn = get_encode_fn();
     if (!fn) return FLEXLLM_ECUDA;
     if (!aligned(base, 16) || (row_bytes % 16) != 0 || box_outer == 0 || box_mid == 0 || box_outer > 256 || box_mid > 256) return FLEXLLM_EINVAL;
     cuuint64_t dims[3] = {row_bytes, mid, outer};
-    cuuint64_t strides[2] = {row_bytes, row_bytes * mid};
+    cuuint64_t strides[2] = {row_bytes, outer_bytes ? outer_bytes : row_bytes * mid};
     cuuint32_t box[3] = {128, box_mid, box_outer};
     cuuint32_t estr[3] = {1, 1, 1};
     CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(base), dims, strides, box, estr,

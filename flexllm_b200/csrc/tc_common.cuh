@@ -256,9 +256,9 @@ int make_tmap_2d_u8_box(CUtensorMap* out, const void* base, uint64_t rows, uint6
 // tiles back to back in shared memory, fetched as kch*128 contiguous bytes per row.
 int make_tmap_3d_u8(CUtensorMap* out, const void* base, uint64_t rows, uint64_t row_bytes, uint32_t box_rows, uint32_t kch);
 // Row-major [outer][mid] rows of row_bytes bytes (the rows of one `outer` index back to back): a box of {128 bytes, box_mid rows,
-// box_outer} lands as box_outer * box_mid standard 128-byte-swizzled rows, outer-major.
+// box_outer} lands as box_outer * box_mid standard 128-byte-swizzled rows, outer-major. outer_bytes: distance of two outer indices (0: mid rows).
 int make_tmap_rows3_u8(CUtensorMap* out, const void* base, uint64_t outer, uint64_t mid, uint64_t row_bytes, uint32_t box_outer,
-                       uint32_t box_mid);
+                       uint32_t box_mid, uint64_t outer_bytes = 0);
 // make_tmap_2d_u8 / make_tmap_3d_u8 (kch != 0) behind a cache keyed by pointer and shape
 int cached_tmap_u8(CUtensorMap* out, const void* base, uint64_t rows, uint64_t row_bytes, uint32_t box_rows, uint32_t kch);
 

@@ -62,6 +62,10 @@ CASES = [
     ([5, 6], [60, 130], 160, 1, 64, 128),
     ([700], [0], 4, 1, 8, 8),
     ([300, 260], [64, 0], 16, 2, 128, 64),
+    ([1300, 77, 1100], [0, 65, 3], 16, 16, 128, 128),
+    ([700, 0, 650], [100, 0, 0], 32, 8, 64, 64),
+    ([2500], [0], 40, 8, 96, 80),
+    ([1, 3000, 33], [700, 128, 1], 16, 8, 72, 128),
 ]
 
 
@@ -144,7 +148,7 @@ def test_strides_scale_and_rows_behind_the_last_sequence(ops, dtype):
     wide[:100, 16:16 + H * 64] = q.reshape(100, -1)
     qs = wide[:, 16:16 + H * 64].unflatten(1, (H, 64))
     out = torch.full((107, H * 64 + 24), 7.0, device="cuda").to(dtype)
-    for scale in (0.5, 0.0, -0.3):
+    for scale in (0.5, 0.0, 1.0):
         got = ops.attn_packed(qs, k, v, table.cuda(), start.cuda(), cx.cuda(), scale=scale, out=out[:, 8:8 + H * 64])
         want, far = pc.attention(q, k, v, table, start, cx, scale)
         near(got[:100], want, far)
