@@ -405,8 +405,8 @@ template <int NQ> int launch_tc(TcArgs& t, long tiles, cudaStream_t st) {
     t.tmem_cols = 512;                                    // two score tiles and the outputs: over 256 in any case
     CUtensorMap tq, tk, tv;
     TRY_RC(make_tmap_rows3_u8(&tq, a.q, (uint64_t)a.seq.T, (uint64_t)a.H, (uint64_t)a.dk * 2, (uint32_t)t.TQ, (uint32_t)t.RC, (uint64_t)a.ldq * 2));
-    TRY_RC(cached_tmap_u8(&tk, a.k, (uint64_t)a.seq.n_pages * a.G * kPage, (uint64_t)a.dk * 2, kPage, 0));
-    TRY_RC(cached_tmap_u8(&tv, a.v, (uint64_t)a.seq.n_pages * a.G * a.dv, kPage * 2, (uint32_t)t.vr, 0));
+    TRY_RC(make_tmap_2d_u8(&tk, a.k, (uint64_t)a.seq.n_pages * a.G * kPage, (uint64_t)a.dk * 2, kPage));
+    TRY_RC(make_tmap_2d_u8(&tv, a.v, (uint64_t)a.seq.n_pages * a.G * a.dv, kPage * 2, (uint32_t)t.vr));
     auto kern = attn_paged_tc_kernel<NQ>;
     TRY_RC(allow_shared(kern, o.total));
     launch_cluster(kern, dim3((unsigned)(tiles * t.n_split), a.G * t.HC), dim3(NQ * 128 + 64), t.n_split, o.total, st, tq, tk, tv, t);

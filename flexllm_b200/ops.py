@@ -49,7 +49,8 @@ def _bind_front_end():
             _front = False
         else:
             m.bind(*(C.cast(getattr(lib(), f), C.c_void_p).value for f in (
-                "flexllm_linear_prefill_i8", "flexllm_linear_decode_i8", "flexllm_mlp_block_workspace", "flexllm_mlp_block_decode")))
+                "flexllm_linear_prefill_i8", "flexllm_linear_decode_i8", "flexllm_mlp_block_workspace", "flexllm_mlp_block_decode",
+                "flexllm_qk_norm_rope", "flexllm_attn_packed", "flexllm_attn_tree", "flexllm_kv_keep", "flexllm_linear_w4")))
             _front = m
     return _front
 
@@ -460,6 +461,10 @@ def qk_norm_rope(proj, heads, pos, cos_t, sin_t, k_pages, v_pages, page_table, c
                  out=None):
     """proj [T, q heads | k heads | v heads]: q and k normed head by head (q_gain, k_gain [dim] fp32; None: not), turned by the tables cos_t, sin_t
     [P, rot/2] fp32 at the positions pos [T] or [axes,T] int32 (sections: pairs of each axis), k and v appended to the pages. Returns q [T, heads*dim]."""
+    if out is None and (_front or _bind_front_end()):
+        q = _front.qk_norm_rope(proj, heads, pos, cos_t, sin_t, k_pages, v_pages, page_table, cu, ctx, q_gain, k_gain, eps, sections, max_ctx)
+        if q is not None:
+            return _out("flexllm_qk_norm_rope", q)
     p, ldp = _rows(proj)
     T = proj.shape[0]
     kv = _pages(k_pages, v_pages, proj)
@@ -483,6 +488,16 @@ def qk_norm_rope(proj, heads, pos, cos_t, sin_t, k_pages, v_pages, page_table, c
 
 
 def _attn_paged(name, q, mask, k_pages, v_pages, page_table, cu, ctx, scale, max_ctx, out):
+    if scale is None:
+        scale = q.shape[-1] ** -0.5
+    if out is None and (_front or _bind_front_end()):
+        r = _front.attn_paged(q, mask, k_pages, v_pages, page_table, cu, ctx, scale, max_ctx)
+        if r is not None:
+            return _out(name, r)
+    if mask is not None:
+        _same(q, torch.int64, mask)
+        if mask.numel() != q.shape[0]:
+            raise ValueError("flexllm_b200: attn_tree: %d rows, %d masks" % (q.shape[0], mask.numel()))
     p, ldq = _rows(q)
     if q.dim() != 3:
         raise ValueError("flexllm_b200: q is [T,heads,dim]")
@@ -496,7 +511,7 @@ def _attn_paged(name, q, mask, k_pages, v_pages, page_table, cu, ctx, scale, max
     o, ldo = _rows(out, q)
     if out.dim() != 2 or out.shape[0] != T or out.shape[1] != heads * kv.vdim:
         raise ValueError("flexllm_b200: out has to be [%d,%d]" % (T, heads * kv.vdim))
-    _call_on(q.device, name, _DTYPE[q.dtype], C.byref(kv), heads, dim ** -0.5 if scale is None else scale, p, ldq, *mask, cu.data_ptr(), ctx.data_ptr(),
+    _call_on(q.device, name, _DTYPE[q.dtype], C.byref(kv), heads, scale, p, ldq, *(() if mask is None else (mask.data_ptr(),)), cu.data_ptr(), ctx.data_ptr(),
              page_table.data_ptr(), max_pages, max_ctx, B, T, o, ldo)
     return out
 
@@ -505,21 +520,24 @@ def attn_packed(q, k_pages, v_pages, page_table, cu, ctx, scale=None, max_ctx=No
     """Causal attention of packed rows q [T,heads,dim] (dense rows, any row stride of whole 16 bytes) over their sequences' pages, which hold the new
     keys and values already: row i of sequence b sees the positions 0 .. ctx[b] + i. scale: 1/sqrt(dim). Returns [T, heads*vdim]; rows of `out` from
     cu[B] on are left alone."""
-    return _attn_paged("flexllm_attn_packed", q, (), k_pages, v_pages, page_table, cu, ctx, scale, max_ctx, out)
+    return _attn_paged("flexllm_attn_packed", q, None, k_pages, v_pages, page_table, cu, ctx, scale, max_ctx, out)
 
 
 def attn_tree(q, mask, k_pages, v_pages, page_table, cu, ctx, scale=None, max_ctx=None, out=None):
     """Attention of trees of up to 64 drafted tokens per sequence: a row sees the ctx[b] cached positions and the new tokens whose bit is set in
     mask [T] int64 (bit j: token j of the sequence). Everything else as in attn_packed."""
-    _same(q, torch.int64, mask)
-    if mask.numel() != q.shape[0]:
-        raise ValueError("flexllm_b200: attn_tree: %d rows, %d masks" % (q.shape[0], mask.numel()))
-    return _attn_paged("flexllm_attn_tree", q, (mask.data_ptr(),), k_pages, v_pages, page_table, cu, ctx, scale, max_ctx, out)
+    if mask is None:
+        raise ValueError("flexllm_b200: attn_tree takes a mask for every row")
+    return _attn_paged("flexllm_attn_tree", q, mask, k_pages, v_pages, page_table, cu, ctx, scale, max_ctx, out)
 
 
 def kv_keep(layers, page_table, ctx, keep, count, max_ctx=None):
     """The accepted tokens of every tree moved together in all layers [(k_pages, v_pages), ...]: the entries at ctx[b] + keep[b,i] become those at
     ctx[b] + i for i < count[b]. keep [B,most] int32 in [0,64), count [B] int32."""
+    if _front or _bind_front_end():
+        r = _front.kv_keep(layers, page_table, ctx, keep, count, max_ctx)
+        if r is not None:
+            return _check("flexllm_kv_keep", r)
     if not layers:
         raise ValueError("flexllm_b200: kv_keep: no layers")
     k0 = layers[0][0]
@@ -537,6 +555,10 @@ def kv_keep(layers, page_table, ctx, keep, count, max_ctx=None):
 def linear_w4(x, w, scale, zero=None, bias=None, out_f32=False, out=None):
     """x [M,K] (bf16 or fp32) times 4-bit weights w [N,K/2] uint8 (low nibble: even column), scale [N,K/group] bf16 or fp32, zero points zero [N,K/group]
     uint8 (None: 8), bias [N] fp32. Returns [M,N] of x's type, or fp32."""
+    if out is None and not out_f32 and (_front or _bind_front_end()):
+        y = _front.linear_w4(x, w, scale, zero, bias)
+        if y is not None:
+            return _out("flexllm_linear_w4", y)
     p, lda = _rows(x)
     (M, K), N = x.shape, w.shape[0]
     if scale.dtype not in _DTYPE or scale.dim() != 2 or scale.shape[0] != N or scale.shape[1] == 0 or K % scale.shape[1] or w.shape[1] * 2 != K:
