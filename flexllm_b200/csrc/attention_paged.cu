@@ -227,7 +227,7 @@ template <int RT> int run_simt(const PagedAttn& a, cudaStream_t st) {
     sa.a = a;
     sa.RC = R < RT ? R : RT; sa.HC = (R + sa.RC - 1) / sa.RC; sa.TQ = RT / sa.RC;
     const long tiles = a.seq.T / sa.TQ + (a.seq.B < a.seq.T ? a.seq.B : a.seq.T);
-    const int splits = key_splits(tiles * a.G * sa.HC, (a.seq.max_ctx + kPage) / kPage, 2);
+    const int splits = key_splits(tiles * a.G * sa.HC, gemm_sm_count(), (a.seq.max_ctx + kPage) / kPage, 1);
     if (tiles * splits > 0x7fffffffL || a.G * sa.HC > 65535) return FLEXLLM_ENOTSUP;
     if (a.dv <= 64) return launch_simt<RT, 4>(sa, (int)tiles, splits, st);
     if (a.dv <= 128) return launch_simt<RT, 8>(sa, (int)tiles, splits, st);

@@ -67,11 +67,11 @@ template <class T> __device__ __noinline__ void attn_row_by_key(const PagedAttn&
 __device__ __forceinline__ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 __device__ __forceinline__ bool not_finite(float v) { return !(fabsf(v) <= 3.402823466e38f); }
 
-// CTAs of a cluster among which a tile's keys are cut, for `tiles` (tile, head) pairs of up to `pages` key pages each: while there are SMs
-// without a tile and each part keeps at least `least` pages. Up to 8, the portable size.
-inline int key_splits(long tiles, int pages, int least) {
+// CTAs of a cluster among which a tile's keys are cut, for `tiles` (tile, head) pairs of up to `pages` key pages each: as many as all run at once
+// (`slots`) while each part keeps `least` pages. Up to 8, the portable size.
+inline int key_splits(long tiles, long slots, int pages, int least) {
     int s = 1;
-    while (s < 8 && tiles * s * 2 <= (long)gemm_sm_count() && pages >= 2 * s * least) s *= 2;
+    while (s < 8 && tiles * s * 2 <= slots && pages >= 2 * s * least) s *= 2;
     return s;
 }
 

@@ -4,10 +4,12 @@
 //   S = Q K^T into TMEM; one thread per row reads its 128 scores, P = 2^(S scale log2 e - m) goes back over them as bf16, and
 //   O += P V takes P from TMEM and V^T from the pages as they lie (keys along the inner index)
 // m is lazy: only a row whose maximum exceeds it by more than kSlack moves it and rescales its O in TMEM.
-//   NQ = 2  two tiles per CTA: one tile's softmax runs under the other's products. For prompts.
-//   NQ = 1  one tile and two score buffers, its keys cut among the CTAs of a cluster when the call has few tiles (trees, decoding): partial
-//           maxima, sums and outputs meet in shared memory, in a fixed order.
-// Warps 0 .. 4 NQ - 1 softmax (one row per thread), then one for TMA, one for the MMAs.
+//   kPair   two tiles per CTA, so that one tile's softmax runs under the other's products: prompts
+//   kOne    one tile per CTA, two CTAs per SM: more tiles than SMs, but not long ones; and heads of more than 128
+//   kTurns  one tile per CTA with two sets of scores, outputs and softmax warps that take the key tiles in turn: fewer tiles than SMs (trees,
+//           decoding), whose keys are also cut among the CTAs of a cluster
+// Where a tile's keys are cut, the parts' maxima, sums and outputs meet in shared memory, in a fixed order.
+// Warps 0 .. 4 W - 1 softmax (W sets, one row per thread), then one for TMA, one for the MMAs.
 // Keys behind a sequence's last one were never written: their scores are replaced, their values zeroed in shared memory. Any other value
 // that a row does not see meets a weight of zero; a row whose result is not finite is computed again, key by key.
 #include "attention_paged.cuh"
@@ -19,6 +21,7 @@ using namespace tc;
 
 namespace {
 
+enum { kOne, kPair, kTurns };
 constexpr int KT = 128;                    // keys per tile
 constexpr float kSlack = 8.0f;             // log2 units by which a score may exceed its row's shift
 constexpr float kNoScore = -1e30f;
@@ -41,6 +44,7 @@ __host__ __device__ inline TcSmem tc_smem(int NQ, int kc, int vr, int ks, int vs
     return o;
 }
 constexpr int kMaxStages = 4;
+constexpr uint32_t kHalfSm = 108 * 1024, kWholeSm = 224 * 1024;       // dynamic shared memory; a few KB are static
 
 // D[tmem] (+)= A[tmem] * B[smem]^T, one 128 x N x 16 bf16 step with A's pairs of elements in 8 columns
 __device__ __forceinline__ void umma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
@@ -57,14 +61,17 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
     return v;
 }
 
-template <int NQ>
-__global__ void __launch_bounds__(NQ * 128 + 64, 1) attn_paged_tc_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_constant__ CUtensorMap tmapK,
+template <int MODE>
+__global__ void __launch_bounds__(MODE == kOne ? 192 : 320, MODE == kOne ? 2 : 1) attn_paged_tc_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_constant__ CUtensorMap tmapK,
                                                                          const __grid_constant__ CUtensorMap tmapV, const __grid_constant__ TcArgs t) {
-    constexpr int WT = NQ * 4, WM = WT + 1;               // the TMA warp, the MMA warp
+    constexpr int NQ = MODE == kPair ? 2 : 1;             // tiles
+    constexpr int W = MODE == kOne ? 1 : 2;               // sets of scores and outputs
+    constexpr int STEP = MODE == kTurns ? 2 : 1;          // set w takes the key tiles w * (STEP - 1), + STEP, ..
+    constexpr int WT = W * 4, WM = WT + 1, NT = W * 128 + 64;      // the TMA warp, the MMA warp, threads
     extern __shared__ uint8_t smem_raw[];
     __shared__ Unit unit_sm;
     __shared__ unsigned redo_sm[4 * NQ];
-    __shared__ float m_sm[128], l_sm[128];
+    __shared__ float m_sm[W * 128], l_sm[W * 128], w_sm[NQ == 2 ? 1 : 128 * STEP];
     const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
     uint8_t* base_ptr = smem_raw + (base - raw);
     const PagedAttn& a = t.a;
@@ -107,7 +114,7 @@ __global__ void __launch_bounds__(NQ * 128 + 64, 1) attn_paged_tc_kernel(const _
         if (b < 0 || i0 + q * t.TQ >= s.n) continue;
         end = a.mask ? s.ctx + s.n : min(s.ctx + i0 + (q + 1) * t.TQ, s.ctx + s.n);
         const int n = (end + KT - 1) / KT;
-        t0 = (int)((long)n * split / t.n_split);          // NQ = 2 is never split
+        t0 = (int)((long)n * split / t.n_split);          // pairs are never cut
         t1[q] = (int)((long)n * (split + 1) / t.n_split);
     }
     const int t_last = t1[0] > t1[NQ - 1] ? t1[0] : t1[NQ - 1];
@@ -148,70 +155,56 @@ __global__ void __launch_bounds__(NQ * 128 + 64, 1) attn_paged_tc_kernel(const _
     } else if (warp == WM) {
         const uint32_t idesc_qk = umma_idesc_bf16(128, KT), idesc_pv = umma_idesc_bf16(128, t.vr);
         const int ksteps = (a.dk + 15) / 16;
-        const uint32_t tO = tmem + 2 * KT;
+        const uint32_t tO = tmem + W * KT;
+        if (lane == 0) {
         bool ok = t0 < t_last;
-        // S of tile q (NQ 1: buffer j & 1) = Q_q K_j^T
-        auto qk = [&](int q, int j) {
-            const int n = j - t0, sk = n % t.ks, sb = NQ == 2 ? q : n & 1;
+        // S of set w = Q K_j^T, over the weights that the product in front has read
+        auto qk = [&](int w, int j) {
+            const int n = j - t0, sk = n % t.ks, q = NQ == 2 ? w : 0;
             if (!mbar_wait(bar_kf + 8 * sk, (uint32_t)(n / t.ks & 1), abort_flag)) return false;
             tc_fence_after();
             for (int k = 0; k < ksteps; k++) {
                 const uint32_t blk = k >> 2, off = 2 * (k & 3);
-                umma_bf16(tmem + sb * KT, umma_desc_k_sw128(base + (uint32_t)(q * t.kc + blk) * 16384u) + off,
+                umma_bf16(tmem + w * KT, umma_desc_k_sw128(base + (uint32_t)(q * t.kc + blk) * 16384u) + off,
                           umma_desc_k_sw128(base + o.k + (uint32_t)(sk * t.kc + blk) * 16384u) + off, idesc_qk, k > 0 ? 1u : 0u);
             }
-            umma_commit(bar_s + 8 * sb);
+            umma_commit(bar_s + 8 * w);
             if (q == NQ - 1 || j >= t1[NQ - 1]) umma_commit(bar_ke + 8 * sk);      // the last product with K_j
             return true;
         };
-        if (lane == 0 && ok) {
-            ok = mbar_wait(bar_q, 0, abort_flag);
-            for (int q = 0; q < NQ; q++)
-                if (ok && t0 < t1[q]) ok = qk(q, t0);
+        if (ok) ok = mbar_wait(bar_q, 0, abort_flag);
+        for (int w = 0; w < W; w++) {
+            const int j = t0 + w * (STEP - 1);
+            if (ok && j < t1[NQ == 2 ? w : 0]) ok = qk(w, j);
         }
-        for (int j = t0; j < t_last; j++) {
-            const int n = j - t0, sv = n % t.vs, left = end - j * KT;
-            if (lane == 0 && ok && NQ == 1 && j + 1 < t1[0]) ok = qk(0, j + 1);
-            if (lane == 0 && ok) ok = mbar_wait(bar_vf + 8 * sv, (uint32_t)(n / t.vs & 1), abort_flag);
-            if (left < KT) {                              // the sequence ends inside the tile: zeros for the values behind its end
-                if (!__shfl_sync(0xffffffffu, (int)ok, 0)) break;
-                for (int e = lane; e < t.vr * 16; e += 32) {
-                    const int c = (e & 15) * 8, d = e >> 4;        // keys c .. c + 7 of row d
-                    if (c + 8 <= left) continue;
-                    uint8_t* row = base_ptr + o.v + (uint32_t)(sv * 2 + (c >> 6)) * t.vr * 128u + d * 128 + ((((c & 63) >> 3) ^ (d & 7)) << 4);
-                    if (c >= left) *reinterpret_cast<uint4*>(row) = make_uint4(0, 0, 0, 0);
-                    else
-                        for (int x = left - c; x < 8; x++) reinterpret_cast<uint16_t*>(row)[x] = 0;
-                }
-                fence_proxy_async_smem();
-                __syncwarp();
+        for (int j = t0; ok && j < t_last; j++) {
+            const int n = j - t0, sv = n % t.vs;
+            if (ok) ok = mbar_wait(bar_vf + 8 * sv, (uint32_t)(n / t.vs & 1), abort_flag);
+            for (int q = 0; ok && q < NQ; q++) {
+                if (j >= t1[q]) continue;
+                const int w = MODE == kTurns ? n & 1 : q;
+                ok = mbar_wait(bar_p + 8 * w, (uint32_t)(n / STEP & 1), abort_flag);
+                if (!ok) break;
+                tc_fence_after();
+                for (int k = 0; k < KT / 16; k++)
+                    umma_bf16_ts(tO + w * t.o_stride, tmem + w * KT + 8 * k,
+                                 umma_desc_k_sw128(base + o.v + (uint32_t)(sv * 2 + (k >> 2)) * t.vr * 128u) + 2 * (k & 3), idesc_pv, n >= STEP || k > 0 ? 1u : 0u);
+                umma_commit((j + STEP < t1[q] ? bar_o : bar_f) + 8 * w);        // the last one has a barrier of its own
+                if (q == NQ - 1 || j >= t1[NQ - 1]) umma_commit(bar_ve + 8 * sv);
+                if (j + STEP < t1[q]) ok = qk(w, j + STEP);
             }
-            if (lane == 0)
-                for (int q = 0; q < NQ; q++) {
-                    if (!ok || j >= t1[q]) continue;
-                    const int sb = NQ == 2 ? q : n & 1;
-                    ok = mbar_wait(bar_p + 8 * sb, (uint32_t)((NQ == 2 ? n : n >> 1) & 1), abort_flag);
-                    if (!ok) continue;
-                    tc_fence_after();
-                    for (int k = 0; k < KT / 16; k++)
-                        umma_bf16_ts(tO + q * t.o_stride, tmem + sb * KT + 8 * k,
-                                     umma_desc_k_sw128(base + o.v + (uint32_t)(sv * 2 + (k >> 2)) * t.vr * 128u) + 2 * (k & 3), idesc_pv, n > 0 || k > 0 ? 1u : 0u);
-                    umma_commit((j + 1 < t1[q] ? bar_o : bar_f) + 8 * q);       // the last one has a barrier of its own
-                    if (q == NQ - 1 || j >= t1[NQ - 1]) umma_commit(bar_ve + 8 * sv);
-                    if (NQ == 2 && j + 1 < t1[q]) ok = qk(q, j + 1);
-                }
-            if (!__shfl_sync(0xffffffffu, (int)ok, 0)) break;
+        }
         }
     } else {
         // ---- one row per thread
-        const int q = warp >> 2, row = threadIdx.x & 127;
+        const int w = warp >> 2, q = NQ == 2 ? w : 0, row = threadIdx.x & 127;
         const uint32_t lane_addr = (uint32_t)((warp & 3) * 32) << 16;
         const int i = i0 + q * t.TQ + row / t.RC, hr = row % t.RC;
         const bool live = row < t.TQ * t.RC && i < s.n && hr < heads;
         const int sure = live ? sure_keys(a, s, i) : 0x40000000;                          // rows of the tile without a token mask nothing
         const unsigned long long bits = live ? mask_bits(a, s, i) : 0ull;
-        const uint32_t tO = tmem + 2 * KT + q * t.o_stride + lane_addr;
-        const int my_t1 = NQ == 2 && q == 1 ? t1[NQ - 1] : t1[0];
+        const uint32_t tO = tmem + W * KT + w * t.o_stride + lane_addr;
+        const int my_t0 = t0 + w * (STEP - 1), my_t1 = q == 1 ? t1[NQ - 1] : t1[0];
         auto wait_bar = [&](uint32_t bar, uint32_t parity) {
             const int got = lane == 0 ? (int)mbar_wait(bar, parity, abort_flag) : 1;
             return __shfl_sync(0xffffffffu, got, 0) != 0;
@@ -220,11 +213,11 @@ __global__ void __launch_bounds__(NQ * 128 + 64, 1) attn_paged_tc_kernel(const _
         f32x2 l2 = pack2(0.0f, 0.0f);
         const f32x2 a22 = pack2(t.a2, t.a2);
         bool ok = true;
-        for (int j = t0; j < my_t1; j++) {
-            const int n = j - t0, sb = NQ == 2 ? q : n & 1;
-            if (!wait_bar(bar_s + 8 * sb, (uint32_t)((NQ == 2 ? n : n >> 1) & 1))) { ok = false; break; }
+        for (int j = my_t0; j < my_t1; j += STEP) {
+            const int n = j - t0, turn = n / STEP, left = end - j * KT;
+            if (!wait_bar(bar_s + 8 * w, (uint32_t)(turn & 1))) { ok = false; break; }
             tc_fence_after();
-            const uint32_t tS = tmem + sb * KT + lane_addr;
+            const uint32_t tS = tmem + w * KT + lane_addr;
             uint32_t v[4][32];
 #pragma unroll
             for (int c = 0; c < 4; c++) tmem_ld_32x32(tS + 32 * c, v[c]);
@@ -234,11 +227,11 @@ __global__ void __launch_bounds__(NQ * 128 + 64, 1) attn_paged_tc_kernel(const _
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
                     const int nv = min(max(hi - 32 * c, 0), 32), sh = 32 * c - (s.ctx - j * KT);
-                    uint32_t w = nv == 32 ? 0xffffffffu : (1u << nv) - 1u;
-                    if (sh > -32 && sh < 64) w |= sh >= 0 ? (uint32_t)(bits >> sh) : (uint32_t)bits << -sh;
+                    uint32_t see = nv == 32 ? 0xffffffffu : (1u << nv) - 1u;
+                    if (sh > -32 && sh < 64) see |= sh >= 0 ? (uint32_t)(bits >> sh) : (uint32_t)bits << -sh;
 #pragma unroll
                     for (int x = 0; x < 32; x++)
-                        if (!(w >> x & 1u)) v[c][x] = 0xff800000u;
+                        if (!(see >> x & 1u)) v[c][x] = 0xff800000u;
                 }
             }
             float mx[4];
@@ -254,16 +247,16 @@ __global__ void __launch_bounds__(NQ * 128 + 64, 1) attn_paged_tc_kernel(const _
                 const float m_new = grow ? top : m, al = ex2_fast(m - m_new);
                 m = m_new;
                 l2 = mul2(l2, pack2(al, al));
-                if (n > 0) {
-                    if (!wait_bar(bar_o + 8 * q, (uint32_t)((n - 1) & 1))) { ok = false; break; }      // the products so far
+                if (turn > 0) {
+                    if (!wait_bar(bar_o + 8 * w, (uint32_t)((turn - 1) & 1))) { ok = false; break; }      // the products so far
                     tc_fence_after();
                     for (int d = 0; d < t.vr; d += 16) {
-                        uint32_t w[16];
-                        tmem_ld_32x16(tO + d, w);
+                        uint32_t u[16];
+                        tmem_ld_32x16(tO + d, u);
                         tmem_ld_wait();
 #pragma unroll
-                        for (int x = 0; x < 16; x++) w[x] = __float_as_uint(__uint_as_float(w[x]) * al);
-                        tmem_st_32x16(tO + d, w);
+                        for (int x = 0; x < 16; x++) u[x] = __float_as_uint(__uint_as_float(u[x]) * al);
+                        tmem_st_32x16(tO + d, u);
                     }
                 }
             }
@@ -281,105 +274,149 @@ __global__ void __launch_bounds__(NQ * 128 + 64, 1) attn_paged_tc_kernel(const _
                 }
                 tmem_st_32x16(tS + 16 * c, pk);
             }
+            if (left < KT) {                              // the sequence ends inside the tile: zeros for the values behind its end
+                const int sv = n % t.vs, c0 = left >> 3;
+                if (!wait_bar(bar_vf + 8 * sv, (uint32_t)(n / t.vs & 1))) { ok = false; break; }
+                for (int d = row; d < t.vr; d += 128) {
+                    uint8_t* vrow = base_ptr + o.v + (uint32_t)(sv * 2) * t.vr * 128u + d * 128;
+                    for (int c = c0; c < 16; c++) {        // keys 8 c .. 8 c + 7
+                        uint8_t* at = vrow + (uint32_t)(c >> 3) * t.vr * 128u + (((c ^ d) & 7) << 4);
+                        if (c > c0 || !(left & 7)) *reinterpret_cast<uint4*>(at) = make_uint4(0, 0, 0, 0);
+                        else
+                            for (int x = left & 7; x < 8; x++) reinterpret_cast<uint16_t*>(at)[x] = 0;
+                    }
+                }
+                fence_proxy_async_smem();
+            }
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(bar_p + 8 * sb);
+            if (lane == 0) mbar_arrive(bar_p + 8 * w);
         }
         float l, l1;
         unpack2(l2, l, l1);
         l += l1;
-        const int n_kt = my_t1 - t0;
-        if (ok && n_kt > 0) ok = wait_bar(bar_f + 8 * q, 0);
+        const bool any = my_t0 < my_t1;
+        if (ok && any) ok = wait_bar(bar_f + 8 * w, 0);
+        if (MODE == kTurns) named_sync<1, 256>();          // every product of both sets has been waited for
         if (ok) {
             tc_fence_after();
-            if (NQ == 2 || t.n_split == 1) {
+            if (MODE == kPair || (MODE == kOne && t.n_split == 1)) {
                 const float rl = l == 0.0f ? 0.0f : 1.0f / l;
                 bool odd = false;
                 bf16* out = (bf16*)a.out + (long)(s.row0 + i) * a.ldo + (long)(h0 + hr) * a.dv;
                 const bool vec = (a.ldo & 7) == 0 && aligned16(a.out);
-                for (int d0 = 0; d0 < t.vr; d0 += 16) {
-                    uint32_t w[16];
-                    tmem_ld_32x16(tO + d0, w);
+                for (int d0 = 0; d0 < t.vr; d0 += 32) {
+                    uint32_t u[32];
+                    tmem_ld_32x32(tO + d0, u);            // o_stride columns are this tile's
                     tmem_ld_wait();
                     if (!live) continue;
-                    float f[16];
 #pragma unroll
-                    for (int x = 0; x < 16; x++) f[x] = l == 0.0f ? 0.0f : __uint_as_float(w[x]) * rl;
+                    for (int c = 0; c < 32; c += 8) {
+                        if (d0 + c >= a.dv) continue;
+                        float f[8];
 #pragma unroll
-                    for (int hf = 0; hf < 2; hf++) {
-                        if (d0 + 8 * hf >= a.dv) continue;
-#pragma unroll
-                        for (int x = 0; x < 8; x++) odd = odd || not_finite(f[8 * hf + x]);
-                        if (vec) *reinterpret_cast<uint4*>(out + d0 + 8 * hf) = make_uint4(bf_pack(f[8 * hf], f[8 * hf + 1]), bf_pack(f[8 * hf + 2], f[8 * hf + 3]),
-                                                                                          bf_pack(f[8 * hf + 4], f[8 * hf + 5]), bf_pack(f[8 * hf + 6], f[8 * hf + 7]));
+                        for (int x = 0; x < 8; x++) {
+                            f[x] = l == 0.0f ? 0.0f : __uint_as_float(u[c + x]) * rl;
+                            odd = odd || not_finite(f[x]);
+                        }
+                        if (vec) *reinterpret_cast<uint4*>(out + d0 + c) = make_uint4(bf_pack(f[0], f[1]), bf_pack(f[2], f[3]), bf_pack(f[4], f[5]), bf_pack(f[6], f[7]));
                         else
 #pragma unroll
-                            for (int x = 0; x < 8; x++) out[d0 + 8 * hf + x] = __float2bfloat16_rn(f[8 * hf + x]);
+                            for (int x = 0; x < 8; x++) out[d0 + c + x] = __float2bfloat16_rn(f[x]);
                     }
                 }
                 const unsigned bad = __ballot_sync(0xffffffffu, odd);
                 if (lane == 0) redo_sm[warp] = bad;
             } else {
-                // this part's row into shared memory, over the operands (every product has been waited for)
-                float* orow = reinterpret_cast<float*>(base_ptr) + (long)row * (a.dv + 4);
-                for (int d0 = 0; d0 < t.vr; d0 += 16) {
-                    uint32_t w[16];
-                    if (n_kt > 0) { tmem_ld_32x16(tO + d0, w); tmem_ld_wait(); }
+                // this part's row into shared memory, over the operands
+                float* orow = reinterpret_cast<float*>(base_ptr) + (long)(w * 128 + row) * (a.dv + 4);
+                for (int d0 = 0; d0 < t.vr; d0 += 32) {
+                    uint32_t u[32];
+                    if (any) {
+                        tmem_ld_32x32(tO + d0, u);
+                        tmem_ld_wait();
+                    } else {
 #pragma unroll
-                    for (int x = 0; x < 16; x += 4)
-                        if (d0 + x < a.dv) {
-                            float4 f = make_float4(0.f, 0.f, 0.f, 0.f);
-                            if (n_kt > 0) f = make_float4(__uint_as_float(w[x]), __uint_as_float(w[x + 1]), __uint_as_float(w[x + 2]), __uint_as_float(w[x + 3]));
-                            *reinterpret_cast<float4*>(orow + d0 + x) = f;
-                        }
+                        for (int x = 0; x < 32; x++) u[x] = 0;
+                    }
+#pragma unroll
+                    for (int x = 0; x < 32; x += 4)
+                        if (d0 + x < a.dv) *reinterpret_cast<uint4*>(orow + d0 + x) = make_uint4(u[x], u[x + 1], u[x + 2], u[x + 3]);
                 }
-                m_sm[row] = m; l_sm[row] = l;
+                m_sm[w * 128 + row] = m; l_sm[w * 128 + row] = l;
             }
         }
     }
     }
-    if (NQ == 1 && b >= 0 && t.n_split > 1) {
-        cluster_sync();
-        // the rows' parts joined, eight columns per thread; CTA r of the cluster has rows r, r + n_split, ..
-        const int rows = min(t.TQ, s.n - i0) * t.RC, per = a.dv / 8;
-        const uint32_t m_at = smem_u32(m_sm), l_at = smem_u32(l_sm);
-        for (int e = threadIdx.x; e < (rows - split + t.n_split - 1) / t.n_split * per; e += NQ * 128 + 64) {
-            const int row = split + e / per * t.n_split, d = e % per * 8;
+    if (b >= 0 && (MODE == kTurns || (MODE == kOne && t.n_split > 1))) {
+        if (t.n_split > 1) cluster_sync(); else __syncthreads();
+        // the rows' parts joined; CTA r of the cluster has rows r, r + n_split, ..: first the parts' weights (over the
+        // sums; parts x rows of a CTA are 128 STEP at most), then the outputs
+        constexpr int MOST = 8 * STEP;                     // parts: set p % STEP of CTA p / STEP
+        const int rows = min(t.TQ, s.n - i0) * t.RC, per = a.dv / 8, mine = (rows - split + t.n_split - 1) / t.n_split, parts = t.n_split * STEP;
+        for (int e = threadIdx.x; e < mine; e += NT) {
+            const int row = split + e * t.n_split;
+            float top = kNoScore, sum = 0.0f, mk[MOST], lk[MOST];
+#pragma unroll
+            for (int p = 0; p < MOST; p++)
+                if (p < parts) {
+                    mk[p] = ld_cluster_f32(cluster_addr(smem_u32(m_sm + (p % STEP) * 128 + row), p / STEP));
+                    lk[p] = ld_cluster_f32(cluster_addr(smem_u32(l_sm + (p % STEP) * 128 + row), p / STEP));
+                }
+#pragma unroll
+            for (int p = 0; p < MOST; p++)
+                if (p < parts) top = fmaxf(top, mk[p]);
+#pragma unroll
+            for (int p = 0; p < MOST; p++)
+                if (p < parts) { mk[p] = ex2_fast(mk[p] - top); sum = __fmaf_rn(lk[p], mk[p], sum); }
+            const float r = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+            for (int p = 0; p < MOST; p++)
+                if (p < parts) w_sm[p * mine + e] = sum == 0.0f ? 0.0f : mk[p] * r;
+        }
+        __syncthreads();
+        for (int e = threadIdx.x; e < mine * per; e += NT) {
+            const int i = e / per, row = split + i * t.n_split, d = e % per * 8;
             if (row % t.RC >= heads) continue;
-            float top = kNoScore;
-            for (int k = 0; k < t.n_split; k++) top = fmaxf(top, ld_cluster_f32(cluster_addr(m_at + 4 * row, k)));
-            float sum = 0.0f, f[8];
+            float f[8];
 #pragma unroll
             for (int x = 0; x < 8; x++) f[x] = 0.0f;
-            for (int k = 0; k < t.n_split; k++) {
-                const float w = ex2_fast(ld_cluster_f32(cluster_addr(m_at + 4 * row, k)) - top);
-                const uint32_t at = cluster_addr(base + (uint32_t)(row * (a.dv + 4) + d) * 4u, k);
-                const float4 x = ld_cluster_f32x4(at), y = ld_cluster_f32x4(at + 16);
-                sum = __fmaf_rn(ld_cluster_f32(cluster_addr(l_at + 4 * row, k)), w, sum);
-                f[0] = __fmaf_rn(x.x, w, f[0]); f[1] = __fmaf_rn(x.y, w, f[1]); f[2] = __fmaf_rn(x.z, w, f[2]); f[3] = __fmaf_rn(x.w, w, f[3]);
-                f[4] = __fmaf_rn(y.x, w, f[4]); f[5] = __fmaf_rn(y.y, w, f[5]); f[6] = __fmaf_rn(y.z, w, f[6]); f[7] = __fmaf_rn(y.w, w, f[7]);
+            for (int p0 = 0; p0 < parts; p0 += 4) {        // the loads of four parts are under way together
+                float4 x[4], y[4];
+#pragma unroll
+                for (int p = 0; p < 4; p++)
+                    if (p0 + p < parts) {
+                        const uint32_t at = cluster_addr(base + (uint32_t)(((p0 + p) % STEP * 128 + row) * (a.dv + 4) + d) * 4u, (p0 + p) / STEP);
+                        x[p] = ld_cluster_f32x4(at); y[p] = ld_cluster_f32x4(at + 16);
+                    }
+#pragma unroll
+                for (int p = 0; p < 4; p++)
+                    if (p0 + p < parts) {
+                        const float w = w_sm[(p0 + p) * mine + i];
+                        f[0] = __fmaf_rn(x[p].x, w, f[0]); f[1] = __fmaf_rn(x[p].y, w, f[1]); f[2] = __fmaf_rn(x[p].z, w, f[2]); f[3] = __fmaf_rn(x[p].w, w, f[3]);
+                        f[4] = __fmaf_rn(y[p].x, w, f[4]); f[5] = __fmaf_rn(y[p].y, w, f[5]); f[6] = __fmaf_rn(y[p].z, w, f[6]); f[7] = __fmaf_rn(y[p].w, w, f[7]);
+                    }
             }
-            const float r = sum == 0.0f ? 0.0f : 1.0f / sum;
             bf16* out = (bf16*)a.out + (long)(s.row0 + i0 + row / t.RC) * a.ldo + (long)(h0 + row % t.RC) * a.dv + d;
             bool odd = false;
 #pragma unroll
-            for (int x = 0; x < 8; x++) {
-                f[x] = sum == 0.0f ? 0.0f : f[x] * r;
-                odd = odd || not_finite(f[x]);
-            }
+            for (int x = 0; x < 8; x++) odd = odd || not_finite(f[x]);
             if (odd) atomicOr(&redo_sm[row >> 5], 1u << (row & 31));
             if ((a.ldo & 7) == 0 && aligned16(a.out)) *reinterpret_cast<uint4*>(out) = make_uint4(bf_pack(f[0], f[1]), bf_pack(f[2], f[3]), bf_pack(f[4], f[5]), bf_pack(f[6], f[7]));
             else
 #pragma unroll
                 for (int x = 0; x < 8; x++) out[x] = __float2bfloat16_rn(f[x]);
         }
-        cluster_sync();
+        if (t.n_split > 1) cluster_sync();
     }
     tc_fence_before();
     __syncthreads();
-    if (b >= 0 && !*abort_flag)
-        for (int row = warp; row < NQ * 128; row += NQ * 4 + 2)
+    unsigned redo = 0;
+#pragma unroll
+    for (int w = 0; w < 4 * NQ; w++) redo |= redo_sm[w];
+    if (redo && !*abort_flag)
+        for (int row = warp; row < NQ * 128; row += NT / 32)
             if (redo_sm[row >> 5] >> (row & 31) & 1) attn_row_by_key<bf16>(a, b, s, i0 + (row >> 7) * t.TQ + (row & 127) / t.RC, h0 + (row & 127) % t.RC);
     if (*abort_flag) {
         const unsigned long long t_0 = globaltimer_ns();
@@ -390,26 +427,29 @@ __global__ void __launch_bounds__(NQ * 128 + 64, 1) attn_paged_tc_kernel(const _
     if (warp == WM) { tc_fence_after(); tmem_dealloc(tmem, t.tmem_cols); }
 }
 
-template <int NQ> int launch_tc(TcArgs& t, long tiles, cudaStream_t st) {
+template <int MODE> int launch_tc(TcArgs& t, long tiles, cudaStream_t st) {
     const PagedAttn& a = t.a;
+    constexpr int NQ = MODE == kPair ? 2 : 1, W = MODE == kOne ? 1 : 2, NT = W * 128 + 64;
+    // stages while they fit, of K and V in turn; kOne: two CTAs per SM where that is possible
+    const bool two = MODE == kOne && KT + t.o_stride <= 256 && tc_smem(1, t.kc, t.vr, 1, 1).total <= kHalfSm;
+    t.tmem_cols = two ? 256 : 512;
     t.ks = t.vs = 1;
-    // stages while they fit: of K and V in turn
     for (int i = 0; i < 2 * (kMaxStages - 1); i++) {
         int& n = i & 1 ? t.vs : t.ks;
         n++;
-        if (tc_smem(NQ, t.kc, t.vr, t.ks, t.vs).total > 224 * 1024) { n--; break; }
+        if (tc_smem(NQ, t.kc, t.vr, t.ks, t.vs).total > (two ? kHalfSm : kWholeSm)) { n--; break; }
     }
-    const TcSmem o = tc_smem(NQ, t.kc, t.vr, t.ks, t.vs);
-    if (o.total > 226 * 1024 || (t.n_split > 1 && 128 * (a.dv + 4) * 4 > (int)o.bars)) return FLEXLLM_ENOTSUP;
-    t.o_stride = (t.vr + 31) / 32 * 32;
-    t.tmem_cols = 512;                                    // two score tiles and the outputs: over 256 in any case
+    TcSmem o = tc_smem(NQ, t.kc, t.vr, t.ks, t.vs);
+    // the parts of a tile go over the operands, not over the barriers
+    const uint32_t parts = MODE == kTurns || t.n_split > 1 ? (uint32_t)(W * 128 * (a.dv + 4) * 4) : 0;
+    if (o.total > kWholeSm || parts > o.bars) return FLEXLLM_ENOTSUP;
     CUtensorMap tq, tk, tv;
     TRY_RC(make_tmap_rows3_u8(&tq, a.q, (uint64_t)a.seq.T, (uint64_t)a.H, (uint64_t)a.dk * 2, (uint32_t)t.TQ, (uint32_t)t.RC, (uint64_t)a.ldq * 2));
     TRY_RC(make_tmap_2d_u8(&tk, a.k, (uint64_t)a.seq.n_pages * a.G * kPage, (uint64_t)a.dk * 2, kPage));
     TRY_RC(make_tmap_2d_u8(&tv, a.v, (uint64_t)a.seq.n_pages * a.G * a.dv, kPage * 2, (uint32_t)t.vr));
-    auto kern = attn_paged_tc_kernel<NQ>;
+    auto kern = attn_paged_tc_kernel<MODE>;
     TRY_RC(allow_shared(kern, o.total));
-    launch_cluster(kern, dim3((unsigned)(tiles * t.n_split), a.G * t.HC), dim3(NQ * 128 + 64), t.n_split, o.total, st, tq, tk, tv, t);
+    launch_cluster(kern, dim3((unsigned)(tiles * t.n_split), a.G * t.HC), dim3(NT), t.n_split, o.total, st, tq, tk, tv, t);
     return launch_status();
 }
 
@@ -420,18 +460,26 @@ int attn_paged_tc(const PagedAttn& a, cudaStream_t st) {
     const int R = a.H / a.G;
     t.a = a;
     t.RC = R < 128 ? R : 128; t.HC = (R + t.RC - 1) / t.RC; t.TQ = 128 / t.RC;
-    t.kc = (a.dk + 63) / 64; t.vr = (a.dv + 15) / 16 * 16;
+    t.kc = (a.dk + 63) / 64; t.vr = (a.dv + 15) / 16 * 16; t.o_stride = (t.vr + 31) / 32 * 32;
     t.a2 = a.scale * kLog2e;
     if (t.a2 < 1e-30f) t.a2 = 1e-30f;                     // scale 0: weights all alike, and no infinity times zero
-    if ((long)a.G * t.HC > 65535) return FLEXLLM_ENOTSUP;
-    const long seqs = a.seq.B < a.seq.T ? a.seq.B : a.seq.T;
-    const long pairs = a.seq.T / (2 * t.TQ) + seqs, ones = a.seq.T / t.TQ + seqs;
-    if (ones * 8 > 0x7fffffffL) return FLEXLLM_ENOTSUP;
+    const long heads = (long)a.G * t.HC, seqs = a.seq.B < a.seq.T ? a.seq.B : a.seq.T;
+    const long pairs = a.seq.T / (2 * t.TQ) + seqs, ones = a.seq.T / t.TQ + seqs;         // at most so many exist
+    if (heads > 65535 || ones * 8 > 0x7fffffffL) return FLEXLLM_ENOTSUP;
+    const long sms = gemm_sm_count(), tiles = ((a.seq.T + seqs - 1) / seqs + t.TQ - 1) / t.TQ * seqs * heads;      // if all sequences are of equal length
+    const int pages = (a.seq.max_ctx + kPage) / kPage;
     t.n_split = 1;
-    // two tiles per CTA where sequences fill them and there is one such CTA for every SM
-    if (a.dk <= 128 && a.dv <= 128 && (long)a.seq.T >= 2L * t.TQ * seqs && a.seq.T / (2 * t.TQ) * a.G * t.HC >= gemm_sm_count()) return launch_tc<2>(t, pairs, st);
-    t.n_split = key_splits(ones * a.G * t.HC, (a.seq.max_ctx + kPage) / kPage, 4);
-    return launch_tc<1>(t, ones, st);
+    if (a.dk <= 128 && a.dv <= 128) {
+        if (tiles <= sms) {
+            t.n_split = key_splits(tiles, sms, pages, 2 * KT / kPage);
+            return launch_tc<kTurns>(t, ones, st);
+        }
+        // pairs where sequences fill them and every SM has one
+        if ((long)a.seq.T >= 2L * t.TQ * seqs && tiles >= 2 * sms) return launch_tc<kPair>(t, pairs, st);
+        return launch_tc<kOne>(t, ones, st);
+    }
+    t.n_split = key_splits(tiles, sms, pages, KT / kPage);
+    return launch_tc<kOne>(t, ones, st);
 }
 
 }  // namespace flexllm

@@ -65,12 +65,14 @@ CASES = [
     ([1300, 77, 1100], [0, 65, 3], 16, 16, 128, 128),
     ([700, 0, 650], [100, 0, 0], 32, 8, 64, 64),
     ([2500], [0], 40, 8, 96, 80),
+    ([300, 310], [0, 70], 32, 8, 64, 64),
+    ([40, 1, 64, 33, 40, 40, 0, 17, 40, 40, 40], [0, 1, 500, 63, 64, 65, 3, 127, 128, 129, 130], 32, 8, 128, 128),
     ([1, 3000, 33], [700, 128, 1], 16, 8, 72, 128),
 ]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF], ids=["f32", "bf16"])
-@pytest.mark.parametrize("case", CASES, ids=lambda c: "n%s-h%dx%d-d%d-%d" % ("_".join(map(str, c[0])), c[2], c[3], c[4], c[5]))
+@pytest.mark.parametrize("case", CASES, ids=lambda c: "n%s-h%dx%d-d%d-%d" % ("_".join(map(str, c[0][:4])), c[2], c[3], c[4], c[5]))
 def test_packed_attention(ops, case, dtype):
     new, ctx, H, G, dim, vdim = case
     q, k, v, table, start, cx = inputs(new, ctx, H, G, dim, vdim, dtype, seed=len(new) + dim)
@@ -87,13 +89,15 @@ TREES = [
     ([5, 63], [700, 1], 10, 2, 96, 96),
     ([30, 64], [3000, 64], 32, 8, 128, 128),
     ([16], [5000], 4, 4, 128, 128),
+    ([i % 33 for i in range(40)], [(77 * i) % 400 for i in range(40)], 32, 8, 64, 64),
+    ([1] * 70, [(77 * i) % 900 for i in range(70)], 32, 8, 128, 128),
     ([12, 3], [70, 10], 6, 1, 256, 256),
     ([3], [200], 136, 1, 64, 64),
 ]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF], ids=["f32", "bf16"])
-@pytest.mark.parametrize("case", TREES, ids=lambda c: "n%s-h%dx%d-d%d-%d" % ("_".join(map(str, c[0])), c[2], c[3], c[4], c[5]))
+@pytest.mark.parametrize("case", TREES, ids=lambda c: "n%s-h%dx%d-d%d-%d" % ("_".join(map(str, c[0][:4])), c[2], c[3], c[4], c[5]))
 def test_tree_attention(ops, case, dtype):
     new, ctx, H, G, dim, vdim = case
     q, k, v, table, start, cx = inputs(new, ctx, H, G, dim, vdim, dtype, seed=len(new) + dim)
