@@ -46,15 +46,6 @@ __host__ __device__ inline TcSmem tc_smem(int NQ, int kc, int vr, int ks, int vs
 constexpr int kMaxStages = 4;
 constexpr uint32_t kHalfSm = 108 * 1024, kWholeSm = 224 * 1024;       // dynamic shared memory; a few KB are static
 
-// D[tmem] (+)= A[tmem] * B[smem]^T, one 128 x N x 16 bf16 step with A's pairs of elements in 8 columns
-__device__ __forceinline__ void umma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n\t}"
-        ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(0u)
-        : "memory");
-}
 __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
     float4 v;
     asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
@@ -136,13 +127,13 @@ __global__ void __launch_bounds__(MODE == kOne ? 192 : 320, MODE == kOne ? 2 : 1
             const int pages = 2 * j + 1 < n_pg ? 2 : 1;
             int ok = 1;
             if (lane == 0) {
-                ok = mbar_wait(bar_ke + 8 * sk, (uint32_t)(n / t.ks & 1) ^ 1u, abort_flag);
+                ok = mbar_spin(bar_ke + 8 * sk, (uint32_t)(n / t.ks & 1) ^ 1u, abort_flag);
                 if (ok) {
                     mbar_expect_tx(bar_kf + 8 * sk, (uint32_t)(t.kc * pages) * 8192u);
                     for (int p = 0; p < pages; p++)
                         for (int i = 0; i < t.kc; i++)
                             tma_load_2d(base + o.k + (uint32_t)(sk * t.kc + i) * 16384u + p * 8192u, &tmapK, bar_kf + 8 * sk, i * 128, ((p ? p1 : p0) * a.G + g) * kPage);
-                    ok = mbar_wait(bar_ve + 8 * sv, (uint32_t)(n / t.vs & 1) ^ 1u, abort_flag);
+                    ok = mbar_spin(bar_ve + 8 * sv, (uint32_t)(n / t.vs & 1) ^ 1u, abort_flag);
                 }
                 if (ok) {
                     mbar_expect_tx(bar_vf + 8 * sv, (uint32_t)(t.vr * pages) * 128u);
@@ -161,34 +152,38 @@ __global__ void __launch_bounds__(MODE == kOne ? 192 : 320, MODE == kOne ? 2 : 1
         // S of set w = Q K_j^T, over the weights that the product in front has read
         auto qk = [&](int w, int j) {
             const int n = j - t0, sk = n % t.ks, q = NQ == 2 ? w : 0;
-            if (!mbar_wait(bar_kf + 8 * sk, (uint32_t)(n / t.ks & 1), abort_flag)) return false;
+            if (!mbar_spin(bar_kf + 8 * sk, (uint32_t)(n / t.ks & 1), abort_flag)) return false;
             tc_fence_after();
-            for (int k = 0; k < ksteps; k++) {
-                const uint32_t blk = k >> 2, off = 2 * (k & 3);
-                umma_bf16(tmem + w * KT, umma_desc_k_sw128(base + (uint32_t)(q * t.kc + blk) * 16384u) + off,
-                          umma_desc_k_sw128(base + o.k + (uint32_t)(sk * t.kc + blk) * 16384u) + off, idesc_qk, k > 0 ? 1u : 0u);
-            }
+            const uint32_t q_lo = umma_desc_lo(base + (uint32_t)(q * t.kc) * 16384u), k_lo = umma_desc_lo(base + o.k + (uint32_t)(sk * t.kc) * 16384u);
+            auto four = [&](uint32_t blk) {
+#pragma unroll
+                for (uint32_t k = 0; k < 4; k++) umma_bf16_lo(tmem + w * KT, q_lo + blk * 1024u + 2 * k, k_lo + blk * 1024u + 2 * k, idesc_qk, blk + k > 0);
+            };
+            for (int blk = 0; blk < ksteps >> 2; blk++) four(blk);
+            for (int k = ksteps & ~3; k < ksteps; k++)
+                umma_bf16_lo(tmem + w * KT, q_lo + (k >> 2) * 1024u + 2 * (k & 3), k_lo + (k >> 2) * 1024u + 2 * (k & 3), idesc_qk, k > 0);
             umma_commit(bar_s + 8 * w);
             if (q == NQ - 1 || j >= t1[NQ - 1]) umma_commit(bar_ke + 8 * sk);      // the last product with K_j
             return true;
         };
-        if (ok) ok = mbar_wait(bar_q, 0, abort_flag);
+        if (ok) ok = mbar_spin(bar_q, 0, abort_flag);
         for (int w = 0; w < W; w++) {
             const int j = t0 + w * (STEP - 1);
             if (ok && j < t1[NQ == 2 ? w : 0]) ok = qk(w, j);
         }
         for (int j = t0; ok && j < t_last; j++) {
             const int n = j - t0, sv = n % t.vs;
-            if (ok) ok = mbar_wait(bar_vf + 8 * sv, (uint32_t)(n / t.vs & 1), abort_flag);
+            if (ok) ok = mbar_spin(bar_vf + 8 * sv, (uint32_t)(n / t.vs & 1), abort_flag);
             for (int q = 0; ok && q < NQ; q++) {
                 if (j >= t1[q]) continue;
                 const int w = MODE == kTurns ? n & 1 : q;
-                ok = mbar_wait(bar_p + 8 * w, (uint32_t)(n / STEP & 1), abort_flag);
+                ok = mbar_spin(bar_p + 8 * w, (uint32_t)(n / STEP & 1), abort_flag);
                 if (!ok) break;
                 tc_fence_after();
-                for (int k = 0; k < KT / 16; k++)
-                    umma_bf16_ts(tO + w * t.o_stride, tmem + w * KT + 8 * k,
-                                 umma_desc_k_sw128(base + o.v + (uint32_t)(sv * 2 + (k >> 2)) * t.vr * 128u) + 2 * (k & 3), idesc_pv, n >= STEP || k > 0 ? 1u : 0u);
+                const uint32_t v_lo = umma_desc_lo(base + o.v + (uint32_t)(sv * 2) * t.vr * 128u), page = (uint32_t)t.vr * 8u;
+#pragma unroll
+                for (uint32_t k = 0; k < KT / 16; k++)
+                    umma_bf16_ts_lo(tO + w * t.o_stride, tmem + w * KT + 8 * k, v_lo + (k >> 2) * page + 2 * (k & 3), idesc_pv, n >= STEP || k > 0 ? 1u : 0u);
                 umma_commit((j + STEP < t1[q] ? bar_o : bar_f) + 8 * w);        // the last one has a barrier of its own
                 if (q == NQ - 1 || j >= t1[NQ - 1]) umma_commit(bar_ve + 8 * sv);
                 if (j + STEP < t1[q]) ok = qk(w, j + STEP);
@@ -205,10 +200,7 @@ __global__ void __launch_bounds__(MODE == kOne ? 192 : 320, MODE == kOne ? 2 : 1
         const unsigned long long bits = live ? mask_bits(a, s, i) : 0ull;
         const uint32_t tO = tmem + W * KT + w * t.o_stride + lane_addr;
         const int my_t0 = t0 + w * (STEP - 1), my_t1 = q == 1 ? t1[NQ - 1] : t1[0];
-        auto wait_bar = [&](uint32_t bar, uint32_t parity) {
-            const int got = lane == 0 ? (int)mbar_wait(bar, parity, abort_flag) : 1;
-            return __shfl_sync(0xffffffffu, got, 0) != 0;
-        };
+        auto wait_bar = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_spin(bar, parity, abort_flag)) != 0; };
         float m = kNoScore;
         f32x2 l2 = pack2(0.0f, 0.0f);
         const f32x2 a22 = pack2(t.a2, t.a2);

@@ -71,6 +71,20 @@ int make_tmap_2d_u8_box(CUtensorMap* out, const void* base, uint64_t rows, uint6
     return FLEXLLM_OK;
 }
 
+int make_tmap_2d_u8_ld(CUtensorMap* out, const void* base, uint64_t rows, uint64_t row_bytes, uint32_t box_rows, uint64_t ld_bytes) {
+    EncodeTiledFn fn = get_encode_fn();
+    if (!fn) return FLEXLLM_ECUDA;
+    if (!aligned(base, 16) || ld_bytes % 16 != 0 || ld_bytes < row_bytes || box_rows == 0 || box_rows > 256) return FLEXLLM_EINVAL;
+    cuuint64_t dims[2] = {row_bytes, rows};
+    cuuint64_t strides[1] = {ld_bytes};
+    cuuint32_t box[2] = {128, box_rows};
+    cuuint32_t estr[2] = {1, 1};
+    CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) { g_last_cuda_error = (int)r; return FLEXLLM_ECUDA; }
+    return FLEXLLM_OK;
+}
+
 int make_tmap_3d_u8(CUtensorMap* out, const void* base, uint64_t rows, uint64_t row_bytes, uint32_t box_rows, uint32_t kch) {
     EncodeTiledFn fn = get_encode_fn();
     if (!fn) return FLEXLLM_ECUDA;

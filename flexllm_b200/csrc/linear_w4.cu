@@ -7,42 +7,23 @@
 //
 // Two nibbles j and j + 4 of a word become a pair of bf16 in three instructions (shift, mask and exponent at once: 0x4300 | q is 128 + q, one
 // subtraction of 128 + z). The inner index may go through the MMA in any order, the same one in both operands: a lane's words are as they lie
-// in memory, and the activations are put into that order on their way into shared memory.
-#include "float_common.cuh"
+// in memory, and the activations follow (16 bytes at a time on their way into shared memory, pairs when they are read).
+#include "linear_w4.h"
 
 namespace flexllm {
 
 namespace {
 
-struct W4Args {
-    const void* a; long lda;
-    const uint8_t* w;
-    const void* scale; int scale_f32;
-    const uint8_t* zero;
-    int group;
-    const float* bias;
-    int M, N, K;
-    void* y; long ldy; int y_f32;
+struct W4Args : W4Call {
     int ks;                                // warps of a CTA along K
-    int kc;                                // inner elements staged at a time
+    int per_group; uint32_t magic;         // blocks of a group, and 2^32 / per_group rounded up: the quotient of block numbers below 2^16
+    int red_at, rows_log;                  // where the parts meet in shared memory; log2 of a CTA's rows
+    int steps, chunks;                     // steps of kStep elements per staged chunk of activations (a multiple of ks), chunks
 };
-constexpr int W4_WARPS = 8;
+constexpr int kStep = 128;
+// warps of a CTA: with many tokens fewer of them, with more registers each
+template <int MT> constexpr int kWarps = MT <= 2 ? 16 : 8;
 
-__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t mask, uint32_t bits) {
-    uint32_t r;
-    asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(a), "r"(mask), "r"(bits));
-    return r;
-}
-__device__ __forceinline__ uint32_t sub_bf2(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("sub.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
-}
-__device__ __forceinline__ uint32_t pick(uint32_t a, uint32_t b, uint32_t sel) {
-    uint32_t r;
-    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(sel));
-    return r;
-}
 template <int VW> struct Words { uint32_t v[VW]; };
 template <int VW> __device__ __forceinline__ Words<VW> load_words(const uint8_t* p) {
     Words<VW> r;
@@ -52,18 +33,16 @@ template <int VW> __device__ __forceinline__ Words<VW> load_words(const uint8_t*
     return r;
 }
 
-// 8 activations k .. k + 7 as the bf16 pairs (0,4) (1,5) (2,6) (3,7), PL parts
-template <int PL> struct Eight { uint4 part[PL]; };
-__device__ __forceinline__ Eight<1> eight(const bf16* p) {
-    const uint4 v = *reinterpret_cast<const uint4*>(p);
-    Eight<1> r;
-    r.part[0] = make_uint4(pick(v.x, v.z, 0x5410), pick(v.x, v.z, 0x7632), pick(v.y, v.w, 0x5410), pick(v.y, v.w, 0x7632));
-    return r;
+// 8 bf16 activations k .. k + 7 as the pairs (0,4) (1,5) (2,6) (3,7)
+__device__ __forceinline__ uint4 pairs(const uint4& v) {
+    return make_uint4(pick(v.x, v.z, 0x5410), pick(v.x, v.z, 0x7632), pick(v.y, v.w, 0x5410), pick(v.y, v.w, 0x7632));
 }
-__device__ __forceinline__ Eight<3> eight(const float* p) {
+// 8 fp32 activations as such pairs of their three parts
+struct Eight { uint4 part[3]; };
+__device__ __forceinline__ Eight eight(const float* p) {
     float f[8];
     load8(p, f);
-    Eight<3> r;
+    Eight r;
 #pragma unroll
     for (int k = 0; k < 3; k++) {
         r.part[k] = make_uint4(bf_pack(f[0], f[4]), bf_pack(f[1], f[5]), bf_pack(f[2], f[6]), bf_pack(f[3], f[7]));
@@ -78,145 +57,293 @@ __device__ __forceinline__ Eight<3> eight(const float* p) {
     return r;
 }
 
-// VW words per lane and row: a quad of lanes covers 32 VW elements of one group. MT tiles of 8 tokens.
-template <class T, int VW, int MT>
-__global__ void __launch_bounds__(W4_WARPS * 32, 2) linear_w4_kernel(const __grid_constant__ W4Args p) {
-    constexpr int PL = sizeof(T) == 2 ? 1 : 3;
-    constexpr int BK = 32 * VW;                            // elements of a block
-    constexpr int U = 4 / VW;                              // blocks per step: four words per lane and row
-    extern __shared__ __align__(16) uint8_t x_sm[];        // [PL][tokens][kc] bf16, pitch of 64 bytes more than a multiple of 128
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, lr = lane >> 2, lc = lane & 3;
-    const int m0 = blockIdx.y * 64, Mb = min(p.M - m0, 8 * MT);
-    const int kw = warp % p.ks, rt = blockIdx.x * (W4_WARPS / p.ks) + warp / p.ks;
-    const int n_lo = rt * 16 + lr, n_hi = n_lo + 8;
-    const int groups = p.K / p.group;
-    const uint8_t* w_lo = p.w + (long)min(n_lo, p.N - 1) * (p.K / 2) + lc * 4 * VW;
-    const uint8_t* w_hi = p.w + (long)min(n_hi, p.N - 1) * (p.K / 2) + lc * 4 * VW;
-    const long g_lo = (long)min(n_lo, p.N - 1) * groups, g_hi = (long)min(n_hi, p.N - 1) * groups;
-    auto scale_at = [&](long i) { return p.scale_f32 ? ((const float*)p.scale)[i] : to_f(((const bf16*)p.scale)[i]); };
-    // 128 + z, twice
-    auto zero_at = [&](long i) { return (p.zero ? (uint32_t)(p.zero[i] & 15u) : 8u) * 0x10001u + 0x43004300u; };
-    float acc[MT][4];
-#pragma unroll
-    for (int t = 0; t < MT; t++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) acc[t][i] = 0.0f;
-    pdl_sync();
-    for (int k0 = 0; k0 < p.K; k0 += p.kc) {
-        const int kc = min(p.kc, p.K - k0), pitch = p.kc * 2 + ((p.kc & 63) ? 0 : 64);
-        if (k0) __syncthreads();
-        for (int e = tid; e < Mb * (kc / 8); e += W4_WARPS * 32) {
-            const int m = e / (kc / 8), k = (e - m * (kc / 8)) * 8;
-            const Eight<PL> x = eight((const T*)p.a + (long)(m0 + m) * p.lda + k0 + k);
-            const int blk = k / BK, c = (k % BK) / (8 * VW), j = k % (8 * VW) / 8;
-#pragma unroll
-            for (int q = 0; q < PL; q++)
-                *reinterpret_cast<uint4*>(x_sm + (long)(q * Mb + m) * pitch + (blk * BK + j * 32 + c * 8) * 2) = x.part[q];
-        }
-        __syncthreads();
-        const int nb = kc / BK, b_beg = nb * kw / p.ks, b_end = nb * (kw + 1) / p.ks;
-        for (int b0 = b_beg; b0 < b_end; b0 += U) {
-            Words<VW> wl[U], wh[U];
-            float sl[U], sh[U];
-            uint32_t zl[U], zh[U];
-#pragma unroll
-            for (int u = 0; u < U; u++) {
-                const int b = min(b0 + u, b_end - 1), k = k0 + b * BK;
-                wl[u] = load_words<VW>(w_lo + k / 2); wh[u] = load_words<VW>(w_hi + k / 2);
-                sl[u] = scale_at(g_lo + k / p.group); sh[u] = scale_at(g_hi + k / p.group);
-                zl[u] = zero_at(g_lo + k / p.group); zh[u] = zero_at(g_hi + k / p.group);
-            }
-#pragma unroll
-            for (int u = 0; u < U; u++) {
-                if (b0 + u >= b_end) break;
-                float part[MT][4];
-#pragma unroll
-                for (int t = 0; t < MT; t++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) part[t][i] = 0.0f;
-#pragma unroll
-                for (int j = 0; j < VW; j++) {
-                    uint32_t al[4], ah[4];
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        al[i] = sub_bf2(and_or(wl[u].v[j] >> (4 * i), 0x000f000fu, 0x43004300u), zl[u]);
-                        ah[i] = sub_bf2(and_or(wh[u].v[j] >> (4 * i), 0x000f000fu, 0x43004300u), zh[u]);
-                    }
-#pragma unroll
-                    for (int t = 0; t < MT; t++) {
-                        const int m = t * 8 + lr;
-#pragma unroll
-                        for (int q = 0; q < PL; q++) {
-                            uint4 x = make_uint4(0, 0, 0, 0);
-                            if (m < Mb) x = *reinterpret_cast<const uint4*>(x_sm + (long)(q * Mb + m) * pitch + ((b0 + u) * BK + j * 32 + lc * 8) * 2);
-                            mma_bf16(part[t], al[0], ah[0], al[1], ah[1], x.x, x.y);
-                            mma_bf16(part[t], al[2], ah[2], al[3], ah[3], x.z, x.w);
-                        }
-                    }
-                }
-#pragma unroll
-                for (int t = 0; t < MT; t++) {
-                    acc[t][0] = __fmaf_rn(part[t][0], sl[u], acc[t][0]); acc[t][1] = __fmaf_rn(part[t][1], sl[u], acc[t][1]);
-                    acc[t][2] = __fmaf_rn(part[t][2], sh[u], acc[t][2]); acc[t][3] = __fmaf_rn(part[t][3], sh[u], acc[t][3]);
-                }
-            }
-        }
-    }
-    // the warps' parts of K, joined in their order; [ks][tokens][rows of the CTA]
-    __syncthreads();
-    float* red = reinterpret_cast<float*>(x_sm);
-    const int rows = 16 * (W4_WARPS / p.ks), r0 = 16 * (warp / p.ks);
-#pragma unroll
-    for (int t = 0; t < MT; t++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int m = t * 8 + 2 * lc + (i & 1);
-            if (m < Mb) red[((long)kw * Mb + m) * rows + r0 + lr + 8 * (i >> 1)] = acc[t][i];
-        }
-    __syncthreads();
-    for (int e = tid; e < Mb * rows; e += W4_WARPS * 32) {
-        const int m = e / rows, n = blockIdx.x * rows + e % rows;
-        if (n >= p.N) continue;
-        float v = 0.0f;
-        for (int k = 0; k < p.ks; k++) v += red[(long)k * Mb * rows + e];
-        if (p.bias) v += p.bias[n];
-        const long at = (long)(m0 + m) * p.ldy + n;
-        if (p.y_f32) ((float*)p.y)[at] = v;
-        else ((T*)p.y)[at] = from_f<T>(v);
-    }
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
-template <class T, int VW, int MT> int launch_w4(W4Args& p, cudaStream_t st) {
-    const int PL = sizeof(T) == 2 ? 1 : 3;
-    const int tokens = p.M < 8 * MT ? p.M : 8 * MT;
-    // warps along K while the CTAs are fewer than two per SM
+// d [16 x 8] = a [16 x 16] b [16 x 8]
+__device__ __forceinline__ void mma_bf16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
+// A step is 128 elements of 32 rows (two MMA tiles, which share the activations' operands): four words per lane and row, U blocks of VW words (a quad of lanes covers the 32 VW elements of a block, which
+// are of one group). A CTA's warps are ks along K, the others along the rows; the tokens' activations are staged in chunks, two in shared
+// memory, and serve all its rows. Where one chunk holds them all, a CTA goes on with further rows. Weights, scales and zero points are asked
+// for D steps ahead, over the end of a chunk and of the rows. MT tiles of 8 tokens.
+// In shared memory 32 elements, those of one word of a quad's lanes, lie together for all tokens: [chunk][8 MT tokens][64 bytes], so that eight
+// lanes read 128 bytes in a row and every address but the step's is a constant.
+// PACKED: K of whole steps, a group per block, bf16 scales: a step's scales and zero points come in one load each.
+template <class T, int VW, int MT, bool PACKED>
+__global__ void __launch_bounds__(kWarps<MT> * 32, 1) linear_w4_kernel(const __grid_constant__ W4Args p) {
+    constexpr int PL = sizeof(T) == 2 ? 1 : 3, NW = kWarps<MT>;
+    constexpr int BK = 32 * VW, U = 4 / VW;                // elements of a block, blocks per step
+    constexpr int D = 2;
+    constexpr int XC = 8 * MT * 64, XS = 4 * XC;           // bytes of 32 elements of all tokens, of a step
+    constexpr int SW = PACKED ? (U + 1) / 2 : U, ZW = PACKED ? 1 : U;
+    extern __shared__ __align__(16) uint8_t x_sm[];        // [2][PL][steps] XS
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, lr = lane >> 2, lc = lane & 3;
+    const int m0 = blockIdx.y * 64, Mb = min(p.M - m0, 8 * MT);
+    const int kw = warp & (p.ks - 1), per_cta = NW / p.ks, rows = 32 * per_cta, r0 = 32 * (warp / p.ks);
+    const int groups = p.K / p.group, plane = p.steps * XS;
+    // a step's words, scales and zero points of this lane's four rows, as they are in memory: a conversion here would wait for the load
+    struct Step { Words<VW> w[4][U]; uint32_t s[4][SW], z[4][ZW]; };
+    auto scale_of = [&](const uint32_t (&v)[SW], int u) {
+        if (PACKED) return __uint_as_float(u & 1 ? v[u >> 1] & 0xffff0000u : v[u >> 1] << 16);
+        return __uint_as_float(p.scale_f32 ? v[u % SW] : v[u % SW] << 16);
+    };
+    auto zero_of = [&](const uint32_t (&v)[ZW], int u) {           // 128 + z, twice
+        return zero2(PACKED ? v[0] >> (8 * u) : v[u % ZW]);
+    };
+    // the next step to ask for: its round (ks steps side by side) and, with 32-bit offsets of this lane's rows from the tile's first row
+    const int all = (p.K + kStep - 1) / kStep, rounds = (all + p.ks - 1) / p.ks;
+    int f_round = 0, f_tile = blockIdx.x;
+    uint32_t w_at[4], g_at[4];
+    auto aim = [&] {
+        const int last = max(p.N - 1 - f_tile * rows, 0);
+        if (f_tile * rows >= p.N) f_tile = 0;             // behind the last rows: something to load, not used
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const uint32_t n = min(r0 + lr + 8 * r, last);
+            w_at[r] = n * (p.K / 2) + lc * 4 * VW; g_at[r] = n * groups;
+        }
+    };
+    auto fetch = [&](Step& s) {
+        const long row0 = (long)f_tile * rows;
+        // in the last round a warp may have no step: something to load, not used
+        const int st = f_round * p.ks + kw < all ? kw : 0;
+        if (PACKED) {
+            const uint8_t* w = p.w + row0 * (p.K / 2) + (f_round * p.ks + st) * (kStep / 2);
+            const long g0 = row0 * groups + (f_round * p.ks + st) * U;
+            const uint16_t* sc = (const uint16_t*)p.scale + g0;
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+#pragma unroll
+                for (int u = 0; u < U; u++) s.w[r][u] = load_words<VW>(w + w_at[r] + u * (BK / 2));
+                if (U == 1) s.s[r][0] = sc[g_at[r]];
+                else if (U == 2) s.s[r][0] = *(const uint32_t*)(sc + g_at[r]);
+                else {
+                    const uint2 x = *(const uint2*)(sc + g_at[r]);
+                    s.s[r][0] = x.x; s.s[r][1 % SW] = x.y;
+                }
+                s.z[r][0] = 0x08080808u;
+            }
+            if (p.zero) {
+                const uint8_t* z = p.zero + g0;
+#pragma unroll
+                for (int r = 0; r < 4; r++) s.z[r][0] = U == 1 ? z[g_at[r]] : U == 2 ? *(const uint16_t*)(z + g_at[r]) : *(const uint32_t*)(z + g_at[r]);
+            }
+        } else {
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int k = min((f_round * p.ks + st) * kStep + u * BK, p.K - BK), g = p.per_group == 1 ? k / BK : (int)__umulhi(k / BK, p.magic);
+                const uint8_t* w = p.w + row0 * (p.K / 2) + k / 2;
+                const long g0 = row0 * groups + g;
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    s.w[r][u] = load_words<VW>(w + w_at[r]);
+                    s.s[r][u % SW] = p.scale_f32 ? ((const uint32_t*)p.scale)[g0 + g_at[r]] : (uint32_t)((const uint16_t*)p.scale)[g0 + g_at[r]];
+                    s.z[r][u % ZW] = 8;
+                    if (p.zero) s.z[r][u % ZW] = p.zero[g0 + g_at[r]];
+                }
+            }
+        }
+        if (++f_round == rounds) { f_round = 0; f_tile += gridDim.x; aim(); }
+    };
+    // Activations of a chunk into its buffer, 16 bytes per lane: 4 VW lanes read the 64 VW bytes of a token's block in a row. Elements k .. k + 7 of
+    // lane c's word j are k = BK block + 8 VW c + 8 j.
+    const int kc = p.steps * kStep;
+    auto pieces = [&](int chunk, auto f) {
+        constexpr int LT = 4 * VW, TW = 32 / LT;           // lanes of a token, tokens of a warp
+        const int n = min(kc, p.K - chunk * kc) / BK, piece = lane % LT, c = piece / VW, j = piece % VW;
+        uint8_t* to = x_sm + (chunk & 1) * PL * plane + j * XC + (lane / LT) * 64 + c * 16;
+        const int k = chunk * kc + piece * 8;
+        for (int e = warp; e < n * (8 * MT / TW); e += NW) {
+            const int b = e / (8 * MT / TW), mt = (e - b * (8 * MT / TW)) * TW, m = mt + lane / LT;
+            if (m < Mb) f(to + b * VW * XC + mt * 64, m, k + b * BK);
+        }
+    };
+    auto stage = [&](int chunk) {
+        pieces(chunk, [&](uint8_t* to, int m, int k) {
+            const T* src = (const T*)p.a + (long)(m0 + m) * p.lda + k;
+            if (PL == 1) copy16((uint32_t)__cvta_generic_to_shared(to), src);
+            else {
+                const Eight x = eight((const float*)src);
+#pragma unroll
+                for (int q = 0; q < 3; q++) *reinterpret_cast<uint4*>(to + q * plane) = x.part[q];
+            }
+        });
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    // the same pieces once they are there: their elements in the order of the weights' pairs
+    auto settle = [&](int chunk) {
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        if (PL == 1) pieces(chunk, [&](uint8_t* at, int, int) { *reinterpret_cast<uint4*>(at) = pairs(*reinterpret_cast<const uint4*>(at)); });
+    };
+    float acc[2][MT][4];
+    auto clear = [&] {
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int t = 0; t < MT; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) acc[h][t][i] = 0.0f;
+    };
+    // one step of the warp: elements k0 .. of its rows, activations at xb
+    auto multiply = [&](const Step& cur, int k0, const uint8_t* xb) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (!PACKED && k0 + u * BK >= p.K) break;
+            float sc[4], part[2][MT][4];
+            uint32_t z[4];
+#pragma unroll
+            for (int r = 0; r < 4; r++) { z[r] = zero_of(cur.z[r], u); sc[r] = scale_of(cur.s[r], u); }
+#pragma unroll
+            for (int j = 0; j < VW; j++) {
+                uint32_t a[4][4];
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) a[r][i] = weights2(cur.w[r][u].v[j], i, z[r]);
+                // all tiles of tokens in turn, so that a product does not wait for the one in front
+#pragma unroll
+                for (int q = 0; q < PL; q++)
+#pragma unroll
+                    for (int t0 = 0; t0 < MT; t0 += 4) {
+                        uint4 x[4];
+#pragma unroll
+                        for (int t = t0; t < t0 + 4 && t < MT; t++) x[t - t0] = *reinterpret_cast<const uint4*>(xb + q * plane + (u * VW + j) * XC + t * 512);
+#pragma unroll
+                        for (int t = t0; t < t0 + 4 && t < MT; t++)
+#pragma unroll
+                            for (int h = 0; h < 2; h++) {
+                                if (j == 0 && q == 0) mma_bf16_first(part[h][t], a[2 * h][0], a[2 * h + 1][0], a[2 * h][1], a[2 * h + 1][1], x[t - t0].x, x[t - t0].y);
+                                else mma_bf16(part[h][t], a[2 * h][0], a[2 * h + 1][0], a[2 * h][1], a[2 * h + 1][1], x[t - t0].x, x[t - t0].y);
+                            }
+#pragma unroll
+                        for (int t = t0; t < t0 + 4 && t < MT; t++)
+#pragma unroll
+                            for (int h = 0; h < 2; h++) mma_bf16(part[h][t], a[2 * h][2], a[2 * h + 1][2], a[2 * h][3], a[2 * h + 1][3], x[t - t0].z, x[t - t0].w);
+                    }
+            }
+#pragma unroll
+            for (int t = 0; t < MT; t++)
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) acc[h][t][i] = __fmaf_rn(part[h][t][i], sc[2 * h + (i >> 1)], acc[h][t][i]);
+        }
+    };
+    // the warps' parts of K, joined in their order; [ks][tokens][rows of the CTA + 4], behind the activations when these are needed again
+    float* red = reinterpret_cast<float*>(x_sm + p.red_at);
+    const int red_row = rows + 4;
+    auto finish = [&](int tile) {
+        __syncthreads();
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+#pragma unroll
+            for (int t = 0; t < MT; t++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int m = t * 8 + 2 * lc + (i & 1);
+                    if (m < Mb) red[(kw * Mb + m) * red_row + r0 + 16 * h + lr + 8 * (i >> 1)] = acc[h][t][i];
+                }
+        __syncthreads();
+        for (int e0 = tid; e0 < Mb * rows; e0 += 4 * NW * 32) {
+            float v[4];
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                const int e = min(e0 + x * NW * 32, Mb * rows - 1), at = (e >> p.rows_log) * red_row + (e & (rows - 1));
+                v[x] = 0.0f;
+                for (int k = 0; k < p.ks; k++) v[x] += red[k * Mb * red_row + at];
+            }
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                const int e = e0 + x * NW * 32, m = e >> p.rows_log, n = tile * rows + (e & (rows - 1));
+                if (m >= Mb || n >= p.N) continue;
+                if (p.bias) v[x] += p.bias[n];
+                const long at = (long)(m0 + m) * p.ldy + n;
+                if (p.y_f32) ((float*)p.y)[at] = v[x];
+                else ((T*)p.y)[at] = from_f<T>(v[x]);
+            }
+        }
+    };
+    pdl_sync();
+    stage(0);
+    Step ring[D];
+    aim();
+#pragma unroll
+    for (int d = 0; d < D; d++) fetch(ring[d]);
+    clear();
+    const int per_chunk = p.chunks > 1 ? p.steps / p.ks : rounds;      // rounds
+    int tile = blockIdx.x, round = 0, chunk = 0, left = 0;             // left: rounds of the chunk at hand
+    // a ring slot is refilled where it was used, with its index known to the compiler: moved from register to register, a load would be waited for
+    while (tile * rows < p.N)
+#pragma unroll
+        for (int d = 0; d < D; d++) {
+            if (tile * rows >= p.N) break;
+            if (left == 0) {
+                if (tile == blockIdx.x) {
+                    settle(chunk);
+                    __syncthreads();                       // the chunk is there, the one before has been read
+                    if (chunk + 1 < p.chunks) stage(chunk + 1);
+                }
+                left = per_chunk;
+            }
+            const int st = round * p.ks + kw;
+            if (st < all) multiply(ring[d], st * kStep, x_sm + (chunk & 1) * PL * plane + (st - chunk * p.steps) * XS + lr * 64 + lc * 16);
+            fetch(ring[d]);
+            if (--left == 0) chunk++;
+            if (++round == rounds) {
+                finish(tile);
+                clear();
+                round = chunk = left = 0;
+                tile += gridDim.x;
+            }
+        }
+}
+
+template <class T, int VW, int MT, bool PACKED> int launch_w4(W4Args& p, cudaStream_t st) {
+    constexpr int NW = kWarps<MT>, PL = sizeof(T) == 2 ? 1 : 3, per_step = PL * 8 * MT * 2 * kStep;       // bytes of activations
+    const int all = (p.K + kStep - 1) / kStep;             // steps of a row
+    p.per_group = p.group / (32 * VW);
+    p.magic = (uint32_t)(((1ull << 32) + p.per_group - 1) / p.per_group);
+    // warps along K while their CTAs find an SM each and every warp keeps a step
     p.ks = 1;
-    const long tiles = (p.N + 15) / 16;
-    while (p.ks < W4_WARPS && tiles * p.ks < 2L * W4_WARPS * gemm_sm_count()) p.ks *= 2;
-    const int least = 32 * VW * p.ks;                     // a block for every warp
-    const int most = 96 * 1024 / (PL * tokens * 2) / 128 * 128;
-    p.kc = p.K <= most ? p.K : most;
-    if (p.kc < p.K && p.kc > least) p.kc = p.kc / least * least;
-    const size_t pitch = (size_t)p.kc * 2 + ((p.kc & 63) ? 0 : 64);
-    size_t smem = pitch * PL * tokens;
-    const size_t red = (size_t)W4_WARPS * 16 * tokens * 4;
-    if (red > smem) smem = red;
-    auto kern = linear_w4_kernel<T, VW, MT>;
+    const long tiles = (p.N + 31) / 32, sms = gemm_sm_count();
+    while (p.ks < NW && 2 * p.ks <= all && (tiles * 2 * p.ks + NW - 1) / NW <= sms) p.ks *= 2;
+    // all activations at once, or two chunks in turn
+    const int tokens = p.M < 8 * MT ? p.M : 8 * MT, red = NW * 36 * tokens * 4, room = 220 * 1024;
+    int steps = (room - red) / per_step;
+    if (steps < all) steps = room / 2 / per_step;
+    while (p.ks > steps) p.ks /= 2;
+    p.steps = steps < all ? steps / p.ks * p.ks : all;
+    p.chunks = (all + p.steps - 1) / p.steps;
+    const int x_bytes = p.steps * per_step;
+    p.red_at = p.chunks > 1 ? 0 : x_bytes;
+    const size_t smem = p.chunks > 1 ? (2 * x_bytes > red ? 2 * x_bytes : red) : x_bytes + red;
+    const int per_cta = NW / p.ks;
+    for (p.rows_log = 5; 32 * per_cta > 1 << p.rows_log;) p.rows_log++;
+    auto kern = linear_w4_kernel<T, VW, MT, PACKED>;
     TRY_RC(allow_shared(kern, smem));
-    const long ctas = (tiles * p.ks + W4_WARPS - 1) / W4_WARPS;
-    launch_k(kern, dim3((unsigned)ctas, (p.M + 63) / 64), dim3(W4_WARPS * 32), smem, st, p);
+    long ctas = (tiles + per_cta - 1) / per_cta;
+    if (p.chunks == 1 && ctas > sms) ctas = sms;
+    launch_k(kern, dim3((unsigned)ctas, (p.M + 63) / 64), dim3(NW * 32), smem, st, p);
     return launch_status();
 }
-template <class T, int VW> int pick_w4(W4Args& p, cudaStream_t st) {
-    if (p.M <= 8) return launch_w4<T, VW, 1>(p, st);
-    if (p.M <= 16) return launch_w4<T, VW, 2>(p, st);
-    if (p.M <= 32) return launch_w4<T, VW, 4>(p, st);
-    return launch_w4<T, VW, 8>(p, st);
+bool packed_groups(const W4Args& p, int block) { return !p.scale_f32 && p.group == block && p.K % kStep == 0 && aligned(p.scale, 8) && aligned(p.zero, 4); }
+template <int VW> int run_w4(W4Args& p, const bf16*, cudaStream_t st) {
+    return packed_groups(p, 32 * VW) ? launch_w4<bf16, VW, 1, true>(p, st) : launch_w4<bf16, VW, 1, false>(p, st);
 }
-template <class T> int run_w4(W4Args& p, cudaStream_t st) {
-    if (p.group % 128 == 0) return pick_w4<T, 4>(p, st);
-    if (p.group % 64 == 0) return pick_w4<T, 2>(p, st);
-    return pick_w4<T, 1>(p, st);
+template <int VW> int run_w4(W4Args& p, const float*, cudaStream_t st) {
+    if (p.M <= 8) return packed_groups(p, 32 * VW) ? launch_w4<float, VW, 1, true>(p, st) : launch_w4<float, VW, 1, false>(p, st);
+    if (p.M <= 32) return launch_w4<float, VW, 4, false>(p, st);
+    return launch_w4<float, VW, 8, false>(p, st);
+}
+template <class T> int pick_w4(W4Args& p, cudaStream_t st) {
+    if (p.group % 128 == 0) return run_w4<4>(p, (const T*)p.a, st);
+    if (p.group % 64 == 0) return run_w4<2>(p, (const T*)p.a, st);
+    return run_w4<1>(p, (const T*)p.a, st);
 }
 
 }  // namespace
@@ -229,10 +356,13 @@ extern "C" int flexllm_linear_w4(int dtype, const void* a, long lda, const uint8
                                  const float* bias, int M, int N, int K, void* y, long ldy, int y_f32, void* stream) {
     FLEXLLM_REQUIRE((dtype == FLEXLLM_F32 || dtype == FLEXLLM_BF16) && (scale_dtype == FLEXLLM_F32 || scale_dtype == FLEXLLM_BF16));
     FLEXLLM_REQUIRE(M >= 0 && N > 0 && K > 0 && group > 0 && group % 32 == 0 && K % group == 0 && lda >= K && lda % 8 == 0 && ldy >= N);
-    if ((M + 63) / 64 > 65535) return FLEXLLM_ENOTSUP;
+    if ((M + 63) / 64 > 65535 || K > 1 << 20) return FLEXLLM_ENOTSUP;
     if (M == 0) return FLEXLLM_OK;
     FLEXLLM_REQUIRE(a && w && scale && y && aligned(a, 16) && aligned(w, 16));
-    W4Args p = {a, lda, w, scale, scale_dtype == FLEXLLM_F32, zero, group, bias, M, N, K, y, ldy, y_f32 != 0, 1, 0};
+    const W4Call c = {a, lda, w, scale, scale_dtype == FLEXLLM_F32, zero, group, bias, M, N, K, y, ldy, y_f32 != 0};
     const SetUpEarly early;
-    return dtype == FLEXLLM_BF16 ? run_w4<bf16>(p, (cudaStream_t)stream) : run_w4<float>(p, (cudaStream_t)stream);
+    if (dtype == FLEXLLM_BF16 && M > 8) return linear_w4_tc(c, (cudaStream_t)stream);
+    W4Args p = {};
+    static_cast<W4Call&>(p) = c;
+    return dtype == FLEXLLM_BF16 ? pick_w4<bf16>(p, (cudaStream_t)stream) : pick_w4<float>(p, (cudaStream_t)stream);
 }

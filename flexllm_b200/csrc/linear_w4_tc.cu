@@ -1,0 +1,278 @@
+// Products with 4-bit weights and bf16 activations on the tensor cores (tcgen05), for more than a few tokens:
+//   y[m][n] = sum_groups s[n][g] * sum_{k in g} a[m][k] (q[n][k] - z[n][g])
+// Weights are on the 128-row side, up to 64 tokens on the other. A CTA walks K in steps of 128:
+//   warp 12        brings words (eight steps ahead) and activations by TMA
+//   warps 4 .. 11  put q - z, exact in bf16, into swizzled shared memory. They load nothing from memory themselves: their fence towards the
+//                  tensor core would wait for it (words in registers, asked for four steps ahead: 18.8 us for 48 x 16384 x 2048)
+//   warp 13        issues the MMAs, accumulators of their own for each group of a step, two steps' worth
+//   warps 0 .. 3   take a step's sums out of TMEM and add them up in fp32 registers, times the groups' scales: no weight is ever rounded;
+//                  they also hand the zero points to the converting warps
+// Few rows: the CTAs of a cluster cut K, and their sums meet in shared memory, in a fixed order.
+// Bound by the chain of a step: one thread's waits and eight MMAs, beside it the conversion, about two instructions for half a byte.
+#include "linear_w4.h"
+#include "tc_common.cuh"
+
+namespace flexllm {
+
+using namespace tc;
+
+namespace {
+
+constexpr int kStepK = 128, kStages = 3, kWords = 8, kTcThreads = 448;
+
+struct W4Tc {
+    W4Call c;
+    int steps, n_split;
+    int* error_flag;
+    int per_group; uint32_t magic;         // blocks of a group, and 2^32 / per_group rounded up: the quotient of block numbers below 2^16
+};
+// shared memory: A [stage][2][128 rows][128 bytes], activations [stage][2][NT][128 bytes], words [kWords][128 rows][64 bytes], zero points [stage][4][128]
+constexpr uint32_t kXAt = kStages * 32768u;
+template <int NT> constexpr uint32_t kWAt = kXAt + kStages * NT * 256u;
+template <int NT> constexpr uint32_t kZAt = kWAt<NT> + kWords * 8192u;
+template <int NT> constexpr uint32_t kBarsAt = kZAt<NT> + kStages * 512u;
+template <int NT> constexpr uint32_t kTcSmem = kBarsAt<NT> + 512u + 1024u;
+
+// U groups (or parts of one) per step
+template <int NT, int U>
+__global__ void __launch_bounds__(kTcThreads, 1) linear_w4_tc_kernel(const __grid_constant__ CUtensorMap tmapX, const __grid_constant__ CUtensorMap tmapW,
+                                                                     const __grid_constant__ W4Tc t) {
+    constexpr int BK = kStepK / U;                         // elements of a block
+    extern __shared__ uint8_t smem_raw[];
+    const W4Call& c = t.c;
+    const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+    uint8_t* base_ptr = smem_raw + (base - raw);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(base_ptr + kBarsAt<NT>);
+    // operands there (conversion and activations) and read; sums there and read; words there; zero points there
+    const uint32_t bar_a = smem_u32(bars), bar_e = bar_a + 8 * kStages, bar_d = bar_e + 8 * kStages, bar_de = bar_d + 16, bar_w = bar_de + 16,
+                   bar_z = bar_w + 8 * kWords;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 32);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    constexpr uint32_t need = 2 * U * NT, cols = need <= 32 ? 32 : need <= 64 ? 64 : need <= 128 ? 128 : need <= 256 ? 256 : 512;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kStages; i++) { mbar_init(bar_a + 8 * i, 9); mbar_init(bar_e + 8 * i, 1); mbar_init(bar_z + 8 * i, 4); }
+        for (int i = 0; i < 2; i++) { mbar_init(bar_d + 8 * i, 1); mbar_init(bar_de + 8 * i, 4); }
+        for (int i = 0; i < kWords; i++) mbar_init(bar_w + 8 * i, 1);
+        *abort_flag = 0;
+        fence_barrier_init();
+    }
+    if (warp == 13) { tmem_alloc(smem_u32(tmem_slot), cols); tmem_relinquish(); }
+    if (warp == 12 && lane == 0) { tma_prefetch_desc(&tmapX); tma_prefetch_desc(&tmapW); }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    pdl_sync();
+    const int split = blockIdx.x % t.n_split, n0 = blockIdx.x / t.n_split * 128, m0 = blockIdx.y * 64;
+    const int s0 = (int)((long)t.steps * split / t.n_split), s1 = (int)((long)t.steps * (split + 1) / t.n_split);
+    // all lanes look: one that looks for the others and tells them takes twice as long
+    auto wait_warp = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_spin(bar, parity, abort_flag)) != 0; };
+    float acc[NT];
+#pragma unroll
+    for (int x = 0; x < NT; x++) acc[x] = 0.0f;
+    if (warp == 12) {
+        if (lane == 0) {
+            // the words of step n lie where those of step n - kWords were, which the conversion has read when the products of that step are done
+            auto words = [&](int n) {
+                if (s0 + n >= s1) return;
+                mbar_expect_tx(bar_w + 8 * (n % kWords), 8192u);
+                tma_load_2d(base + kWAt<NT> + (uint32_t)(n % kWords) * 8192u, &tmapW, bar_w + 8 * (n % kWords), (s0 + n) * (kStepK / 2), n0);
+            };
+            for (int n = 0; n < kWords; n++) words(n);
+            for (int n = 0; s0 + n < s1; n++) {
+                const int st = n % kStages;
+                if (!mbar_spin(bar_e + 8 * st, (uint32_t)(n / kStages & 1) ^ 1u, abort_flag)) break;
+                mbar_expect_tx(bar_a + 8 * st, NT * 256u);
+                for (int b = 0; b < 2; b++)
+                    tma_load_2d(base + kXAt + (uint32_t)(st * 2 + b) * (NT * 128u), &tmapX, bar_a + 8 * st, ((s0 + n) * kStepK + b * 64) * 2, m0);
+                if (n >= kStages) words(n - kStages + kWords);
+            }
+        }
+    } else if (warp == 13) {
+        if (lane == 0) {
+            const uint32_t idesc = umma_idesc_bf16(128, NT), a_lo = umma_desc_lo(base), x_lo = umma_desc_lo(base + kXAt);
+            for (int n = 0; s0 + n < s1; n++) {
+                const int st = n % kStages, buf = n & 1;
+                if (!mbar_spin(bar_de + 8 * buf, (uint32_t)(n >> 1 & 1) ^ 1u, abort_flag)) break;
+                if (!mbar_spin(bar_a + 8 * st, (uint32_t)(n / kStages & 1), abort_flag)) break;
+                tc_fence_after();
+#pragma unroll
+                for (int k = 0; k < 8; k++)
+                    umma_bf16_lo(tmem + (buf * U + k / (8 / U)) * NT, a_lo + st * 2048 + (k >> 2) * 1024 + 2 * (k & 3), x_lo + st * (NT * 16) + (k >> 2) * (NT * 8) + 2 * (k & 3),
+                                 idesc, k % (8 / U) > 0);
+                umma_commit(bar_d + 8 * buf);
+                umma_commit(bar_e + 8 * st);
+            }
+        }
+    } else if (warp >= 4) {
+        // lane: bits 0 - 2 and 4 the row, bit 3 the half of the step, so that eight lanes in a row meet eight different 16-byte columns
+        const int h = lane >> 3 & 1, r = (warp - 4) * 16 + (lane & 7) + (lane >> 4) * 8;
+        uint8_t* to = base_ptr + h * 16384 + r * 128;
+        for (int n = 0; s0 + n < s1; n++) {
+            const int st = n % kStages, sw = n % kWords;
+            if (!wait_warp(bar_w + 8 * sw, (uint32_t)(n / kWords & 1))) break;
+            uint4 v[2];
+#pragma unroll
+            for (int x = 0; x < 2; x++) v[x] = *reinterpret_cast<const uint4*>(base_ptr + kWAt<NT> + sw * 8192 + r * 64 + (((h * 2 + x) ^ (r >> 1 & 3)) << 4));
+            if (!wait_warp(bar_e + 8 * st, (uint32_t)(n / kStages & 1) ^ 1u)) break;
+            uint32_t z[2] = {8u, 8u};
+            if (c.zero) {
+                if (!wait_warp(bar_z + 8 * st, (uint32_t)(n / kStages & 1))) break;
+                const uint8_t* zs = base_ptr + kZAt<NT> + st * 512 + r;
+                z[0] = zs[h * U / 2 * 128];
+                z[1] = U == 4 ? zs[(h * 2 + 1) * 128] : z[0];
+            }
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                const uint32_t z2 = zero2(z[x]);
+                const uint32_t word[4] = {v[x].x, v[x].y, v[x].z, v[x].w};
+#pragma unroll
+                for (int y = 0; y < 4; y++) {
+                    const uint32_t p0 = weights2(word[y], 0, z2), p1 = weights2(word[y], 1, z2), p2 = weights2(word[y], 2, z2), p3 = weights2(word[y], 3, z2);
+                    *reinterpret_cast<uint4*>(to + st * 32768 + (((x * 4 + y) ^ (r & 7)) << 4)) =
+                        make_uint4(pick(p0, p1, 0x5410), pick(p2, p3, 0x5410), pick(p0, p1, 0x7632), pick(p2, p3, 0x7632));
+                }
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_a + 8 * st);
+        }
+    } else {
+        const int groups = c.K / c.group, rr = warp * 32 + lane;
+        const long g0 = (long)min(n0 + rr, c.N - 1) * groups;
+        const uint32_t lane_addr = (uint32_t)(warp * 32) << 16;
+        auto group_at = [&](int i, int u) {               // behind K: the last one, for zeros
+            const int kb = min(i * U + u, c.K / BK - 1);
+            return g0 + (t.per_group == 1 ? kb : (int)__umulhi(kb, t.magic));
+        };
+        uint32_t next[U], zero[U];
+        auto fetch = [&](int i) {
+#pragma unroll
+            for (int u = 0; u < U; u++) next[u] = c.scale_f32 ? ((const uint32_t*)c.scale)[group_at(i, u)] : (uint32_t)((const uint16_t*)c.scale)[group_at(i, u)];
+        };
+        auto fetch_zero = [&](int i) {
+#pragma unroll
+            for (int u = 0; u < U; u++) zero[u] = c.zero[group_at(i, u)];
+        };
+        // zero points of step n, asked for a step ahead, into its slot, which the conversion of step n - kStages has left
+        auto hand_zero = [&](int n) {
+            if (!wait_warp(bar_e + 8 * (n % kStages), (uint32_t)(n / kStages & 1) ^ 1u)) return false;
+#pragma unroll
+            for (int u = 0; u < U; u++) base_ptr[kZAt<NT> + n % kStages * 512 + u * 128 + rr] = (uint8_t)zero[u];
+            fetch_zero(s0 + n + 1);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_z + 8 * (n % kStages));
+            return true;
+        };
+        bool ok = s0 < s1;
+        if (ok) fetch(s0);
+        if (ok && c.zero) {
+            fetch_zero(s0);
+            for (int n = 0; ok && n < 2 && s0 + n < s1; n++) ok = hand_zero(n);
+        }
+        for (int n = 0; ok && s0 + n < s1; n++) {
+            float sc[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) sc[u] = __uint_as_float(c.scale_f32 ? next[u] : next[u] << 16);
+            fetch(s0 + n + 1);
+            ok = wait_warp(bar_d + 8 * (n & 1), (uint32_t)(n >> 1 & 1));
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll
+            for (int x0 = 0; x0 < U * NT; x0 += 16) {
+                uint32_t v[16];
+                tmem_ld_32x16(tmem + (n & 1) * (U * NT) + x0 + lane_addr, v);
+                tmem_ld_wait();
+#pragma unroll
+                for (int x = 0; x < 16; x++) acc[x0 % NT + x] = __fmaf_rn(__uint_as_float(v[x]), sc[x0 / NT], acc[x0 % NT + x]);
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_de + 8 * (n & 1));
+            if (c.zero && s0 + n + 2 < s1) ok = hand_zero(n + 2);
+        }
+    }
+    // the sums into shared memory (every product has been waited for), [token][132]; the CTAs of the cluster join the tokens in turn
+    float* red = reinterpret_cast<float*>(base_ptr);
+    __syncthreads();
+    if (warp < 4)
+#pragma unroll
+        for (int x = 0; x < NT; x++) red[x * 132 + warp * 32 + lane] = acc[x];
+    if (t.n_split > 1) cluster_sync(); else __syncthreads();
+    const int Mb = min(c.M - m0, NT), rows = min(128, c.N - n0);
+    for (int e = threadIdx.x; e < (Mb - split + t.n_split - 1) / t.n_split * 32; e += kTcThreads) {
+        const int m = split + (e >> 5) * t.n_split, r = (e & 31) * 4;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (t.n_split == 1) v = *reinterpret_cast<const float4*>(red + m * 132 + r);
+        else
+            for (int p = 0; p < t.n_split; p++) {
+                const uint32_t at = cluster_addr(base + (uint32_t)(m * 132 + r) * 4u, p);
+                float4 x;
+                asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(at) : "memory");
+                v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
+            }
+        const long at = (long)(m0 + m) * c.ldy + n0 + r;
+        const float f[4] = {v.x, v.y, v.z, v.w};
+        float o[4];
+#pragma unroll
+        for (int x = 0; x < 4; x++) o[x] = f[x] + (c.bias && r + x < rows ? c.bias[n0 + r + x] : 0.0f);
+        const bool whole = r + 4 <= rows && (c.ldy & 3) == 0;
+        if (c.y_f32) {
+            float* y = (float*)c.y + at;
+            if (whole && ((uintptr_t)c.y & 15) == 0) store4(y, make_float4(o[0], o[1], o[2], o[3]));
+            else
+                for (int x = 0; x < 4; x++) if (r + x < rows) y[x] = o[x];
+        } else {
+            bf16* y = (bf16*)c.y + at;
+            if (whole && ((uintptr_t)c.y & 7) == 0) store4(y, make_float4(o[0], o[1], o[2], o[3]));
+            else
+                for (int x = 0; x < 4; x++) if (r + x < rows) y[x] = __float2bfloat16_rn(o[x]);
+        }
+    }
+    if (t.n_split > 1) cluster_sync();
+    tc_fence_before();
+    __syncthreads();
+    if (*abort_flag) {
+        const unsigned long long t_0 = globaltimer_ns();
+        while (globaltimer_ns() - t_0 < 200000ull) { __nanosleep(1000); }
+        if (threadIdx.x == 0 && t.error_flag) atomicOr(t.error_flag, 1);
+        __syncthreads();
+    }
+    if (warp == 13) { tc_fence_after(); tmem_dealloc(tmem, cols); }
+}
+
+template <int NT, int U> int launch_tc(W4Tc& t, cudaStream_t st) {
+    const W4Call& c = t.c;
+    t.steps = (c.K + kStepK - 1) / kStepK;
+    t.per_group = c.group / (kStepK / U);
+    t.magic = (uint32_t)(((1ull << 32) + t.per_group - 1) / t.per_group);
+    const long tiles = (c.N + 127) / 128, sms = gemm_sm_count();
+    t.n_split = 1;
+    while (t.n_split < 8 && tiles * t.n_split * 2 <= sms && t.steps >= 4 * t.n_split) t.n_split *= 2;
+    CUtensorMap tx, tw;
+    TRY_RC(make_tmap_2d_u8_ld(&tx, c.a, (uint64_t)c.M, (uint64_t)c.K * 2, NT, (uint64_t)c.lda * 2));
+    TRY_RC(make_tmap_2d_u8_box(&tw, c.w, (uint64_t)c.N, (uint64_t)c.K / 2, 64, 128, 64));
+    auto kern = linear_w4_tc_kernel<NT, U>;
+    TRY_RC(allow_shared(kern, kTcSmem<NT>));
+    launch_cluster(kern, dim3((unsigned)(tiles * t.n_split), (c.M + 63) / 64), dim3(kTcThreads), t.n_split, kTcSmem<NT>, st, tx, tw, t);
+    return launch_status();
+}
+template <int NT> int pick_tc(W4Tc& t, cudaStream_t st) {
+    if (t.c.group % 128 == 0) return launch_tc<NT, 1>(t, st);
+    if (t.c.group % 64 == 0) return launch_tc<NT, 2>(t, st);
+    return launch_tc<NT, 4>(t, st);
+}
+
+}  // namespace
+
+int linear_w4_tc(const W4Call& c, cudaStream_t st) {
+    W4Tc t = {};
+    t.c = c; t.error_flag = device_error_flag();
+    if (c.M <= 16) return pick_tc<16>(t, st);
+    if (c.M <= 32) return pick_tc<32>(t, st);
+    if (c.M <= 48) return pick_tc<48>(t, st);
+    return pick_tc<64>(t, st);
+}
+
+}  // namespace flexllm
