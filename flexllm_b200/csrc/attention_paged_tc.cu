@@ -69,14 +69,14 @@ __global__ void __launch_bounds__(MODE == kOne ? 192 : 320, MODE == kOne ? 2 : 1
     const TcSmem o = tc_smem(NQ, t.kc, t.vr, t.ks, t.vs);
     uint64_t* bars = reinterpret_cast<uint64_t*>(base_ptr + o.bars);
     const uint32_t bar_q = smem_u32(bars), bar_kf = bar_q + 8, bar_ke = bar_kf + 8 * kMaxStages, bar_vf = bar_ke + 8 * kMaxStages,
-                   bar_ve = bar_vf + 8 * kMaxStages, bar_s = bar_ve + 8 * kMaxStages, bar_p = bar_s + 16, bar_o = bar_p + 16, bar_f = bar_o + 16;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 26);
+                   bar_ve = bar_vf + 8 * kMaxStages, bar_s = bar_ve + 8 * kMaxStages, bar_p = bar_s + 16, bar_o = bar_p + 16, bar_f = bar_o + 16, bar_h = bar_f + 16;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 28);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         mbar_init(bar_q, 1);
         for (int i = 0; i < kMaxStages; i++) { mbar_init(bar_kf + 8 * i, 1); mbar_init(bar_ke + 8 * i, 1); mbar_init(bar_vf + 8 * i, 1); mbar_init(bar_ve + 8 * i, 1); }
-        for (int i = 0; i < 2; i++) { mbar_init(bar_s + 8 * i, 1); mbar_init(bar_p + 8 * i, 4); mbar_init(bar_o + 8 * i, 1); mbar_init(bar_f + 8 * i, 1); }
+        for (int i = 0; i < 2; i++) { mbar_init(bar_s + 8 * i, 1); mbar_init(bar_p + 8 * i, 4); mbar_init(bar_o + 8 * i, 1); mbar_init(bar_f + 8 * i, 1); mbar_init(bar_h + 8 * i, 4); }
         *abort_flag = 0;
         fence_barrier_init();
     }
@@ -177,13 +177,17 @@ __global__ void __launch_bounds__(MODE == kOne ? 192 : 320, MODE == kOne ? 2 : 1
             for (int q = 0; ok && q < NQ; q++) {
                 if (j >= t1[q]) continue;
                 const int w = MODE == kTurns ? n & 1 : q;
-                ok = mbar_spin(bar_p + 8 * w, (uint32_t)(n / STEP & 1), abort_flag);
-                if (!ok) break;
-                tc_fence_after();
                 const uint32_t v_lo = umma_desc_lo(base + o.v + (uint32_t)(sv * 2) * t.vr * 128u), page = (uint32_t)t.vr * 8u;
+                // the weights of the first 64 keys, then the others. A tile that ends early is only right when its values' zeros are there too
+                for (uint32_t half = 0; ok && half < 2; half++) {
+                    ok = mbar_spin((half == 0 && end - j * KT >= KT ? bar_h : bar_p) + 8 * w, (uint32_t)(n / STEP & 1), abort_flag);
+                    if (!ok) break;
+                    tc_fence_after();
 #pragma unroll
-                for (uint32_t k = 0; k < KT / 16; k++)
-                    umma_bf16_ts_lo(tO + w * t.o_stride, tmem + w * KT + 8 * k, v_lo + (k >> 2) * page + 2 * (k & 3), idesc_pv, n >= STEP || k > 0 ? 1u : 0u);
+                    for (uint32_t k = 0; k < 4; k++)
+                        umma_bf16_ts_lo(tO + w * t.o_stride, tmem + w * KT + 32 * half + 8 * k, v_lo + half * page + 2 * k, idesc_pv, n >= STEP || half + k > 0 ? 1u : 0u);
+                }
+                if (!ok) break;
                 umma_commit((j + STEP < t1[q] ? bar_o : bar_f) + 8 * w);        // the last one has a barrier of its own
                 if (q == NQ - 1 || j >= t1[NQ - 1]) umma_commit(bar_ve + 8 * sv);
                 if (j + STEP < t1[q]) ok = qk(w, j + STEP);
@@ -202,7 +206,7 @@ __global__ void __launch_bounds__(MODE == kOne ? 192 : 320, MODE == kOne ? 2 : 1
         const int my_t0 = t0 + w * (STEP - 1), my_t1 = q == 1 ? t1[NQ - 1] : t1[0];
         auto wait_bar = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_spin(bar, parity, abort_flag)) != 0; };
         float m = kNoScore;
-        f32x2 l2 = pack2(0.0f, 0.0f);
+        f32x2 l2[2] = {pack2(0.0f, 0.0f), pack2(0.0f, 0.0f)};
         const f32x2 a22 = pack2(t.a2, t.a2);
         bool ok = true;
         for (int j = my_t0; j < my_t1; j += STEP) {
@@ -215,7 +219,8 @@ __global__ void __launch_bounds__(MODE == kOne ? 192 : 320, MODE == kOne ? 2 : 1
             for (int c = 0; c < 4; c++) tmem_ld_32x32(tS + 32 * c, v[c]);
             tmem_ld_wait();
             const int hi = sure - j * KT;
-            if (!__all_sync(0xffffffffu, hi >= KT)) {
+            const bool masked = !__all_sync(0xffffffffu, hi >= KT);
+            if (masked) {
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
                     const int nv = min(max(hi - 32 * c, 0), 32), sh = 32 * c - (s.ctx - j * KT);
@@ -238,7 +243,7 @@ __global__ void __launch_bounds__(MODE == kOne ? 192 : 320, MODE == kOne ? 2 : 1
             if (__any_sync(0xffffffffu, grow)) {
                 const float m_new = grow ? top : m, al = ex2_fast(m - m_new);
                 m = m_new;
-                l2 = mul2(l2, pack2(al, al));
+                l2[0] = mul2(l2[0], pack2(al, al)); l2[1] = mul2(l2[1], pack2(al, al));
                 if (turn > 0) {
                     if (!wait_bar(bar_o + 8 * w, (uint32_t)((turn - 1) & 1))) { ok = false; break; }      // the products so far
                     tc_fence_after();
@@ -261,10 +266,16 @@ __global__ void __launch_bounds__(MODE == kOne ? 192 : 320, MODE == kOne ? 2 : 1
                     float e0, e1;
                     unpack2(fma2(pack2(__uint_as_float(v[c][x]), __uint_as_float(v[c][x + 1])), a22, nm), e0, e1);
                     e0 = ex2_fast(e0); e1 = ex2_fast(e1);
-                    l2 = add2(l2, pack2(e0, e1));
+                    l2[(x >> 1) & 1] = add2(l2[(x >> 1) & 1], pack2(e0, e1));
                     pk[x >> 1] = bf_pack(e0, e1);
                 }
                 tmem_st_32x16(tS + 16 * c, pk);
+                if (c == 1) {                             // half the weights are there: their product may start
+                    tmem_st_wait();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar_h + 8 * w);
+                }
             }
             if (left < KT) {                              // the sequence ends inside the tile: zeros for the values behind its end
                 const int sv = n % t.vs, c0 = left >> 3;
@@ -286,7 +297,7 @@ __global__ void __launch_bounds__(MODE == kOne ? 192 : 320, MODE == kOne ? 2 : 1
             if (lane == 0) mbar_arrive(bar_p + 8 * w);
         }
         float l, l1;
-        unpack2(l2, l, l1);
+        unpack2(add2(l2[0], l2[1]), l, l1);
         l += l1;
         const bool any = my_t0 < my_t1;
         if (ok && any) ok = wait_bar(bar_f + 8 * w, 0);
