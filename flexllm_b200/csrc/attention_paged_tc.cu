@@ -34,6 +34,13 @@ struct TcArgs {
     float a2;                              // scale * log2 e
     int tmem_cols, o_stride, n_split;
 };
+// Stage of a ring and the parity of its round, counted up: a quotient by a stage count that is only known at run time takes one thread 250 clocks
+// (a tile's four of them took as long as its products).
+struct Ring {
+    int st; uint32_t ph; const int n;
+    __device__ __forceinline__ Ring(int n_, int at) : st(at % n_), ph((uint32_t)(at / n_) & 1u), n(n_) {}
+    __device__ __forceinline__ void next() { if (++st == n) { st = 0; ph ^= 1u; } }
+};
 struct TcSmem { uint32_t k, v, bars, total; };
 __host__ __device__ inline TcSmem tc_smem(int NQ, int kc, int vr, int ks, int vs) {
     TcSmem o;
@@ -120,20 +127,21 @@ __global__ void __launch_bounds__(MODE == kOne ? 192 : 320, MODE == kOne ? 2 : 1
         }
         const int n_pg = (end + kPage - 1) / kPage;
         int ids = 0;
-        for (int j = t0; j < t_last; j++) {
-            const int n = j - t0, sk = n % t.ks, sv = n % t.vs;
+        Ring rk(t.ks, 0), rv(t.vs, 0);
+        for (int j = t0; j < t_last; j++, rk.next(), rv.next()) {
+            const int n = j - t0, sk = rk.st, sv = rv.st;
             if ((n & 15) == 0) ids = 2 * j + lane < n_pg ? page_of(a.seq, b, 2 * j + lane) : 0;
             const int p0 = __shfl_sync(0xffffffffu, ids, 2 * (n & 15)), p1 = __shfl_sync(0xffffffffu, ids, 2 * (n & 15) + 1);
             const int pages = 2 * j + 1 < n_pg ? 2 : 1;
             int ok = 1;
             if (lane == 0) {
-                ok = mbar_spin(bar_ke + 8 * sk, (uint32_t)(n / t.ks & 1) ^ 1u, abort_flag);
+                ok = mbar_spin(bar_ke + 8 * sk, rk.ph ^ 1u, abort_flag);
                 if (ok) {
                     mbar_expect_tx(bar_kf + 8 * sk, (uint32_t)(t.kc * pages) * 8192u);
                     for (int p = 0; p < pages; p++)
                         for (int i = 0; i < t.kc; i++)
                             tma_load_2d(base + o.k + (uint32_t)(sk * t.kc + i) * 16384u + p * 8192u, &tmapK, bar_kf + 8 * sk, i * 128, ((p ? p1 : p0) * a.G + g) * kPage);
-                    ok = mbar_spin(bar_ve + 8 * sv, (uint32_t)(n / t.vs & 1) ^ 1u, abort_flag);
+                    ok = mbar_spin(bar_ve + 8 * sv, rv.ph ^ 1u, abort_flag);
                 }
                 if (ok) {
                     mbar_expect_tx(bar_vf + 8 * sv, (uint32_t)(t.vr * pages) * 128u);
@@ -150,9 +158,9 @@ __global__ void __launch_bounds__(MODE == kOne ? 192 : 320, MODE == kOne ? 2 : 1
         if (lane == 0) {
         bool ok = t0 < t_last;
         // S of set w = Q K_j^T, over the weights that the product in front has read
-        auto qk = [&](int w, int j) {
-            const int n = j - t0, sk = n % t.ks, q = NQ == 2 ? w : 0;
-            if (!mbar_spin(bar_kf + 8 * sk, (uint32_t)(n / t.ks & 1), abort_flag)) return false;
+        auto qk = [&](int w, int j, const Ring& r) {
+            const int sk = r.st, q = NQ == 2 ? w : 0;
+            if (!mbar_spin(bar_kf + 8 * sk, r.ph, abort_flag)) return false;
             tc_fence_after();
             const uint32_t q_lo = umma_desc_lo(base + (uint32_t)(q * t.kc) * 16384u), k_lo = umma_desc_lo(base + o.k + (uint32_t)(sk * t.kc) * 16384u);
             auto four = [&](uint32_t blk) {
@@ -169,11 +177,12 @@ __global__ void __launch_bounds__(MODE == kOne ? 192 : 320, MODE == kOne ? 2 : 1
         if (ok) ok = mbar_spin(bar_q, 0, abort_flag);
         for (int w = 0; w < W; w++) {
             const int j = t0 + w * (STEP - 1);
-            if (ok && j < t1[NQ == 2 ? w : 0]) ok = qk(w, j);
+            if (ok && j < t1[NQ == 2 ? w : 0]) ok = qk(w, j, Ring(t.ks, j - t0));
         }
-        for (int j = t0; ok && j < t_last; j++) {
-            const int n = j - t0, sv = n % t.vs;
-            if (ok) ok = mbar_spin(bar_vf + 8 * sv, (uint32_t)(n / t.vs & 1), abort_flag);
+        Ring rk(t.ks, STEP), rv(t.vs, 0);                  // K of the tile that follows in the same set, V of this one
+        for (int j = t0; ok && j < t_last; j++, rk.next(), rv.next()) {
+            const int n = j - t0, sv = rv.st;
+            if (ok) ok = mbar_spin(bar_vf + 8 * sv, rv.ph, abort_flag);
             for (int q = 0; ok && q < NQ; q++) {
                 if (j >= t1[q]) continue;
                 const int w = MODE == kTurns ? n & 1 : q;
@@ -190,7 +199,7 @@ __global__ void __launch_bounds__(MODE == kOne ? 192 : 320, MODE == kOne ? 2 : 1
                 if (!ok) break;
                 umma_commit((j + STEP < t1[q] ? bar_o : bar_f) + 8 * w);        // the last one has a barrier of its own
                 if (q == NQ - 1 || j >= t1[NQ - 1]) umma_commit(bar_ve + 8 * sv);
-                if (j + STEP < t1[q]) ok = qk(w, j + STEP);
+                if (j + STEP < t1[q]) ok = qk(w, j + STEP, rk);
             }
         }
         }
