@@ -154,54 +154,58 @@ __global__ void __launch_bounds__(MODE == kOne ? 192 : 320, MODE == kOne ? 2 : 1
     } else if (warp == WM) {
         const uint32_t idesc_qk = umma_idesc_bf16(128, KT), idesc_pv = umma_idesc_bf16(128, t.vr);
         const int ksteps = (a.dk + 15) / 16;
-        const uint32_t tO = tmem + W * KT;
-        if (lane == 0) {
-        bool ok = t0 < t_last;
+        const uint32_t leader = elect_leader();
+        // the same for all lanes, and known to be: the bounds of this warp's loops
+        const int u0 = uniform_max(t0), u_last = uniform_max(t_last), u_end = uniform_max(end);
+        int u1[NQ];
+#pragma unroll
+        for (int q = 0; q < NQ; q++) u1[q] = uniform_max(t1[q]);
+        auto wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_spin(bar, parity, abort_flag)) != 0; };
+        const uint32_t u_tmem = (uint32_t)uniform_max((int)tmem), tP = u_tmem + W * KT, page = (uint32_t)t.vr * 8u;
+        const uint32_t q_lo = umma_desc_lo(base), k_lo = umma_desc_lo(base + o.k), v_lo = umma_desc_lo(base + o.v);
         // S of set w = Q K_j^T, over the weights that the product in front has read
         auto qk = [&](int w, int j, const Ring& r) {
-            const int sk = r.st, q = NQ == 2 ? w : 0;
-            if (!mbar_spin(bar_kf + 8 * sk, r.ph, abort_flag)) return false;
+            const int q = NQ == 2 ? w : 0;
+            if (!wait(bar_kf + 8 * r.st, r.ph)) return false;
             tc_fence_after();
-            const uint32_t q_lo = umma_desc_lo(base + (uint32_t)(q * t.kc) * 16384u), k_lo = umma_desc_lo(base + o.k + (uint32_t)(sk * t.kc) * 16384u);
-            auto four = [&](uint32_t blk) {
+            const uint32_t a_at = q_lo + (uint32_t)(q * t.kc) * 1024u, b_at = k_lo + (uint32_t)(r.st * t.kc) * 1024u, d_at = u_tmem + w * KT;
+            for (int blk = 0; blk < ksteps >> 2; blk++)
 #pragma unroll
-                for (uint32_t k = 0; k < 4; k++) umma_bf16_lo(tmem + w * KT, q_lo + blk * 1024u + 2 * k, k_lo + blk * 1024u + 2 * k, idesc_qk, blk + k > 0);
-            };
-            for (int blk = 0; blk < ksteps >> 2; blk++) four(blk);
+                for (uint32_t k = 0; k < 4; k++) umma_bf16_lo(leader, d_at, a_at + blk * 1024u + 2 * k, b_at + blk * 1024u + 2 * k, idesc_qk, blk + k > 0);
             for (int k = ksteps & ~3; k < ksteps; k++)
-                umma_bf16_lo(tmem + w * KT, q_lo + (k >> 2) * 1024u + 2 * (k & 3), k_lo + (k >> 2) * 1024u + 2 * (k & 3), idesc_qk, k > 0);
-            umma_commit(bar_s + 8 * w);
-            if (q == NQ - 1 || j >= t1[NQ - 1]) umma_commit(bar_ke + 8 * sk);      // the last product with K_j
+                umma_bf16_lo(leader, d_at, a_at + (k >> 2) * 1024u + 2 * (k & 3), b_at + (k >> 2) * 1024u + 2 * (k & 3), idesc_qk, k > 0);
+            umma_commit_by(leader, bar_s + 8 * w);
+            if (q == NQ - 1 || j >= u1[NQ - 1]) umma_commit_by(leader, bar_ke + 8 * r.st);      // the last product with K_j
             return true;
         };
-        if (ok) ok = mbar_spin(bar_q, 0, abort_flag);
+        bool ok = u0 < u_last && wait(bar_q, 0);
         for (int w = 0; w < W; w++) {
-            const int j = t0 + w * (STEP - 1);
-            if (ok && j < t1[NQ == 2 ? w : 0]) ok = qk(w, j, Ring(t.ks, j - t0));
+            const int j = u0 + w * (STEP - 1);
+            if (ok && j < u1[NQ == 2 ? w : 0]) ok = qk(w, j, Ring(t.ks, j - u0));
         }
         Ring rk(t.ks, STEP), rv(t.vs, 0);                  // K of the tile that follows in the same set, V of this one
-        for (int j = t0; ok && j < t_last; j++, rk.next(), rv.next()) {
-            const int n = j - t0, sv = rv.st;
-            if (ok) ok = mbar_spin(bar_vf + 8 * sv, rv.ph, abort_flag);
-            for (int q = 0; ok && q < NQ; q++) {
-                if (j >= t1[q]) continue;
+        for (int j = u0; ok && j < u_last; j++, rk.next(), rv.next()) {
+            const int n = j - u0;
+            ok = wait(bar_vf + 8 * rv.st, rv.ph);
+#pragma unroll
+            for (int q = 0; q < NQ; q++) {
+                if (!ok || j >= u1[q]) continue;
                 const int w = MODE == kTurns ? n & 1 : q;
-                const uint32_t v_lo = umma_desc_lo(base + o.v + (uint32_t)(sv * 2) * t.vr * 128u), page = (uint32_t)t.vr * 8u;
+                const uint32_t b_at = v_lo + (uint32_t)(rv.st * 2) * page, p_at = u_tmem + w * KT, d_at = tP + w * t.o_stride;
                 // the weights of the first 64 keys, then the others. A tile that ends early is only right when its values' zeros are there too
-                for (uint32_t half = 0; ok && half < 2; half++) {
-                    ok = mbar_spin((half == 0 && end - j * KT >= KT ? bar_h : bar_p) + 8 * w, (uint32_t)(n / STEP & 1), abort_flag);
+#pragma unroll
+                for (uint32_t half = 0; half < 2; half++) {
+                    ok = ok && wait((half == 0 && u_end - j * KT >= KT ? bar_h : bar_p) + 8 * w, (uint32_t)(n / STEP & 1));
                     if (!ok) break;
                     tc_fence_after();
 #pragma unroll
-                    for (uint32_t k = 0; k < 4; k++)
-                        umma_bf16_ts_lo(tO + w * t.o_stride, tmem + w * KT + 32 * half + 8 * k, v_lo + half * page + 2 * k, idesc_pv, n >= STEP || half + k > 0 ? 1u : 0u);
+                    for (uint32_t k = 0; k < 4; k++) umma_bf16_ts_lo(leader, d_at, p_at + 32 * half + 8 * k, b_at + half * page + 2 * k, idesc_pv, n >= STEP || half + k > 0 ? 1u : 0u);
                 }
-                if (!ok) break;
-                umma_commit((j + STEP < t1[q] ? bar_o : bar_f) + 8 * w);        // the last one has a barrier of its own
-                if (q == NQ - 1 || j >= t1[NQ - 1]) umma_commit(bar_ve + 8 * sv);
-                if (j + STEP < t1[q]) ok = qk(w, j + STEP, rk);
+                if (!ok) continue;
+                umma_commit_by(leader, (j + STEP < u1[q] ? bar_o : bar_f) + 8 * w);        // the last one has a barrier of its own
+                if (q == NQ - 1 || j >= u1[NQ - 1]) umma_commit_by(leader, bar_ve + 8 * rv.st);
+                if (j + STEP < u1[q]) ok = qk(w, j + STEP, rk);
             }
-        }
         }
     } else {
         // ---- one row per thread

@@ -90,20 +90,19 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_w4_tc_kernel(const __gri
             }
         }
     } else if (warp == 13) {
-        if (lane == 0) {
-            const uint32_t idesc = umma_idesc_bf16(128, NT), a_lo = umma_desc_lo(base), x_lo = umma_desc_lo(base + kXAt);
-            for (int n = 0; s0 + n < s1; n++) {
-                const int st = n % kStages, buf = n & 1;
-                if (!mbar_spin(bar_de + 8 * buf, (uint32_t)(n >> 1 & 1) ^ 1u, abort_flag)) break;
-                if (!mbar_spin(bar_a + 8 * st, (uint32_t)(n / kStages & 1), abort_flag)) break;
-                tc_fence_after();
+        const uint32_t leader = elect_leader(), u_tmem = (uint32_t)uniform_max((int)tmem);
+        const uint32_t idesc = umma_idesc_bf16(128, NT), a_lo = umma_desc_lo(base), x_lo = umma_desc_lo(base + kXAt);
+        for (int n = 0; s0 + n < s1; n++) {
+            const int st = n % kStages, buf = n & 1;
+            if (!wait_warp(bar_de + 8 * buf, (uint32_t)(n >> 1 & 1) ^ 1u)) break;
+            if (!wait_warp(bar_a + 8 * st, (uint32_t)(n / kStages & 1))) break;
+            tc_fence_after();
 #pragma unroll
-                for (int k = 0; k < 8; k++)
-                    umma_bf16_lo(tmem + (buf * U + k / (8 / U)) * NT, a_lo + st * 2048 + (k >> 2) * 1024 + 2 * (k & 3), x_lo + st * (NT * 16) + (k >> 2) * (NT * 8) + 2 * (k & 3),
-                                 idesc, k % (8 / U) > 0);
-                umma_commit(bar_d + 8 * buf);
-                umma_commit(bar_e + 8 * st);
-            }
+            for (int k = 0; k < 8; k++)
+                umma_bf16_lo(leader, u_tmem + (buf * U + k / (8 / U)) * NT, a_lo + st * 2048 + (k >> 2) * 1024 + 2 * (k & 3), x_lo + st * (NT * 16) + (k >> 2) * (NT * 8) + 2 * (k & 3),
+                             idesc, k % (8 / U) > 0);
+            umma_commit_by(leader, bar_d + 8 * buf);
+            umma_commit_by(leader, bar_e + 8 * st);
         }
     } else if (warp >= 4) {
         // lane: bits 0 - 2 and 4 the row, bit 3 the half of the step, so that eight lanes in a row meet eight different 16-byte columns

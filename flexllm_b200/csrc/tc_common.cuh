@@ -174,28 +174,40 @@ __device__ __forceinline__ void umma_bf16(uint32_t tmem_d, uint64_t adesc, uint6
         ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(0u)
         : "memory");
 }
-// The same with the descriptors' lower words, all that differs between tiles (the upper one: 8-row groups 1024 bytes apart, 128-byte swizzle): a step of
-// K, 32 bytes, is 2. Built from 64-bit descriptors the issue of eight MMAs took one thread 900 clocks, longer than most of them run.
+// The same for a whole warp, of which `leader` (elect_leader) issues: as long as the warp stays together and its loop bounds are the same for all lanes
+// by construction (uniform_max), addresses and descriptors live in uniform registers, where the instruction wants them. Issued from a branch
+// of one lane, every operand is moved there first. Descriptors: their lower words, all that differs between tiles (the upper one: 8-row groups
+// 1024 bytes apart, 128-byte swizzle); a step of K, 32 bytes, is 2.
+__device__ __forceinline__ uint32_t elect_leader() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ int uniform_max(int v) { return __reduce_max_sync(0xffffffffu, v); }
 __device__ __forceinline__ uint32_t umma_desc_lo(uint32_t smem_addr) { return ((smem_addr & 0x3FFFFu) >> 4) | (1u << 16); }
 constexpr uint32_t kUmmaDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
-__device__ __forceinline__ void umma_bf16_lo(uint32_t tmem_d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void umma_bf16_lo(uint32_t leader, uint32_t tmem_d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 da, db;\n\t"
         "mov.b64 da, {%1, %6};\n\tmov.b64 db, {%2, %6};\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, {%5, %5, %5, %5}, p;\n\t}"
-        ::"r"(tmem_d), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(0u), "n"(kUmmaDescHi)
+        "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %7, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, {%5, %5, %5, %5}, p;\n\t}"
+        ::"r"(tmem_d), "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(0u), "n"(kUmmaDescHi), "r"(leader)
         : "memory");
 }
 // D[tmem] (+)= A[tmem] * B[smem]^T, A's pairs of elements in 8 columns
-__device__ __forceinline__ void umma_bf16_ts_lo(uint32_t tmem_d, uint32_t tmem_a, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void umma_bf16_ts_lo(uint32_t leader, uint32_t tmem_d, uint32_t tmem_a, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
+        "{\n\t.reg .pred p, q;\n\t.reg .b64 db;\n\t"
         "mov.b64 db, {%2, %6};\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, {%5, %5, %5, %5}, p;\n\t}"
-        ::"r"(tmem_d), "r"(tmem_a), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(0u), "n"(kUmmaDescHi)
+        "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %7, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, {%5, %5, %5, %5}, p;\n\t}"
+        ::"r"(tmem_d), "r"(tmem_a), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(0u), "n"(kUmmaDescHi), "r"(leader)
         : "memory");
+}
+__device__ __forceinline__ void umma_commit_by(uint32_t leader, uint32_t bar) {
+    asm volatile("{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+                 "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(leader) : "memory");
 }
 // Arrive on `bar` once every MMA issued so far by this thread has finished.
 __device__ __forceinline__ void umma_commit(uint32_t bar) {
