@@ -1,8 +1,10 @@
 // Attention of packed rows over their sequences' pages on the CUDA cores, for the 32-bit mode. A CTA of 256 threads takes RT rows
 // (TQ tokens x the query heads of one key/value head) and walks the sequence's pages, one page of 64 keys per step: S = Q K^T and
 // O += P V are both dot products of rows in shared memory (Q and K along the head, P and V^T along the keys), RT/16 x 4 and RT/16 x dv/16
-// of them per thread, two partial sums each (even and odd elements) in packed fp32 pairs. K of the next page comes in under P V, V of
-// this page under Q K^T. Few tiles: a cluster of CTAs cuts the keys, and its partial maxima, sums and outputs meet in shared memory.
+// of them per thread, two partial sums each (even and odd elements) in packed fp32 pairs. A row's 16 threads are half a warp, so that its weights
+// change hands without a barrier; the next page comes in under this one's products where shared memory holds two (heads up to 128).
+// Few tiles: a cluster of CTAs cuts the keys, and its partial maxima, sums and outputs meet in shared memory.
+// Bound by the fp32 units, at half their rate: FIGURES
 #include "attention_paged.cuh"
 #include "tc_common.cuh"
 
@@ -14,9 +16,12 @@ namespace {
 
 constexpr int PPITCH = kPage + 4;         // pitch of P and V^T rows: 16-byte reads of eight consecutive rows meet no bank twice
 
-struct SimtArgs { PagedAttn a; int RC, HC, TQ; };      // heads per tile, head chunks per group, tokens per tile
+template <int N> struct Const { static constexpr int value = N; };
+struct SimtArgs { PagedAttn a; int RC, HC, TQ, bufs; };      // heads per tile, head chunks per group, tokens per tile, pages in shared memory
 
-__host__ __device__ inline size_t simt_floats(int RT, int dk, int dv16) { return (size_t)(RT + kPage) * (dk + 4) + (size_t)(dv16 + RT) * PPITCH; }
+__host__ __device__ inline size_t simt_floats(int RT, int dk, int dv16, int bufs) {
+    return (size_t)(RT + bufs * kPage) * (dk + 4) + (size_t)(bufs * dv16 + RT) * PPITCH;
+}
 
 __device__ __forceinline__ void copy16(float* dst, const float* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
@@ -25,10 +30,10 @@ __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_
 template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 template <int RT, int NV>
-__global__ void __launch_bounds__(256) attn_paged_simt_kernel(const __grid_constant__ SimtArgs sa, int n_split) {
+__global__ void __launch_bounds__(256, RT * NV <= 256 ? 2 : 1) attn_paged_simt_kernel(const __grid_constant__ SimtArgs sa, int n_split) {
     constexpr int RR = RT / 16;           // rows per thread
     extern __shared__ __align__(16) float sm[];
-    __shared__ float m_sm[RT], l_sm[RT];
+    __shared__ float m_sm[RT], l_sm[RT], w_sm[RT + 8];
     __shared__ Unit unit_sm;
     __shared__ unsigned redo_sm[2];
     const PagedAttn& a = sa.a;
@@ -48,7 +53,8 @@ __global__ void __launch_bounds__(256) attn_paged_simt_kernel(const __grid_const
     const SeqRows s = unit_sm.s;
     const int i0 = unit_sm.i * sa.TQ;     // first row of the tile within the sequence
     const int DP = a.dk + 4;
-    float *q_sm = sm, *k_sm = q_sm + RT * DP, *v_sm = k_sm + kPage * DP, *p_sm = v_sm + NV * 16 * PPITCH;
+    float *q_sm = sm, *p_sm = q_sm + RT * DP, *kv_sm = p_sm + RT * PPITCH;      // a page: K [64][DP], V^T [16 NV][PPITCH]
+    const int kv_floats = kPage * DP + NV * 16 * PPITCH, warp = tid >> 5, lane = tid & 31;
     const int end = a.mask ? s.ctx + s.n : min(s.ctx + i0 + sa.TQ, s.ctx + s.n);
     const int n_pg = (end + kPage - 1) / kPage;
     const int t_beg = (int)((long)n_pg * split / n_split), t_end = (int)((long)n_pg * (split + 1) / n_split);
@@ -64,26 +70,25 @@ __global__ void __launch_bounds__(256) attn_paged_simt_kernel(const __grid_const
         sure[r] = live[r] ? sure_keys(a, s, i) : 0;
         bits[r] = live[r] ? mask_bits(a, s, i) : 0ull;
     }
-    for (int e = tid; e < RT * (a.dk / 4); e += 256) {
-        const int row = e / (a.dk / 4), c = (e - row * (a.dk / 4)) * 4, i = i0 + row / sa.RC;
+    for (int row = warp; row < RT; row += 8) {
+        const int i = i0 + row / sa.RC;
         const bool on = row < sa.TQ * sa.RC && i < s.n && row % sa.RC < heads;
-        if (on) copy16(q_sm + row * DP + c, (const float*)a.q + (long)(s.row0 + i) * a.ldq + (long)(h0 + row % sa.RC) * a.dk + c);
-        else store4(q_sm + row * DP + c, make_float4(0.0f, 0.0f, 0.0f, 0.0f));
+        for (int c = lane * 4; c < a.dk; c += 128)
+            if (on) copy16(q_sm + row * DP + c, (const float*)a.q + (long)(s.row0 + i) * a.ldq + (long)(h0 + row % sa.RC) * a.dk + c);
+            else store4(q_sm + row * DP + c, make_float4(0.0f, 0.0f, 0.0f, 0.0f));
     }
-    auto load_k = [&](int t) {
-        const float* kp = (const float*)a.k + ((long)page_of(a.seq, b, t) * a.G + g) * kPage * a.dk;
-        for (int e = tid; e < kPage * (a.dk / 4); e += 256) {
-            const int key = e / (a.dk / 4), c = (e - key * (a.dk / 4)) * 4;
-            copy16(k_sm + key * DP + c, kp + (long)key * a.dk + c);
-        }
-        copies_commit();
-    };
-    // keys from `end` on were never written: zeros in their place, so that a weight of zero stays without effect
-    auto load_v = [&](int t) {
-        const float* vp = (const float*)a.v + ((long)page_of(a.seq, b, t) * a.G + g) * a.dv * kPage;
-        const int left = end - t * kPage;
-        for (int e = tid; e < a.dv * (kPage / 4); e += 256) {
-            const int d = e / (kPage / 4), c = (e % (kPage / 4)) * 4;
+    // page ids are asked for a page ahead: the copies of a page would wait for its id
+    int next_page = t_beg < t_end ? page_of(a.seq, b, t_beg) : 0;
+    auto load_page = [&](int t) {
+        float *k_sm = kv_sm + (sa.bufs == 2 ? (t - t_beg) & 1 : 0) * kv_floats, *v_sm = k_sm + kPage * DP;
+        const long at = ((long)next_page * a.G + g) * kPage;
+        const float *kp = (const float*)a.k + at * a.dk, *vp = (const float*)a.v + at * a.dv;
+        if (t + 1 < t_end) next_page = page_of(a.seq, b, t + 1);
+        for (int key = warp; key < kPage; key += 8)
+            for (int c = lane * 4; c < a.dk; c += 128) copy16(k_sm + key * DP + c, kp + (long)key * a.dk + c);
+        // keys from `end` on were never written: zeros for their values, so that a weight of zero stays without effect
+        const int left = end - t * kPage, c = (tid & 15) * 4;
+        for (int d = tid >> 4; d < a.dv; d += 16) {
             const float* src = vp + (long)d * kPage + c;
             float* dst = v_sm + d * PPITCH + c;
             if (c + 4 <= left) copy16(dst, src);
@@ -91,6 +96,13 @@ __global__ void __launch_bounds__(256) attn_paged_simt_kernel(const __grid_const
                 for (int x = 0; x < 4; x++) dst[x] = c + x < left ? src[x] : 0.0f;
         }
         copies_commit();
+    };
+    // products of the groups of 16 rows that have any: a sequence's last tile is seldom full
+    const int groups = (min(sa.TQ, s.n - i0) * sa.RC + 15) / 16;
+    auto by_rows = [&](auto f) {
+        if (RR == 1 || groups == 1) f(Const<1>());
+        else if (RR == 2 || groups == 2) f(Const<2>());
+        else f(Const<RR>());
     };
     f32x2 acc[RR][NV];
     float m[RR], l[RR];
@@ -100,30 +112,35 @@ __global__ void __launch_bounds__(256) attn_paged_simt_kernel(const __grid_const
 #pragma unroll
         for (int j = 0; j < NV; j++) acc[r][j] = pack2(0.0f, 0.0f);
     }
-    if (t_beg < t_end) { load_k(t_beg); load_v(t_beg); }
+    if (t_beg < t_end) load_page(t_beg);
     for (int t = t_beg; t < t_end; t++) {
-        copies_wait<1>();
-        __syncthreads();
+        const float *k_sm = kv_sm + (sa.bufs == 2 ? (t - t_beg) & 1 : 0) * kv_floats, *v_sm = k_sm + kPage * DP;
+        copies_wait<0>();
+        __syncthreads();                                  // the page is there, the one before has been read
+        if (sa.bufs == 2 && t + 1 < t_end) load_page(t + 1);
         f32x2 sc[RR][4];
 #pragma unroll
         for (int r = 0; r < RR; r++)
 #pragma unroll
             for (int j = 0; j < 4; j++) sc[r][j] = pack2(0.0f, 0.0f);
-#pragma unroll 2
-        for (int c = 0; c < a.dk; c += 4) {
-            float4 qv[RR], kv[4];
+        by_rows([&](auto rows) {
+            constexpr int L = decltype(rows)::value;
+#pragma unroll 4
+            for (int c = 0; c < a.dk; c += 4) {
+                float4 qv[L], kv[4];
 #pragma unroll
-            for (int r = 0; r < RR; r++) qv[r] = load4(q_sm + (ty + 16 * r) * DP + c);
+                for (int r = 0; r < L; r++) qv[r] = load4(q_sm + (ty + 16 * r) * DP + c);
 #pragma unroll
-            for (int j = 0; j < 4; j++) kv[j] = load4(k_sm + (tx + 16 * j) * DP + c);
+                for (int j = 0; j < 4; j++) kv[j] = load4(k_sm + (tx + 16 * j) * DP + c);
 #pragma unroll
-            for (int r = 0; r < RR; r++)
+                for (int r = 0; r < L; r++)
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    sc[r][j] = fma2(pack2(qv[r].x, qv[r].y), pack2(kv[j].x, kv[j].y), sc[r][j]);
-                    sc[r][j] = fma2(pack2(qv[r].z, qv[r].w), pack2(kv[j].z, kv[j].w), sc[r][j]);
-                }
-        }
+                    for (int j = 0; j < 4; j++) {
+                        sc[r][j] = fma2(pack2(qv[r].x, qv[r].y), pack2(kv[j].x, kv[j].y), sc[r][j]);
+                        sc[r][j] = fma2(pack2(qv[r].z, qv[r].w), pack2(kv[j].z, kv[j].w), sc[r][j]);
+                    }
+            }
+        });
 #pragma unroll
         for (int r = 0; r < RR; r++) {
             float x[4], mx = -INFINITY;
@@ -151,26 +168,30 @@ __global__ void __launch_bounds__(256) attn_paged_simt_kernel(const __grid_const
 #pragma unroll
             for (int j = 0; j < NV; j++) acc[r][j] = mul2(acc[r][j], al2);
         }
-        __syncthreads();                                  // P is there, K has been read
-        if (t + 1 < t_end) { load_k(t + 1); copies_wait<1>(); } else copies_wait<0>();
-        __syncthreads();                                  // V is there
-#pragma unroll 2
-        for (int c = 0; c < kPage; c += 4) {
-            float4 pv[RR];
+        __syncwarp();                                     // a row's weights are read by the half warp that wrote them
+        by_rows([&](auto rows) {
+            constexpr int L = decltype(rows)::value;
+#pragma unroll 4
+            for (int c = 0; c < kPage; c += 4) {
+                float4 pv[L];
 #pragma unroll
-            for (int r = 0; r < RR; r++) pv[r] = load4(p_sm + (ty + 16 * r) * PPITCH + c);
+                for (int r = 0; r < L; r++) pv[r] = load4(p_sm + (ty + 16 * r) * PPITCH + c);
 #pragma unroll
-            for (int j = 0; j < NV; j++) {
-                const float4 vv = load4(v_sm + (tx + 16 * j) * PPITCH + c);
+                for (int j = 0; j < NV; j++) {
+                    const float4 vv = load4(v_sm + (tx + 16 * j) * PPITCH + c);
 #pragma unroll
-                for (int r = 0; r < RR; r++) {
-                    acc[r][j] = fma2(pack2(pv[r].x, pv[r].y), pack2(vv.x, vv.y), acc[r][j]);
-                    acc[r][j] = fma2(pack2(pv[r].z, pv[r].w), pack2(vv.z, vv.w), acc[r][j]);
+                    for (int r = 0; r < L; r++) {
+                        acc[r][j] = fma2(pack2(pv[r].x, pv[r].y), pack2(vv.x, vv.y), acc[r][j]);
+                        acc[r][j] = fma2(pack2(pv[r].z, pv[r].w), pack2(vv.z, vv.w), acc[r][j]);
+                    }
                 }
             }
+        });
+        __syncwarp();
+        if (sa.bufs == 1 && t + 1 < t_end) {
+            __syncthreads();
+            load_page(t + 1);
         }
-        __syncthreads();                                  // V and P have been read
-        if (t + 1 < t_end) load_v(t + 1);
     }
     copies_wait<0>();
     __syncthreads();
@@ -189,24 +210,48 @@ __global__ void __launch_bounds__(256) attn_paged_simt_kernel(const __grid_const
         }
     }
     if (n_split > 1) cluster_sync(); else __syncthreads();
-    const int rows = min(sa.TQ, s.n - i0) * sa.RC;
-    for (int e = tid; e < rows * a.dv; e += 256) {
-        const int row = e / a.dv, d = e - row * a.dv;
-        if (row % n_split != split || row % sa.RC >= heads) continue;
-        float mx = -INFINITY, sum = 0.0f, v = 0.0f;
-        if (n_split == 1) {
-            sum = l_sm[row]; v = o_sm[e];
-        } else {
-            for (int k = 0; k < n_split; k++) mx = fmaxf(mx, ld_cluster_f32(cluster_addr(smem_u32(m_sm + row), k)));
-            for (int k = 0; k < n_split; k++) {
-                const float mk = ld_cluster_f32(cluster_addr(smem_u32(m_sm + row), k)), w = mk == -INFINITY ? 0.0f : expf(mk - mx);
-                sum = __fmaf_rn(ld_cluster_f32(cluster_addr(smem_u32(l_sm + row), k)), w, sum);
-                v = __fmaf_rn(ld_cluster_f32(cluster_addr(smem_u32(o_sm + e), k)), w, v);
+    // CTA r of the cluster has rows r, r + n_split, ..: the parts' weights over the sums, then the outputs
+    const int rows = min(sa.TQ, s.n - i0) * sa.RC, mine = (rows - split + n_split - 1) / n_split;
+    for (int e = tid; e < mine; e += 256) {
+        const int row = split + e * n_split;
+        float mk[8], lk[8], mx = -INFINITY, sum = 0.0f;
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            if (k < n_split) {
+                mk[k] = ld_cluster_f32(cluster_addr(smem_u32(m_sm + row), k));
+                lk[k] = ld_cluster_f32(cluster_addr(smem_u32(l_sm + row), k));
             }
-        }
-        v = sum == 0.0f ? 0.0f : v / sum;
-        if (not_finite(v)) atomicOr(&redo_sm[row >> 5], 1u << (row & 31));
-        ((float*)a.out)[(long)(s.row0 + i0 + row / sa.RC) * a.ldo + (long)(h0 + row % sa.RC) * a.dv + d] = v;
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            if (k < n_split) mx = fmaxf(mx, mk[k]);
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            if (k < n_split) {
+                mk[k] = mk[k] == -INFINITY ? 0.0f : expf(mk[k] - mx);
+                sum = __fmaf_rn(lk[k], mk[k], sum);
+            }
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            if (k < n_split) w_sm[k * mine + e] = sum == 0.0f ? 0.0f : mk[k] / sum;
+    }
+    __syncthreads();
+    for (int e = tid; e < mine * (a.dv / 4); e += 256) {
+        const int at = e / (a.dv / 4), row = split + at * n_split, d = (e - at * (a.dv / 4)) * 4;
+        if (row % sa.RC >= heads) continue;
+        float4 x[8], v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            if (k < n_split) x[k] = ld_cluster_f32x4(cluster_addr(smem_u32(o_sm + row * a.dv + d), k));
+#pragma unroll
+        for (int k = 0; k < 8; k++)
+            if (k < n_split) {
+                const float w = w_sm[k * mine + at];
+                v = make_float4(__fmaf_rn(x[k].x, w, v.x), __fmaf_rn(x[k].y, w, v.y), __fmaf_rn(x[k].z, w, v.z), __fmaf_rn(x[k].w, w, v.w));
+            }
+        if (not_finite(v.x) || not_finite(v.y) || not_finite(v.z) || not_finite(v.w)) atomicOr(&redo_sm[row >> 5], 1u << (row & 31));
+        float* out = (float*)a.out + (long)(s.row0 + i0 + row / sa.RC) * a.ldo + (long)(h0 + row % sa.RC) * a.dv + d;
+        if ((a.ldo & 3) == 0 && aligned16(a.out)) store4(out, v);
+        else { out[0] = v.x; out[1] = v.y; out[2] = v.z; out[3] = v.w; }
     }
     if (n_split > 1) cluster_sync(); else __syncthreads();
     if (redo_sm[0] | redo_sm[1])
@@ -214,8 +259,9 @@ __global__ void __launch_bounds__(256) attn_paged_simt_kernel(const __grid_const
             if (redo_sm[row >> 5] >> (row & 31) & 1) attn_row_by_key<float>(a, b, s, i0 + row / sa.RC, h0 + row % sa.RC);
 }
 
-template <int RT, int NV> int launch_simt(const SimtArgs& sa, int tiles, int splits, cudaStream_t st) {
-    const size_t smem = simt_floats(RT, sa.a.dk, NV * 16) * 4;
+template <int RT, int NV> int launch_simt(SimtArgs& sa, int tiles, int splits, cudaStream_t st) {
+    sa.bufs = simt_floats(RT, sa.a.dk, NV * 16, 2) * 4 <= 220 * 1024 ? 2 : 1;
+    const size_t smem = simt_floats(RT, sa.a.dk, NV * 16, sa.bufs) * 4;
     auto kern = attn_paged_simt_kernel<RT, NV>;
     TRY_RC(allow_shared(kern, smem));
     launch_cluster(kern, dim3(tiles * splits, sa.a.G * sa.HC), dim3(256), splits, smem, st, sa, splits);
@@ -226,8 +272,9 @@ template <int RT> int run_simt(const PagedAttn& a, cudaStream_t st) {
     const int R = a.H / a.G;
     sa.a = a;
     sa.RC = R < RT ? R : RT; sa.HC = (R + sa.RC - 1) / sa.RC; sa.TQ = RT / sa.RC;
-    const long tiles = a.seq.T / sa.TQ + (a.seq.B < a.seq.T ? a.seq.B : a.seq.T);
-    const int splits = key_splits(tiles * a.G * sa.HC, gemm_sm_count(), (a.seq.max_ctx + kPage) / kPage, 1);
+    const long seqs = a.seq.B < a.seq.T ? a.seq.B : a.seq.T;
+    const long tiles = a.seq.T / sa.TQ + seqs, real = ((a.seq.T + seqs - 1) / seqs + sa.TQ - 1) / sa.TQ * seqs;      // at most; with sequences of equal length
+    const int splits = key_splits(real * a.G * sa.HC, 2 * gemm_sm_count(), (a.seq.max_ctx + kPage) / kPage, 1);
     if (tiles * splits > 0x7fffffffL || a.G * sa.HC > 65535) return FLEXLLM_ENOTSUP;
     if (a.dv <= 64) return launch_simt<RT, 4>(sa, (int)tiles, splits, st);
     if (a.dv <= 128) return launch_simt<RT, 8>(sa, (int)tiles, splits, st);

@@ -53,12 +53,6 @@ __host__ __device__ inline TcSmem tc_smem(int NQ, int kc, int vr, int ks, int vs
 constexpr int kMaxStages = 4;
 constexpr uint32_t kHalfSm = 108 * 1024, kWholeSm = 224 * 1024;       // dynamic shared memory; a few KB are static
 
-__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
-    return v;
-}
-
 template <int MODE>
 __global__ void __launch_bounds__(MODE == kOne ? 192 : 320, MODE == kOne ? 2 : 1) attn_paged_tc_kernel(const __grid_constant__ CUtensorMap tmapQ, const __grid_constant__ CUtensorMap tmapK,
                                                                          const __grid_constant__ CUtensorMap tmapV, const __grid_constant__ TcArgs t) {

@@ -206,9 +206,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_w4_tc_kernel(const __gri
         if (t.n_split == 1) v = *reinterpret_cast<const float4*>(red + m * 132 + r);
         else
             for (int p = 0; p < t.n_split; p++) {
-                const uint32_t at = cluster_addr(base + (uint32_t)(m * 132 + r) * 4u, p);
-                float4 x;
-                asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(at) : "memory");
+                const float4 x = ld_cluster_f32x4(cluster_addr(base + (uint32_t)(m * 132 + r) * 4u, p));
                 v.x += x.x; v.y += x.y; v.z += x.z; v.w += x.w;
             }
         const long at = (long)(m0 + m) * c.ldy + n0 + r;
