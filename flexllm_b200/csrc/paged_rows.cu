@@ -11,7 +11,8 @@ namespace {
 // the tables hold at [pos[axis of p]][p]; elements from rot on stay. All in fp32, rounded once.
 // HBM bound: every row is read and written once, the tables' rows come from L2. A group of L lanes holds a head: lane c the pairs
 // 4 c .. 4 c + 3 (two vectors of four elements, so that both halves of a pair meet in one thread), the lanes behind them eight of the unrotated
-// elements each. A warp stays with one token, so that its table entries are read once for the heads that it takes.
+// elements each. A warp stays with one token, whose sequence, positions and table entries it looks up once for eight heads. In bf16 the
+// instructions count as much as the bytes: pairs of fp32 throughout.
 struct RopeArgs {
     PackedSeqs seq;
     int H, G, dk, dv, rot;
@@ -22,65 +23,109 @@ struct RopeArgs {
     const float *cos_t, *sin_t; int table_len;
     void *k, *v;
     void* q; long ldq;
-    int chunks, qk_ctas, v_units;
+    int chunks, qk_ctas;                           // warps of a token, CTAs of such warps
+    bool fours;                                    // the pairs of a lane are of one axis, the tables' rows 16-byte aligned
 };
-constexpr int kRopeHeads = 8;             // heads of one warp
+constexpr int kRopeHeads = 8;                      // heads of a warp
 
-template <class T, int L> __device__ __forceinline__ void rope_warp(const RopeArgs& a, long w) {
+// four elements as two pairs
+struct Four { f32x2 a, b; };
+__device__ __forceinline__ Four load_four(const float* p) { const float4 v = load4(p); return {pack2(v.x, v.y), pack2(v.z, v.w)}; }
+// four elements as they are in memory
+template <class T> struct Raw;
+template <> struct Raw<bf16> {
+    static constexpr int kRounds = 4;              // of heads under way together
+    uint2 v;
+    __device__ __forceinline__ void load(const bf16* p) { v = *reinterpret_cast<const uint2*>(p); }
+    __device__ __forceinline__ Four four() const { return {pack2(bf_lo(v.x), bf_hi(v.x)), pack2(bf_lo(v.y), bf_hi(v.y))}; }
+};
+template <> struct Raw<float> {
+    static constexpr int kRounds = 2;
+    float4 v;
+    __device__ __forceinline__ void load(const float* p) { v = load4(p); }
+    __device__ __forceinline__ Four four() const { return {pack2(v.x, v.y), pack2(v.z, v.w)}; }
+};
+template <class T> __device__ __forceinline__ void store_four(T* p, const Four& v) {
+    float4 f;
+    unpack2(v.a, f.x, f.y); unpack2(v.b, f.z, f.w);
+    store4(p, f);
+}
+__device__ __forceinline__ Four times(const Four& x, const Four& y) { return {mul2(x.a, y.a), mul2(x.b, y.b)}; }
+__device__ __forceinline__ Four times_plus(const Four& x, const Four& y, const Four& z) { return {fma2(x.a, y.a, z.a), fma2(x.b, y.b, z.b)}; }
+__device__ __forceinline__ Four all_four(float v) { return {pack2(v, v), pack2(v, v)}; }
+
+template <class T, int L> __device__ __forceinline__ void rope_warp(const RopeArgs& a, unsigned w) {
+    constexpr int kRounds = Raw<T>::kRounds * (32 / L) <= kRopeHeads ? Raw<T>::kRounds : kRopeHeads * L / 32;
     const int lane = threadIdx.x & 31, c = lane % L, sub = lane / L;
-    const int t = (int)(w / a.chunks), h0 = (int)(w % a.chunks) * kRopeHeads;
+    const int t = w / (unsigned)a.chunks, h0 = (w - t * a.chunks) * kRopeHeads, h1 = min(h0 + kRopeHeads, a.H + a.G);
     if (t >= a.seq.T) return;
-    // the sequence of the row: the last one that starts at or before it and has rows
-    int lo = 0, hi = a.seq.B - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (a.seq.cu[mid] <= t) lo = mid; else hi = mid - 1;
-    }
-    const SeqRows s = seq_rows(a.seq, lo);
-    if (t < s.row0 || t >= s.row0 + s.n) return;
-    const int at = s.ctx + t - s.row0;
     const int half = a.rot >> 1, nrot = half >> 2;
-    const bool turns = c < nrot, rest = !turns && a.rot + (c - nrot) * 8 < a.dk;
+    const bool turns = c < nrot, rest = !turns && a.rot + (c - nrot) * 8 < a.dk, mine = turns || rest;
     const int e0 = turns ? 4 * c : a.rot + (c - nrot) * 8, e1 = turns ? e0 + half : e0 + 4;
-    float co[4], si[4];
-    if (turns) {
+    const T* src = (const T*)a.proj + (long)t * a.ldp;
+    // a round: 32 / L heads
+    Raw<T> x[kRounds], y[kRounds];
+    auto load = [&](int h) {
 #pragma unroll
-        for (int p = 0; p < 4; p++) {
+        for (int j = 0; j < kRounds; j++) {
+            const int hj = h + j * (32 / L) + sub;
+            if (hj < h1 && mine) { x[j].load(src + hj * a.dk + e0); y[j].load(src + hj * a.dk + e1); }
+        }
+    };
+    load(h0);
+    // the sequence of the row: the last one that starts at or before it
+    int b = -1;
+    for (int b0 = 0; b0 < a.seq.B; b0 += 32) b += __popc(__ballot_sync(0xffffffffu, b0 + lane < a.seq.B && a.seq.cu[b0 + lane] <= t));
+    Four co = all_four(1.0f), si = all_four(0.0f);         // the other elements do not turn
+    if (turns) {
+        auto row_of = [&](int pair) {
             int axis = 0;
-            while (axis < a.axes - 1 && e0 + p >= a.sec_end[axis]) axis++;
+            while (axis < a.axes - 1 && pair >= a.sec_end[axis]) axis++;
             int row = a.pos[(long)axis * a.seq.T + t];
             if ((unsigned)row >= (unsigned)a.table_len) { data_error(a.seq.error_flag); row = row < 0 ? 0 : a.table_len - 1; }
-            co[p] = a.cos_t[(long)row * half + e0 + p]; si[p] = a.sin_t[(long)row * half + e0 + p];
+            return (long)row * half + pair;
+        };
+        if (a.fours) {
+            const long at = row_of(e0);
+            co = load_four(a.cos_t + at); si = load_four(a.sin_t + at);
+        } else {
+            float f[8];
+#pragma unroll
+            for (int p = 0; p < 4; p++) { const long at = row_of(e0 + p); f[p] = a.cos_t[at]; f[4 + p] = a.sin_t[at]; }
+            co = {pack2(f[0], f[1]), pack2(f[2], f[3])}; si = {pack2(f[4], f[5]), pack2(f[6], f[7])};
         }
     }
-    const T* src = (const T*)a.proj + (long)t * a.ldp;
-    const long page = page_of(a.seq, lo, at / kPage);
+    const Four minus_si = times(si, all_four(-1.0f));
+    if (b < 0) return;
+    const SeqRows s = seq_rows(a.seq, b);
+    if (t < s.row0 || t >= s.row0 + s.n) return;
+    const int at = s.ctx + t - s.row0;
+    const long page = h1 > a.H ? page_of(a.seq, b, at / kPage) : 0;
+    const float inv_dk = 1.0f / (float)a.dk;
+    for (int h = h0; h < h1; h += kRounds * (32 / L)) {
+        if (h > h0) load(h);
 #pragma unroll
-    for (int j = 0; j < kRopeHeads * L / 32; j++) {
-        const int h = h0 + j * (32 / L) + sub;
-        const bool on = h < a.H + a.G && (turns || rest);
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f), y = x;
-        if (on) { x = load4(src + (long)h * a.dk + e0); y = load4(src + (long)h * a.dk + e1); }
-        const float* gain = h < a.H ? a.q_gain : a.k_gain;
-        float ss = x.x * x.x + x.y * x.y + x.z * x.z + x.w * x.w + y.x * y.x + y.y * y.y + y.z * y.z + y.w * y.w;
+        for (int j = 0; j < kRounds; j++) {
+            const int hj = h + j * (32 / L) + sub;
+            const float* gain = hj < a.H ? a.q_gain : a.k_gain;
+            Four u = all_four(0.0f), v = u;
+            if (hj < h1 && mine) { u = x[j].four(); v = y[j].four(); }
+            float s0, s1;
+            unpack2(fma2(u.a, u.a, fma2(u.b, u.b, fma2(v.a, v.a, mul2(v.b, v.b)))), s0, s1);
+            float ss = s0 + s1;
 #pragma unroll
-        for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        if (!on) continue;
-        if (gain) {
-            const float r = 1.0f / sqrtf(ss / (float)a.dk + a.eps);
-            const float4 gx = load4(gain + e0), gy = load4(gain + e1);
-            x = make_float4(x.x * r * gx.x, x.y * r * gx.y, x.z * r * gx.z, x.w * r * gx.w);
-            y = make_float4(y.x * r * gy.x, y.y * r * gy.y, y.z * r * gy.z, y.w * r * gy.w);
+            for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            if (hj >= h1 || !mine) continue;
+            if (gain) {
+                const Four r = all_four(rsqrtf(__fmaf_rn(ss, inv_dk, a.eps)));
+                u = times(times(u, r), load_four(gain + e0));
+                v = times(times(v, r), load_four(gain + e1));
+            }
+            T* dst = hj < a.H ? (T*)a.q + (long)t * a.ldq + (long)hj * a.dk
+                              : (T*)a.k + ((page * a.G + (hj - a.H)) * kPage + (at & (kPage - 1))) * a.dk;
+            store_four(dst + e0, times_plus(v, minus_si, times(u, co)));
+            store_four(dst + e1, times_plus(u, si, times(v, co)));
         }
-        if (turns) {
-            const float4 u = x;
-            x = make_float4(u.x * co[0] - y.x * si[0], u.y * co[1] - y.y * si[1], u.z * co[2] - y.z * si[2], u.w * co[3] - y.w * si[3]);
-            y = make_float4(y.x * co[0] + u.x * si[0], y.y * co[1] + u.y * si[1], y.z * co[2] + u.z * si[2], y.w * co[3] + u.w * si[3]);
-        }
-        T* dst = h < a.H ? (T*)a.q + (long)t * a.ldq + (long)h * a.dk
-                         : (T*)a.k + ((page * a.G + (h - a.H)) * kPage + (at & (kPage - 1))) * a.dk;
-        store4(dst + e0, x);
-        store4(dst + e1, y);
     }
 }
 
@@ -91,12 +136,12 @@ template <> struct Slots<float> { static constexpr int N = 4; };
 
 // CTAs below qk_ctas: eight warps of the above. Then one (page of a sequence, key/value head) each: the page's new value rows through shared
 // memory into its columns, whole 16-byte pieces where the call fills them.
-template <class T, int L> __global__ void __launch_bounds__(256) qk_norm_rope_kernel(const __grid_constant__ RopeArgs a) {
+template <class T, int L> __global__ void __launch_bounds__(256, 4) qk_norm_rope_kernel(const __grid_constant__ RopeArgs a) {
     extern __shared__ __align__(16) uint8_t raw[];
     __shared__ Unit unit_sm;
     pdl_sync();
     if ((int)blockIdx.x < a.qk_ctas) {
-        rope_warp<T, L>(a, (long)blockIdx.x * 8 + (threadIdx.x >> 5));
+        rope_warp<T, L>(a, blockIdx.x * 8u + (threadIdx.x >> 5));
         return;
     }
     const int id = blockIdx.x - a.qk_ctas, g = id % a.G, tid = threadIdx.x;
@@ -144,7 +189,7 @@ template <class T, int L> int launch_rope(RopeArgs& a, cudaStream_t st) {
     const long qk = ((long)a.seq.T * a.chunks + 7) / 8;
     // a sequence's rows touch at most two pages more than they would fill
     const long units = (long)a.seq.T / kPage + 2L * (a.seq.B < a.seq.T ? a.seq.B : a.seq.T);
-    if (qk + units * a.G > 0x7fffffffL) return FLEXLLM_ENOTSUP;
+    if (qk + units * a.G > 0x7fffffffL || qk > 0x1fffffffL) return FLEXLLM_ENOTSUP;      // warps are counted in 32 bits
     a.qk_ctas = (int)qk;
     const size_t smem = (size_t)kPage * (a.dv * sizeof(T) + 4);
     auto kern = qk_norm_rope_kernel<T, L>;
@@ -258,6 +303,8 @@ extern "C" int flexllm_qk_norm_rope(int dtype, const flexllm_kv_pages* kv, int h
     FLEXLLM_REQUIRE(end == rot / 2);
     if (T == 0) return FLEXLLM_OK;
     FLEXLLM_REQUIRE(proj && q && (rot == 0 || pos) && aligned(proj, 16) && aligned(q, 16) && aligned(q_gain, 16) && aligned(k_gain, 16));
+    a.fours = aligned(cos_t, 16) && aligned(sin_t, 16);
+    for (int i = 0; i < axes; i++) a.fours = a.fours && a.sec_end[i] % 4 == 0;
     a.proj = proj; a.ldp = ldp; a.q_gain = q_gain; a.k_gain = k_gain; a.eps = eps; a.pos = pos; a.axes = axes;
     a.cos_t = cos_t; a.sin_t = sin_t; a.table_len = table_len; a.k = kv->k; a.v = kv->v; a.q = q; a.ldq = ldq;
     a.seq.error_flag = device_error_flag();
