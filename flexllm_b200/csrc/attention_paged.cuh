@@ -76,6 +76,7 @@ inline int key_splits(long tiles, long slots, int pages, int least) {
 }
 
 int attn_paged_simt(const PagedAttn& a, cudaStream_t st);      // fp32
+int attn_paged_f32(const PagedAttn& a, cudaStream_t st);       // fp32, heads up to 128
 int attn_paged_tc(const PagedAttn& a, cudaStream_t st);        // bf16, scale >= 0
 
 }  // namespace flexllm

@@ -1,0 +1,389 @@
+// Attention of packed rows over their sequences' pages in fp32, on the tensor cores (heads up to 128). A number is the sum of three bf16 parts of eight bits
+// each, which hold it to the last bit; a product is the six of nine products of parts that reach 2^-24 of it, summed in fp32. Six bf16 MMAs
+// are a quarter of what the same product takes the fp32 units.
+// A tile is 128 rows (tokens x the query heads of one key/value head), walked page by page with the running softmax of the bf16 kernel:
+//   warp 12        brings K and V^T of a page in pieces of 8 KB
+//   warps 4 .. 11  cut them into parts, in swizzled shared memory (Q at the start)
+//   warp 13        S = Q K^T and O += P V, P from TMEM
+//   warps 0 .. 3   one row per thread: maximum, weights 2^(S scale log2 e - m) in three parts, sum
+// Few tiles: a cluster of CTAs cuts the keys. FIGURES
+#include "attention_join.cuh"
+
+namespace flexllm {
+
+using namespace tc;
+
+namespace {
+
+constexpr int kPieces = 4, kF32Threads = 448;
+constexpr uint32_t kPieceBytes = 8192;
+
+struct F32Args {
+    PagedAttn a;
+    int RC, HC, TQ;                        // heads per tile, head chunks per group, tokens per tile
+    int kc, vr, o_stride, n_split;         // 128-byte blocks of a part's Q or K row, rows of a V^T part, columns of O
+    float a2;                              // scale * log2 e
+};
+struct F32Smem { uint32_t k, v, raw, bars, total; };
+__host__ __device__ inline F32Smem f32_smem(int kc, int vr) {
+    F32Smem o;
+    o.k = 3u * kc * 16384u;
+    o.v = o.k + 3u * kc * 8192u;
+    o.raw = o.v + 3u * vr * 128u;
+    o.bars = o.raw + kPieces * kPieceBytes;
+    o.total = o.bars + 256u + 1024u;
+    return o;
+}
+
+// 8 numbers as their three parts, pairs in order. The first part carries an infinity or NaN.
+__device__ __forceinline__ void cut8(float (&f)[8], uint4 (&part)[3]) {
+#pragma unroll
+    for (int p = 0; p < 3; p++) {
+        const uint32_t w[4] = {bf_pack(f[0], f[1]), bf_pack(f[2], f[3]), bf_pack(f[4], f[5]), bf_pack(f[6], f[7])};
+        part[p] = make_uint4(w[0], w[1], w[2], w[3]);
+        if (p < 2)
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                f[2 * j] = fabsf(f[2 * j]) <= 3.0e38f ? f[2 * j] - bf_lo(w[j]) : 0.0f;
+                f[2 * j + 1] = fabsf(f[2 * j + 1]) <= 3.0e38f ? f[2 * j + 1] - bf_hi(w[j]) : 0.0f;
+            }
+    }
+}
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
+__global__ void __launch_bounds__(kF32Threads, 1) attn_paged_f32_kernel(const __grid_constant__ F32Args t) {
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ Unit unit_sm;
+    __shared__ unsigned redo_sm[4];
+    const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+    uint8_t* base_ptr = smem_raw + (base - raw);
+    const PagedAttn& a = t.a;
+    const F32Smem o = f32_smem(t.kc, t.vr);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(base_ptr + o.bars);
+    const uint32_t bar_rf = smem_u32(bars), bar_re = bar_rf + 8 * kPieces, bar_q = bar_re + 8 * kPieces, bar_k = bar_q + 8, bar_ke = bar_k + 8, bar_v = bar_ke + 8,
+                   bar_ve = bar_v + 8, bar_s = bar_ve + 8, bar_p = bar_s + 8, bar_o = bar_p + 8, bar_f = bar_o + 8;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 20);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kPieces; i++) { mbar_init(bar_rf + 8 * i, 1); mbar_init(bar_re + 8 * i, 8); }
+        mbar_init(bar_q, 8); mbar_init(bar_k, 8); mbar_init(bar_ke, 1); mbar_init(bar_v, 8); mbar_init(bar_ve, 1);
+        mbar_init(bar_s, 1); mbar_init(bar_p, 4); mbar_init(bar_o, 1); mbar_init(bar_f, 1);
+        *abort_flag = 0;
+        fence_barrier_init();
+    }
+    if (threadIdx.x < 4) redo_sm[threadIdx.x] = 0;
+    if (warp == 13) { tmem_alloc(smem_u32(tmem_slot), 512); tmem_relinquish(); }
+    pdl_sync();
+    if (warp == 0) {
+        const int TQ = t.TQ;
+        const Unit u = find_unit(a.seq, (int)blockIdx.x / t.n_split, [TQ](const SeqRows& s) { return (s.n + TQ - 1) / TQ; });
+        if (lane == 0) unit_sm = u;
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot, tP = tmem + 64, tO = tmem + 192;
+    const int split = blockIdx.x % t.n_split, b = unit_sm.b;
+    const SeqRows s = unit_sm.s;
+    const int R = a.H / a.G, g = blockIdx.y / t.HC, h0 = g * R + (blockIdx.y % t.HC) * t.RC, heads = min(t.RC, (g + 1) * R - h0);
+    const int i0 = unit_sm.i * t.TQ;                      // first row of the tile within the sequence
+    const int end = b < 0 ? 0 : a.mask ? s.ctx + s.n : min(s.ctx + i0 + t.TQ, s.ctx + s.n), n_pg = (end + kPage - 1) / kPage;
+    const int t0 = (int)((long)n_pg * split / t.n_split), t1 = (int)((long)n_pg * (split + 1) / t.n_split);
+    auto wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_spin(bar, parity, abort_flag)) != 0; };
+    const int v_pieces = (a.dv + 31) / 32;
+    if (b >= 0) {
+    if (warp == 12) {
+        int ids = 0, piece = 0;
+        bool ok = true;
+        for (int j = t0; ok && j < t1; j++) {
+            const int n = j - t0;
+            if ((n & 31) == 0) ids = j + lane < t1 ? page_of(a.seq, b, j + lane) : 0;
+            const long at = ((long)__shfl_sync(0xffffffffu, ids, n & 31) * a.G + g) * kPage;
+            for (int c = 0; ok && c < 4 + v_pieces; c++, piece++) {
+                const int st = piece % kPieces;
+                ok = wait(bar_re + 8 * st, (uint32_t)(piece / kPieces & 1) ^ 1u);
+                if (!ok || lane != 0) continue;
+                const uint32_t bytes = c < 4 ? 16u * a.dk * 4u : (uint32_t)min(32, a.dv - 32 * (c - 4)) * 256u;
+                const float* src = c < 4 ? (const float*)a.k + at * a.dk + (long)c * 16 * a.dk : (const float*)a.v + at * a.dv + (long)(c - 4) * 32 * kPage;
+                mbar_expect_tx(bar_rf + 8 * st, bytes);
+                bulk_copy(base + o.raw + st * kPieceBytes, src, bytes, bar_rf + 8 * st);
+            }
+        }
+    } else if (warp == 13) {
+        const uint32_t leader = elect_leader(), u_tmem = (uint32_t)uniform_max((int)tmem);
+        const int u0 = uniform_max(t0), u1 = uniform_max(t1);
+        const uint32_t idesc_qk = umma_idesc_bf16(128, kPage), idesc_pv = umma_idesc_bf16(128, t.vr);
+        const int ksteps = (a.dk + 15) / 16;
+        const uint32_t q_lo = umma_desc_lo(base), k_lo = umma_desc_lo(base + o.k), v_lo = umma_desc_lo(base + o.v);
+        // products of parts, the small ones first
+        auto parts = [](int x, uint32_t& pa, uint32_t& pb) {
+            pa = x == 1 ? 2u : x == 2 || x == 4 ? 1u : 0u;
+            pb = x == 0 ? 2u : x == 2 || x == 3 ? 1u : 0u;
+        };
+        auto qk = [&](int n) {
+            if (!wait(bar_k, (uint32_t)(n & 1))) return false;
+            tc_fence_after();
+#pragma unroll
+            for (int x = 0; x < 6; x++) {
+                uint32_t pa, pb;
+                parts(x, pa, pb);
+                const uint32_t qa = q_lo + pa * (uint32_t)t.kc * 1024u, ka = k_lo + pb * (uint32_t)t.kc * 512u;
+                for (int k = 0; k < ksteps; k++)
+                    umma_bf16_lo(leader, u_tmem, qa + (k >> 2) * 1024u + 2 * (k & 3), ka + (k >> 2) * 512u + 2 * (k & 3), idesc_qk, x > 0 || k > 0);
+            }
+            umma_commit_by(leader, bar_s);
+            umma_commit_by(leader, bar_ke);
+            return true;
+        };
+        bool ok = u0 < u1 && wait(bar_q, 0) && qk(0);
+        for (int j = u0; ok && j < u1; j++) {
+            const int n = j - u0;
+            ok = wait(bar_v, (uint32_t)(n & 1)) && wait(bar_p, (uint32_t)(n & 1));
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll
+            for (int x = 0; x < 6; x++) {
+                uint32_t pa, pb;
+                parts(x, pa, pb);
+#pragma unroll
+                for (uint32_t k = 0; k < 4; k++)
+                    umma_bf16_ts_lo(leader, u_tmem + 192, u_tmem + 64 + 32 * pa + 8 * k, v_lo + pb * (uint32_t)t.vr * 8u + 2 * k, idesc_pv, n > 0 || x > 0 || k > 0);
+            }
+            umma_commit_by(leader, j + 1 < u1 ? bar_o : bar_f);           // the last one has a barrier of its own
+            umma_commit_by(leader, bar_ve);
+            if (j + 1 < u1) ok = qk(n + 1);
+        }
+    } else if (warp >= 4) {
+        // ---- numbers into parts: 8 of them per thread and piece
+        const int ct = threadIdx.x - 128, per = a.dk / 8;
+        uint4 part[3];
+        auto put = [&](uint32_t at, uint32_t stride, int row, int c) {         // the 16 bytes c of a row of all parts; `at` the row's block
+#pragma unroll
+            for (int p = 0; p < 3; p++) *reinterpret_cast<uint4*>(base_ptr + at + p * stride + row * 128 + (((c ^ row) & 7) << 4)) = part[p];
+        };
+        const uint32_t q_part = (uint32_t)t.kc * 16384u, k_part = (uint32_t)t.kc * 8192u, v_part = (uint32_t)t.vr * 128u;
+        if (t0 < t1) {
+            for (int e = ct; e < 128 * per; e += 256) {
+                const int row = e / per, c = e - row * per, i = i0 + row / t.RC;
+                float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                if (row < t.TQ * t.RC && i < s.n && row % t.RC < heads) load8((const float*)a.q + (long)(s.row0 + i) * a.ldq + (long)(h0 + row % t.RC) * a.dk + c * 8, f);
+                cut8(f, part);
+                put((uint32_t)(c >> 3) * 16384u, q_part, row, c);
+            }
+            if (per & 1) {                                // the last 16 elements of a product reach beyond the row: zeros in Q and K
+                part[0] = part[1] = part[2] = make_uint4(0, 0, 0, 0);
+                if (ct < 128) put((uint32_t)(per >> 3) * 16384u, q_part, ct, per);
+                if (ct < kPage) put(o.k + (uint32_t)(per >> 3) * 8192u, k_part, ct, per);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_q);
+        }
+        const int key = ct / per, col = ct - key * per;   // of a piece of K: 16 keys
+        int piece = 0;
+        bool ok = true;
+        auto next_piece = [&](auto f) {
+            const int st = piece % kPieces;
+            ok = ok && wait(bar_rf + 8 * st, (uint32_t)(piece / kPieces & 1));
+            if (ok) f((const float*)(base_ptr + o.raw + st * kPieceBytes));
+            __syncwarp();
+            if (ok && lane == 0) mbar_arrive(bar_re + 8 * st);
+            piece++;
+        };
+        for (int j = t0; ok && j < t1; j++) {
+            const int n = j - t0, left = end - j * kPage;
+            ok = wait(bar_ke, (uint32_t)(n & 1) ^ 1u);
+            for (int c = 0; ok && c < 4; c++)
+                next_piece([&](const float* src) {
+                    if (key >= 16) return;
+                    float f[8];
+                    load8(src + key * a.dk + col * 8, f);
+                    cut8(f, part);
+                    put(o.k + (uint32_t)(col >> 3) * 8192u, k_part, c * 16 + key, col);
+                });
+            if (!ok) break;
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_k);
+            ok = wait(bar_ve, (uint32_t)(n & 1) ^ 1u);
+            for (int c = 0; ok && c < v_pieces; c++)
+                next_piece([&](const float* src) {
+                    const int d = ct >> 3, k8 = (ct & 7) * 8;
+                    if (32 * c + d >= a.dv) return;
+                    float f[8];
+                    load8(src + d * kPage + k8, f);
+                    // keys behind the sequence's last one were never written: zeros, so that a weight of zero stays without effect
+                    if (k8 + 8 > left)
+#pragma unroll
+                        for (int x = 0; x < 8; x++)
+                            if (k8 + x >= left) f[x] = 0.0f;
+                    cut8(f, part);
+                    put(o.v, v_part, 32 * c + d, k8 >> 3);
+                });
+            if (!ok) break;
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_v);
+        }
+    } else {
+        // ---- one row per thread
+        const int row = threadIdx.x;
+        const uint32_t lane_addr = (uint32_t)(warp * 32) << 16;
+        const int i = i0 + row / t.RC, hr = row % t.RC;
+        const bool live = row < t.TQ * t.RC && i < s.n && hr < heads;
+        const int sure = live ? sure_keys(a, s, i) : 0x40000000;
+        const unsigned long long bits = live ? mask_bits(a, s, i) : 0ull;
+        float m = kNoScore, l = 0.0f;
+        bool ok = true;
+        for (int j = t0; j < t1; j++) {
+            const int n = j - t0;
+            if (!wait(bar_s, (uint32_t)(n & 1))) { ok = false; break; }
+            tc_fence_after();
+            uint32_t v[2][32];
+            tmem_ld_32x32(tmem + lane_addr, v[0]);
+            tmem_ld_32x32(tmem + 32 + lane_addr, v[1]);
+            tmem_ld_wait();
+            if (!__all_sync(0xffffffffu, sure - j * kPage >= kPage))
+#pragma unroll
+                for (int c = 0; c < 2; c++) {
+                    const uint32_t see = seen_word(c, sure, bits, s.ctx, j * kPage);
+#pragma unroll
+                    for (int x = 0; x < 32; x++)
+                        if (!(see >> x & 1u)) v[c][x] = 0xff800000u;
+                }
+            float mx = fmaxf(__uint_as_float(v[0][0]), __uint_as_float(v[1][0])), my = fmaxf(__uint_as_float(v[0][1]), __uint_as_float(v[1][1]));
+#pragma unroll
+            for (int x = 2; x < 32; x += 2) {
+                mx = max3(mx, __uint_as_float(v[0][x]), __uint_as_float(v[1][x]));
+                my = max3(my, __uint_as_float(v[0][x + 1]), __uint_as_float(v[1][x + 1]));
+            }
+            const float top = fmaxf(mx, my) * t.a2;
+            const bool grow = top > m + kSlack;
+            if (__any_sync(0xffffffffu, grow)) {
+                const float m_new = grow ? top : m, al = ex2_fast(m - m_new);
+                m = m_new;
+                l *= al;
+                if (n > 0) {
+                    if (!wait(bar_o, (uint32_t)((n - 1) & 1))) { ok = false; break; }
+                    tc_fence_after();
+                    for (int d = 0; d < t.vr; d += 16) {
+                        uint32_t u[16];
+                        tmem_ld_32x16(tO + d + lane_addr, u);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int x = 0; x < 16; x++) u[x] = __float_as_uint(__uint_as_float(u[x]) * al);
+                        tmem_st_32x16(tO + d + lane_addr, u);
+                    }
+                }
+            }
+            float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+            for (int c = 0; c < 2; c++) {
+                uint32_t pk[3][16];
+#pragma unroll
+                for (int x = 0; x < 32; x += 2) {
+                    float e0 = ex2_fast(__fmaf_rn(__uint_as_float(v[c][x]), t.a2, -m)), e1 = ex2_fast(__fmaf_rn(__uint_as_float(v[c][x + 1]), t.a2, -m));
+                    sum[0] += e0; sum[1] += e1;
+#pragma unroll
+                    for (int p = 0; p < 3; p++) {
+                        pk[p][x >> 1] = bf_pack(e0, e1);
+                        e0 -= bf_lo(pk[p][x >> 1]); e1 -= bf_hi(pk[p][x >> 1]);
+                    }
+                }
+#pragma unroll
+                for (int p = 0; p < 3; p++) tmem_st_32x16(tP + 32 * p + 16 * c + lane_addr, pk[p]);
+            }
+            l += sum[0] + sum[1];
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_p);
+        }
+        const bool any = t0 < t1;
+        if (ok && any) ok = wait(bar_f, 0);
+        if (ok) {
+            tc_fence_after();
+            const float rl = t.n_split > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
+            bool odd = false;
+            float* orow = reinterpret_cast<float*>(base_ptr) + (long)row * (a.dv + 4);
+            float* out = (float*)a.out + (long)(s.row0 + i) * a.ldo + (long)(h0 + hr) * a.dv;
+            const bool vec = whole_stores<float>(a);
+            for (int d0 = 0; d0 < t.vr; d0 += 16) {
+                uint32_t u[16];
+                if (any) {
+                    tmem_ld_32x16(tO + d0 + lane_addr, u);
+                    tmem_ld_wait();
+                } else {
+#pragma unroll
+                    for (int x = 0; x < 16; x++) u[x] = 0;
+                }
+#pragma unroll
+                for (int c = 0; c < 16; c += 8) {
+                    if (d0 + c >= a.dv) continue;
+                    float f[8];
+#pragma unroll
+                    for (int x = 0; x < 8; x++) f[x] = t.n_split == 1 && l == 0.0f ? 0.0f : __uint_as_float(u[c + x]) * rl;
+                    if (t.n_split > 1) {                  // this part's row into shared memory, over the operands (every product has been waited for)
+                        store8f(orow + d0 + c, f, true);
+                    } else if (live) {
+#pragma unroll
+                        for (int x = 0; x < 8; x++) odd = odd || not_finite(f[x]);
+                        store8f(out + d0 + c, f, vec);
+                    }
+                }
+            }
+            if (t.n_split > 1) {
+                float* ml = reinterpret_cast<float*>(base_ptr) + 128 * (a.dv + 4);
+                ml[row] = m; ml[128 + row] = l;
+            } else {
+                const unsigned bad = __ballot_sync(0xffffffffu, odd);
+                if (lane == 0) redo_sm[warp] = bad;
+            }
+        }
+    }
+    }
+    if (b >= 0 && t.n_split > 1) {
+        cluster_sync();
+        float* ml = reinterpret_cast<float*>(base_ptr) + 128 * (a.dv + 4);
+        join_parts<float, 1>(a, s, i0, t.RC, t.TQ, heads, h0, t.n_split, split, base, smem_u32(ml), smem_u32(ml + 128), ml + 256, redo_sm, kF32Threads);
+        cluster_sync();
+    }
+    tc_fence_before();
+    __syncthreads();
+    if ((redo_sm[0] | redo_sm[1] | redo_sm[2] | redo_sm[3]) && !*abort_flag)
+        for (int row = warp; row < 128; row += kF32Threads / 32)
+            if (redo_sm[row >> 5] >> (row & 31) & 1) attn_row_by_key<float>(a, b, s, i0 + row / t.RC, h0 + row % t.RC);
+    if (*abort_flag) {
+        const unsigned long long t_0 = globaltimer_ns();
+        while (globaltimer_ns() - t_0 < 200000ull) { __nanosleep(1000); }
+        if (threadIdx.x == 0 && a.seq.error_flag) atomicOr(a.seq.error_flag, 1);
+        __syncthreads();
+    }
+    if (warp == 13) { tc_fence_after(); tmem_dealloc(tmem, 512); }
+}
+
+}  // namespace
+
+int attn_paged_f32(const PagedAttn& a, cudaStream_t st) {
+    F32Args t = {};
+    const int R = a.H / a.G;
+    t.a = a;
+    t.RC = R < 128 ? R : 128; t.HC = (R + t.RC - 1) / t.RC; t.TQ = 128 / t.RC;
+    t.kc = (a.dk + 63) / 64; t.vr = (a.dv + 15) / 16 * 16; t.o_stride = (t.vr + 31) / 32 * 32;
+    t.a2 = a.scale * kLog2e;
+    if (t.a2 < 1e-30f) t.a2 = 1e-30f;                     // scale 0: weights all alike, and no infinity times zero
+    const long heads = (long)a.G * t.HC, seqs = a.seq.B < a.seq.T ? a.seq.B : a.seq.T, ones = a.seq.T / t.TQ + seqs;
+    if (heads > 65535 || ones * 8 > 0x7fffffffL) return FLEXLLM_ENOTSUP;
+    const long tiles = ((a.seq.T + seqs - 1) / seqs + t.TQ - 1) / t.TQ * seqs * heads;
+    t.n_split = key_splits(tiles, gemm_sm_count(), (a.seq.max_ctx + kPage) / kPage, 2);
+    const F32Smem o = f32_smem(t.kc, t.vr);
+    if (o.total > 226u * 1024u || (128u * (a.dv + 4) + 384u) * 4u > o.bars) return FLEXLLM_ENOTSUP;
+    TRY_RC(allow_shared(attn_paged_f32_kernel, o.total));
+    launch_cluster(attn_paged_f32_kernel, dim3((unsigned)(ones * t.n_split), (unsigned)heads), dim3(kF32Threads), t.n_split, o.total, st, t);
+    return launch_status();
+}
+
+}  // namespace flexllm

@@ -12,8 +12,7 @@
 // Warps 0 .. 4 W - 1 softmax (W sets, one row per thread), then one for TMA, one for the MMAs.
 // Keys behind a sequence's last one were never written: their scores are replaced, their values zeroed in shared memory. Any other value
 // that a row does not see meets a weight of zero; a row whose result is not finite is computed again, key by key.
-#include "attention_paged.cuh"
-#include "tc_common.cuh"
+#include "attention_join.cuh"
 
 namespace flexllm {
 
@@ -23,8 +22,6 @@ namespace {
 
 enum { kOne, kPair, kTurns };
 constexpr int KT = 128;                    // keys per tile
-constexpr float kSlack = 8.0f;             // log2 units by which a score may exceed its row's shift
-constexpr float kNoScore = -1e30f;
 
 struct TcArgs {
     PagedAttn a;
@@ -230,9 +227,7 @@ __global__ void __launch_bounds__(MODE == kOne ? 192 : 320, MODE == kOne ? 2 : 1
             if (masked) {
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
-                    const int nv = min(max(hi - 32 * c, 0), 32), sh = 32 * c - (s.ctx - j * KT);
-                    uint32_t see = nv == 32 ? 0xffffffffu : (1u << nv) - 1u;
-                    if (sh > -32 && sh < 64) see |= sh >= 0 ? (uint32_t)(bits >> sh) : (uint32_t)bits << -sh;
+                    const uint32_t see = seen_word(c, sure, bits, s.ctx, j * KT);
 #pragma unroll
                     for (int x = 0; x < 32; x++)
                         if (!(see >> x & 1u)) v[c][x] = 0xff800000u;
@@ -361,63 +356,7 @@ __global__ void __launch_bounds__(MODE == kOne ? 192 : 320, MODE == kOne ? 2 : 1
     }
     if (b >= 0 && (MODE == kTurns || (MODE == kOne && t.n_split > 1))) {
         if (t.n_split > 1) cluster_sync(); else __syncthreads();
-        // the rows' parts joined; CTA r of the cluster has rows r, r + n_split, ..: first the parts' weights (over the
-        // sums; parts x rows of a CTA are 128 STEP at most), then the outputs
-        constexpr int MOST = 8 * STEP;                     // parts: set p % STEP of CTA p / STEP
-        const int rows = min(t.TQ, s.n - i0) * t.RC, per = a.dv / 8, mine = (rows - split + t.n_split - 1) / t.n_split, parts = t.n_split * STEP;
-        for (int e = threadIdx.x; e < mine; e += NT) {
-            const int row = split + e * t.n_split;
-            float top = kNoScore, sum = 0.0f, mk[MOST], lk[MOST];
-#pragma unroll
-            for (int p = 0; p < MOST; p++)
-                if (p < parts) {
-                    mk[p] = ld_cluster_f32(cluster_addr(smem_u32(m_sm + (p % STEP) * 128 + row), p / STEP));
-                    lk[p] = ld_cluster_f32(cluster_addr(smem_u32(l_sm + (p % STEP) * 128 + row), p / STEP));
-                }
-#pragma unroll
-            for (int p = 0; p < MOST; p++)
-                if (p < parts) top = fmaxf(top, mk[p]);
-#pragma unroll
-            for (int p = 0; p < MOST; p++)
-                if (p < parts) { mk[p] = ex2_fast(mk[p] - top); sum = __fmaf_rn(lk[p], mk[p], sum); }
-            const float r = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-            for (int p = 0; p < MOST; p++)
-                if (p < parts) w_sm[p * mine + e] = sum == 0.0f ? 0.0f : mk[p] * r;
-        }
-        __syncthreads();
-        for (int e = threadIdx.x; e < mine * per; e += NT) {
-            const int i = e / per, row = split + i * t.n_split, d = e % per * 8;
-            if (row % t.RC >= heads) continue;
-            float f[8];
-#pragma unroll
-            for (int x = 0; x < 8; x++) f[x] = 0.0f;
-            for (int p0 = 0; p0 < parts; p0 += 4) {        // the loads of four parts are under way together
-                float4 x[4], y[4];
-#pragma unroll
-                for (int p = 0; p < 4; p++)
-                    if (p0 + p < parts) {
-                        const uint32_t at = cluster_addr(base + (uint32_t)(((p0 + p) % STEP * 128 + row) * (a.dv + 4) + d) * 4u, (p0 + p) / STEP);
-                        x[p] = ld_cluster_f32x4(at); y[p] = ld_cluster_f32x4(at + 16);
-                    }
-#pragma unroll
-                for (int p = 0; p < 4; p++)
-                    if (p0 + p < parts) {
-                        const float w = w_sm[(p0 + p) * mine + i];
-                        f[0] = __fmaf_rn(x[p].x, w, f[0]); f[1] = __fmaf_rn(x[p].y, w, f[1]); f[2] = __fmaf_rn(x[p].z, w, f[2]); f[3] = __fmaf_rn(x[p].w, w, f[3]);
-                        f[4] = __fmaf_rn(y[p].x, w, f[4]); f[5] = __fmaf_rn(y[p].y, w, f[5]); f[6] = __fmaf_rn(y[p].z, w, f[6]); f[7] = __fmaf_rn(y[p].w, w, f[7]);
-                    }
-            }
-            bf16* out = (bf16*)a.out + (long)(s.row0 + i0 + row / t.RC) * a.ldo + (long)(h0 + row % t.RC) * a.dv + d;
-            bool odd = false;
-#pragma unroll
-            for (int x = 0; x < 8; x++) odd = odd || not_finite(f[x]);
-            if (odd) atomicOr(&redo_sm[row >> 5], 1u << (row & 31));
-            if ((a.ldo & 7) == 0 && aligned16(a.out)) *reinterpret_cast<uint4*>(out) = make_uint4(bf_pack(f[0], f[1]), bf_pack(f[2], f[3]), bf_pack(f[4], f[5]), bf_pack(f[6], f[7]));
-            else
-#pragma unroll
-                for (int x = 0; x < 8; x++) out[x] = __float2bfloat16_rn(f[x]);
-        }
+        join_parts<bf16, STEP>(a, s, i0, t.RC, t.TQ, heads, h0, t.n_split, split, base, smem_u32(m_sm), smem_u32(l_sm), w_sm, redo_sm, NT);
         if (t.n_split > 1) cluster_sync();
     }
     tc_fence_before();
