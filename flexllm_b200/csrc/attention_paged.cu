@@ -285,7 +285,7 @@ template <int RT> int run_simt(const PagedAttn& a, cudaStream_t st) {
 
 int attn_paged_simt(const PagedAttn& a, cudaStream_t st) {
     const long rows = (long)(a.seq.T / a.seq.B) * (a.H / a.G);          // of an average sequence and a key/value head
-    if (a.dk <= 128 && a.dv <= 128 && rows > 0) return attn_paged_f32(a, st);
+    if (a.dk <= 128 && a.dv <= 128) return attn_paged_f32(a, st);
     return rows <= 16 ? run_simt<16>(a, st) : run_simt<64>(a, st);
 }
 
