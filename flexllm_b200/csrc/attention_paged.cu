@@ -284,8 +284,8 @@ template <int RT> int run_simt(const PagedAttn& a, cudaStream_t st) {
 }  // namespace
 
 int attn_paged_simt(const PagedAttn& a, cudaStream_t st) {
-    const long rows = (long)(a.seq.T / a.seq.B) * (a.H / a.G);          // of an average sequence and a key/value head
     if (a.dk <= 128 && a.dv <= 128) return attn_paged_f32(a, st);
+    const long rows = (long)(a.seq.T / a.seq.B) * (a.H / a.G);          // of an average sequence and a key/value head
     return rows <= 16 ? run_simt<16>(a, st) : run_simt<64>(a, st);
 }
 
@@ -293,7 +293,7 @@ namespace {
 int attn_paged(int dtype, const flexllm_kv_pages* kv, int heads, float scale, const void* q, long ldq, const uint64_t* mask, const int32_t* cu,
                const int32_t* ctx, const int32_t* page_table, int max_pages, int max_ctx, int B, int T, void* out, long ldo, void* stream) {
     FLEXLLM_REQUIRE(dtype == FLEXLLM_F32 || dtype == FLEXLLM_BF16);
-    FLEXLLM_REQUIRE(kv && kv->k && kv->v && kv->hkv > 0 && heads > 0 && heads % kv->hkv == 0 && kv->kdim > 0 && kv->vdim > 0);
+    FLEXLLM_REQUIRE(kv && kv->k && kv->v && kv->hkv > 0 && heads > 0 && heads <= 65535 && heads % kv->hkv == 0 && kv->kdim > 0 && kv->vdim > 0);
     PagedAttn a = {};
     a.seq = {cu, ctx, page_table, max_pages, max_ctx, B, T, kv->n_pages, mask ? 64 : 0x7fffffff, nullptr};
     a.H = heads; a.G = kv->hkv; a.dk = kv->kdim; a.dv = kv->vdim;

@@ -358,7 +358,8 @@ extern "C" int flexllm_linear_w4(int dtype, const void* a, long lda, const uint8
     FLEXLLM_REQUIRE(M >= 0 && N > 0 && K > 0 && group > 0 && group % 32 == 0 && K % group == 0 && lda >= K && lda % 8 == 0 && ldy >= N);
     if ((M + 63) / 64 > 65535 || K > 1 << 20) return FLEXLLM_ENOTSUP;
     if (M == 0) return FLEXLLM_OK;
-    FLEXLLM_REQUIRE(a && w && scale && y && aligned(a, 16) && aligned(w, 16));
+    FLEXLLM_REQUIRE(a && w && scale && y && aligned(a, 16) && aligned(w, 16) && aligned(scale, scale_dtype == FLEXLLM_F32 ? 4 : 2) && aligned(bias, 4) &&
+                    aligned(y, y_f32 || dtype == FLEXLLM_F32 ? 4 : 2));
     const W4Call c = {a, lda, w, scale, scale_dtype == FLEXLLM_F32, zero, group, bias, M, N, K, y, ldy, y_f32 != 0};
     const SetUpEarly early;
     if (dtype == FLEXLLM_BF16 && M > 8) return linear_w4_tc(c, (cudaStream_t)stream);

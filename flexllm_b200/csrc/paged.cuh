@@ -70,10 +70,13 @@ template <class Count> __device__ __forceinline__ Unit find_unit(const PackedSeq
     return r;
 }
 
-// The host's checks of those arguments.
-inline bool packed_ok(const PackedSeqs& p) {
-    return p.cu && p.ctx && p.page_table && p.B > 0 && p.T >= 0 && p.max_pages > 0 && p.n_pages > 0 && p.max_ctx >= 0 &&
+// The host's checks of those arguments. Positions stay far from the end of 32 bits, so that a sum with a row's index does.
+inline bool table_ok(const PackedSeqs& p) {
+    return p.ctx && p.page_table && aligned(p.ctx, 4) && aligned(p.page_table, 4) && p.max_pages > 0 && p.max_ctx >= 0 && p.max_ctx < 1 << 30 &&
            (long)p.max_ctx < (long)p.max_pages * kPage;
+}
+inline bool packed_ok(const PackedSeqs& p) {
+    return p.cu && aligned(p.cu, 4) && p.B > 0 && p.T >= 0 && p.n_pages > 0 && table_ok(p);
 }
 
 }  // namespace flexllm

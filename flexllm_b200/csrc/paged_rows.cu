@@ -77,12 +77,13 @@ template <class T, int L> __device__ __forceinline__ void rope_warp(const RopeAr
     int b = -1;
     for (int b0 = 0; b0 < a.seq.B; b0 += 32) b += __popc(__ballot_sync(0xffffffffu, b0 + lane < a.seq.B && a.seq.cu[b0 + lane] <= t));
     Four co = all_four(1.0f), si = all_four(0.0f);         // the other elements do not turn
+    bool outside = false;                                  // an error only if the row is a sequence's
     if (turns) {
         auto row_of = [&](int pair) {
             int axis = 0;
             while (axis < a.axes - 1 && pair >= a.sec_end[axis]) axis++;
             int row = a.pos[(long)axis * a.seq.T + t];
-            if ((unsigned)row >= (unsigned)a.table_len) { data_error(a.seq.error_flag); row = row < 0 ? 0 : a.table_len - 1; }
+            if ((unsigned)row >= (unsigned)a.table_len) { outside = true; row = row < 0 ? 0 : a.table_len - 1; }
             return (long)row * half + pair;
         };
         if (a.fours) {
@@ -99,6 +100,7 @@ template <class T, int L> __device__ __forceinline__ void rope_warp(const RopeAr
     if (b < 0) return;
     const SeqRows s = seq_rows(a.seq, b);
     if (t < s.row0 || t >= s.row0 + s.n) return;
+    if (outside) data_error(a.seq.error_flag);
     const int at = s.ctx + t - s.row0;
     const long page = h1 > a.H ? page_of(a.seq, b, at / kPage) : 0;
     const float inv_dk = 1.0f / (float)a.dk;
@@ -227,9 +229,10 @@ template <class T> __global__ void __launch_bounds__(256) kv_keep_kernel(const _
     if (tid < count) {
         PackedSeqs p = a.seq;
         p.n_pages = y.n_pages;
-        const int from = a.keep[(long)b * a.most + tid], s = ctx + from, d = ctx + tid;
-        if (ctx < 0 || from < 0 || from >= 64 || s > a.seq.max_ctx || d > a.seq.max_ctx) data_error(a.seq.error_flag);      // such an entry is not moved
-        else if (s != d) {
+        const int from = a.keep[(long)b * a.most + tid];
+        if (ctx < 0 || from < 0 || from >= 64 || max(from, tid) > a.seq.max_ctx - ctx) data_error(a.seq.error_flag);      // such an entry is not moved
+        else if (from != tid) {
+            const int s = ctx + from, d = ctx + tid;
             const int sp = page_of(p, b, s / kPage), dp = page_of(p, b, d / kPage), m = atomicAdd(&n_moves, 1);
             src_page[m] = sp; src_slot[m] = s & (kPage - 1);
             dst_page[m] = dp; dst_slot[m] = d & (kPage - 1);
@@ -285,13 +288,13 @@ extern "C" int flexllm_qk_norm_rope(int dtype, const flexllm_kv_pages* kv, int h
                                     int table_len, const int32_t* cu, const int32_t* ctx, const int32_t* page_table, int max_pages, int max_ctx, int B,
                                     int T, void* q, long ldq, void* stream) {
     FLEXLLM_REQUIRE(dtype == FLEXLLM_F32 || dtype == FLEXLLM_BF16);
-    FLEXLLM_REQUIRE(pages_ok(kv) && heads > 0 && eps >= 0.0f);
+    FLEXLLM_REQUIRE(pages_ok(kv) && heads > 0 && heads <= 65535 && kv->hkv <= 65535 && eps >= 0.0f);
     RopeArgs a = {};
     a.seq = {cu, ctx, page_table, max_pages, max_ctx, B, T, kv->n_pages, 0x7fffffff, nullptr};
     a.H = heads; a.G = kv->hkv; a.dk = kv->kdim; a.dv = kv->vdim; a.rot = rot;
     const long per16 = dtype == FLEXLLM_BF16 ? 8 : 4;
     FLEXLLM_REQUIRE(packed_ok(a.seq) && ldp >= (long)(a.H + a.G) * a.dk + (long)a.G * a.dv && ldq >= (long)a.H * a.dk && ldp % per16 == 0 && ldq % per16 == 0);
-    FLEXLLM_REQUIRE(rot >= 0 && rot <= a.dk && axes >= 1 && axes <= 4 && (axes == 1 || sections_host) && (rot == 0 || (cos_t && sin_t && table_len > 0)));
+    FLEXLLM_REQUIRE(rot >= 0 && rot <= a.dk && axes >= 1 && axes <= 4 && (axes == 1 || sections_host) && (rot == 0 || (cos_t && sin_t && aligned(cos_t, 4) && aligned(sin_t, 4) && table_len > 0)));
     if (!dims_ok(kv) || rot % 8) return FLEXLLM_ENOTSUP;
     int end = 0;
     for (int i = 0; i < axes; i++) {
@@ -302,7 +305,7 @@ extern "C" int flexllm_qk_norm_rope(int dtype, const flexllm_kv_pages* kv, int h
     }
     FLEXLLM_REQUIRE(end == rot / 2);
     if (T == 0) return FLEXLLM_OK;
-    FLEXLLM_REQUIRE(proj && q && (rot == 0 || pos) && aligned(proj, 16) && aligned(q, 16) && aligned(q_gain, 16) && aligned(k_gain, 16));
+    FLEXLLM_REQUIRE(proj && q && (rot == 0 || pos) && aligned(pos, 4) && aligned(proj, 16) && aligned(q, 16) && aligned(q_gain, 16) && aligned(k_gain, 16));
     a.fours = aligned(cos_t, 16) && aligned(sin_t, 16);
     for (int i = 0; i < axes; i++) a.fours = a.fours && a.sec_end[i] % 4 == 0;
     a.proj = proj; a.ldp = ldp; a.q_gain = q_gain; a.k_gain = k_gain; a.eps = eps; a.pos = pos; a.axes = axes;
@@ -315,20 +318,21 @@ extern "C" int flexllm_qk_norm_rope(int dtype, const flexllm_kv_pages* kv, int h
 extern "C" int flexllm_kv_keep(int dtype, const flexllm_kv_pages* layers_host, int layers, const int32_t* page_table, int max_pages, const int32_t* ctx,
                                int max_ctx, const int32_t* keep, const int32_t* count, int most, int B, void* stream) {
     FLEXLLM_REQUIRE(dtype == FLEXLLM_F32 || dtype == FLEXLLM_BF16);
-    FLEXLLM_REQUIRE(layers_host && layers > 0 && most >= 0 && B > 0 && B <= 0x7fffffff && page_table && ctx && max_pages > 0 && max_ctx >= 0 &&
-                    (long)max_ctx < (long)max_pages * kPage);
+    PackedSeqs seq = {nullptr, ctx, page_table, max_pages, max_ctx, B, 0, 0, 0, nullptr};
+    FLEXLLM_REQUIRE(layers_host && layers > 0 && most >= 0 && B > 0 && table_ok(seq));
     if (most > 64) return FLEXLLM_ENOTSUP;
     for (int i = 0; i < layers; i++) {
         FLEXLLM_REQUIRE(pages_ok(layers_host + i));
         if (!dims_ok(layers_host + i) || layers_host[i].hkv > 65535) return FLEXLLM_ENOTSUP;
     }
     if (most == 0) return FLEXLLM_OK;
-    FLEXLLM_REQUIRE(keep && count);
+    FLEXLLM_REQUIRE(keep && count && aligned(keep, 4) && aligned(count, 4));
+    seq.error_flag = device_error_flag();
     const SetUpEarly early;
     for (int l0 = 0; l0 < layers; l0 += kKeepLayers) {
         const int n = layers - l0 < kKeepLayers ? layers - l0 : kKeepLayers;
         KeepArgs a = {};
-        a.seq = {nullptr, ctx, page_table, max_pages, max_ctx, B, 0, 0, 0, device_error_flag()};
+        a.seq = seq;
         a.keep = keep; a.count = count; a.most = most;
         int heads = 0, widest = 0;
         for (int i = 0; i < n; i++) {

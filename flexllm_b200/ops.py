@@ -424,34 +424,45 @@ def _packed(like, page_table, cu, ctx, max_ctx):
 
 
 class PagedKV:
-    """A floating-point paged cache owned by the library: shapes [(kv heads, dim, vdim)] per layer. k[l] and v[l] are its pages as tensors."""
+    """A floating-point paged cache owned by the library: shapes [(kv heads, dim, vdim)] per layer. k[l] and v[l] are its pages as tensors, which keep
+    the memory until the last of them is gone."""
+
+    class _Memory:
+        def __init__(self):
+            self.h = C.c_void_p()
+
+        def __del__(self):
+            try:
+                lib().flexllm_kv_cache_destroy(self.h)
+            except Exception:
+                pass
 
     def __init__(self, n_pages, shapes, dtype=torch.bfloat16, device="cuda"):
-        self._h = C.c_void_p()
+        if dtype not in _DTYPE:
+            raise ValueError("flexllm_b200: pages are bfloat16 or float32, not %s" % dtype)
+        self._memory = m = PagedKV._Memory()
         dev = torch.empty(0, device=device).device
         size = 2 if dtype == torch.bfloat16 else 4
         kv = (_lib.KvShape * len(shapes))(*[_lib.KvShape(*s) for s in shapes])
         with torch.cuda.device(dev):
-            _check("flexllm_kv_cache_create_float", lib().flexllm_kv_cache_create_float(C.byref(self._h), len(shapes), n_pages, kv, 64, size))
+            _check("flexllm_kv_cache_create_float", lib().flexllm_kv_cache_create_float(C.byref(m.h), len(shapes), n_pages, kv, 64, size))
         self.k, self.v = [], []
         for layer, (g, dim, vdim) in enumerate(shapes):
             p = _lib.KvPages()
-            _check("flexllm_kv_cache_pages", lib().flexllm_kv_cache_pages(self._h, layer, C.byref(p)))
-            self.k.append(_wrap(p.k, (n_pages, g, 64, dim), dtype, dev))
-            self.v.append(_wrap(p.v, (n_pages, g, vdim, 64), dtype, dev))
+            _check("flexllm_kv_cache_pages", lib().flexllm_kv_cache_pages(m.h, layer, C.byref(p)))
+            self.k.append(_wrap(m, p.k, (n_pages, g, 64, dim), dtype, dev))
+            self.v.append(_wrap(m, p.v, (n_pages, g, vdim, 64), dtype, dev))
 
     def close(self):
-        if self._h:
-            self.k, self.v = [], []
-            lib().flexllm_kv_cache_destroy(self._h)
-            self._h = C.c_void_p()
+        self.k, self.v, self._memory = [], [], None
 
 
-def _wrap(ptr, shape, dtype, device):
-    """Device memory of the library as a tensor (bfloat16 has no type string: as int16, seen as bfloat16)."""
+def _wrap(memory, ptr, shape, dtype, device):
+    """Device memory of the library as a tensor that holds on to it (bfloat16 has no type string: as int16, seen as bfloat16)."""
     class _H:
         pass
     h = _H()
+    h.memory = memory
     h.__cuda_array_interface__ = {"shape": tuple(shape), "typestr": "<i2" if dtype == torch.bfloat16 else "<f4", "data": (ptr, False), "version": 2}
     t = torch.as_tensor(h, device=device)
     return t.view(torch.bfloat16) if dtype == torch.bfloat16 else t
