@@ -38,13 +38,13 @@ __global__ void __launch_bounds__(256, RT * NV <= 256 ? 2 : 1) attn_paged_simt_k
     __shared__ unsigned redo_sm[2];
     const PagedAttn& a = sa.a;
     const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-    const int tile = blockIdx.x / n_split, split = blockIdx.x % n_split;
-    const int g = blockIdx.y / sa.HC, h0 = g * (a.H / a.G) + (blockIdx.y % sa.HC) * sa.RC;
+    const int tile = blockIdx.x / n_split, split = blockIdx.x % n_split, all = a.G * sa.HC, hg = tile % all;
+    const int g = hg / sa.HC, h0 = g * (a.H / a.G) + (hg % sa.HC) * sa.RC;
     const int heads = min(sa.RC, (g + 1) * (a.H / a.G) - h0);
     pdl_sync();
     if (tid < 32) {
         const int TQ = sa.TQ;
-        const Unit u = find_unit(a.seq, tile, [TQ](const SeqRows& s) { return (s.n + TQ - 1) / TQ; });
+        const Unit u = find_unit(a.seq, tile / all, [TQ](const SeqRows& s) { return (s.n + TQ - 1) / TQ; });
         if (tid == 0) { unit_sm = u; redo_sm[0] = redo_sm[1] = 0; }
     }
     __syncthreads();
@@ -264,7 +264,7 @@ template <int RT, int NV> int launch_simt(SimtArgs& sa, int tiles, int splits, c
     const size_t smem = simt_floats(RT, sa.a.dk, NV * 16, sa.bufs) * 4;
     auto kern = attn_paged_simt_kernel<RT, NV>;
     TRY_RC(allow_shared(kern, smem));
-    launch_cluster(kern, dim3(tiles * splits, sa.a.G * sa.HC), dim3(256), splits, smem, st, sa, splits);
+    launch_cluster(kern, dim3((unsigned)tiles * splits * sa.a.G * sa.HC), dim3(256), splits, smem, st, sa, splits);
     return launch_status();
 }
 template <int RT> int run_simt(const PagedAttn& a, cudaStream_t st) {
@@ -273,9 +273,9 @@ template <int RT> int run_simt(const PagedAttn& a, cudaStream_t st) {
     sa.a = a;
     sa.RC = R < RT ? R : RT; sa.HC = (R + sa.RC - 1) / sa.RC; sa.TQ = RT / sa.RC;
     const long seqs = a.seq.B < a.seq.T ? a.seq.B : a.seq.T;
-    const long tiles = a.seq.T / sa.TQ + seqs, real = ((a.seq.T + seqs - 1) / seqs + sa.TQ - 1) / sa.TQ * seqs;      // at most; with sequences of equal length
+    const long tiles = most_units(a.seq, sa.TQ), real = ((a.seq.T + seqs - 1) / seqs + sa.TQ - 1) / sa.TQ * seqs;      // at most; with sequences of equal length
     const int splits = key_splits(real * a.G * sa.HC, 2 * gemm_sm_count(), (a.seq.max_ctx + kPage) / kPage, 1);
-    if (tiles * splits > 0x7fffffffL || a.G * sa.HC > 65535) return FLEXLLM_ENOTSUP;
+    if (tiles * splits * a.G * sa.HC > 0x7fffffffL) return FLEXLLM_ENOTSUP;
     if (a.dv <= 64) return launch_simt<RT, 4>(sa, (int)tiles, splits, st);
     if (a.dv <= 128) return launch_simt<RT, 8>(sa, (int)tiles, splits, st);
     return launch_simt<RT, 16>(sa, (int)tiles, splits, st);

@@ -20,7 +20,7 @@ constexpr uint32_t kPieceBytes = 8192;
 
 struct F32Args {
     PagedAttn a;
-    int RC, HC, TQ;                        // heads per tile, head chunks per group, tokens per tile
+    int RC, HC, TQ, heads;                 // heads per tile, head chunks per group, tokens per tile, head chunks
     int kc, vr, o_stride, n_split;         // 128-byte blocks of a part's Q or K row, rows of a V^T part, columns of O
     float a2;                              // scale * log2 e
 };
@@ -77,18 +77,19 @@ __global__ void __launch_bounds__(kF32Threads, 1) attn_paged_f32_kernel(const __
     if (threadIdx.x < 4) redo_sm[threadIdx.x] = 0;
     if (warp == 13) { tmem_alloc(smem_u32(tmem_slot), 512); tmem_relinquish(); }
     pdl_sync();
+    const int tile = blockIdx.x / t.n_split, split = blockIdx.x % t.n_split, hg = tile % t.heads;
     if (warp == 0) {
         const int TQ = t.TQ;
-        const Unit u = find_unit(a.seq, (int)blockIdx.x / t.n_split, [TQ](const SeqRows& s) { return (s.n + TQ - 1) / TQ; });
+        const Unit u = find_unit(a.seq, tile / t.heads, [TQ](const SeqRows& s) { return (s.n + TQ - 1) / TQ; });
         if (lane == 0) unit_sm = u;
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot, tP = tmem + 64, tO = tmem + 192;
-    const int split = blockIdx.x % t.n_split, b = unit_sm.b;
+    const int b = unit_sm.b;
     const SeqRows s = unit_sm.s;
-    const int R = a.H / a.G, g = blockIdx.y / t.HC, h0 = g * R + (blockIdx.y % t.HC) * t.RC, heads = min(t.RC, (g + 1) * R - h0);
+    const int R = a.H / a.G, g = hg / t.HC, h0 = g * R + (hg % t.HC) * t.RC, heads = min(t.RC, (g + 1) * R - h0);
     const int i0 = unit_sm.i * t.TQ;                      // first row of the tile within the sequence
     const int end = b < 0 ? 0 : a.mask ? s.ctx + s.n : min(s.ctx + i0 + t.TQ, s.ctx + s.n), n_pg = (end + kPage - 1) / kPage;
     const int t0 = (int)((long)n_pg * split / t.n_split), t1 = (int)((long)n_pg * (split + 1) / t.n_split);
@@ -375,14 +376,15 @@ int attn_paged_f32(const PagedAttn& a, cudaStream_t st) {
     t.kc = (a.dk + 63) / 64; t.vr = (a.dv + 15) / 16 * 16; t.o_stride = (t.vr + 31) / 32 * 32;
     t.a2 = a.scale * kLog2e;
     if (t.a2 < 1e-30f) t.a2 = 1e-30f;                     // scale 0: weights all alike, and no infinity times zero
-    const long heads = (long)a.G * t.HC, seqs = a.seq.B < a.seq.T ? a.seq.B : a.seq.T, ones = a.seq.T / t.TQ + seqs;
-    if (heads > 65535 || ones * 8 > 0x7fffffffL) return FLEXLLM_ENOTSUP;
+    const long heads = (long)a.G * t.HC, seqs = a.seq.B < a.seq.T ? a.seq.B : a.seq.T, ones = most_units(a.seq, t.TQ);
+    t.heads = (int)heads;
+    if (ones * 8 * heads > 0x7fffffffL) return FLEXLLM_ENOTSUP;
     const long tiles = ((a.seq.T + seqs - 1) / seqs + t.TQ - 1) / t.TQ * seqs * heads;
     t.n_split = key_splits(tiles, gemm_sm_count(), (a.seq.max_ctx + kPage) / kPage, 2);
     const F32Smem o = f32_smem(t.kc, t.vr);
     if (o.total > 226u * 1024u || (128u * (a.dv + 4) + 384u) * 4u > o.bars) return FLEXLLM_ENOTSUP;
     TRY_RC(allow_shared(attn_paged_f32_kernel, o.total));
-    launch_cluster(attn_paged_f32_kernel, dim3((unsigned)(ones * t.n_split), (unsigned)heads), dim3(kF32Threads), t.n_split, o.total, st, t);
+    launch_cluster(attn_paged_f32_kernel, dim3((unsigned)(ones * t.n_split * heads)), dim3(kF32Threads), t.n_split, o.total, st, t);
     return launch_status();
 }
 

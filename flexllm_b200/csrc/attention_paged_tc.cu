@@ -25,7 +25,7 @@ constexpr int KT = 128;                    // keys per tile
 
 struct TcArgs {
     PagedAttn a;
-    int RC, HC, TQ;                        // heads per tile, head chunks per group, tokens per tile
+    int RC, HC, TQ, heads;                 // heads per tile, head chunks per group, tokens per tile, head chunks
     int kc, vr;                            // 128-byte blocks of a Q or K row, rows of a V^T tile (dv rounded up to 16)
     int ks, vs;                            // stages of K and V
     float a2;                              // scale * log2 e
@@ -82,18 +82,20 @@ __global__ void __launch_bounds__(MODE == kOne ? 192 : 320, MODE == kOne ? 2 : 1
     if (warp == WM) { tmem_alloc(smem_u32(tmem_slot), t.tmem_cols); tmem_relinquish(); }
     if (warp == WT && lane == 0) { tma_prefetch_desc(&tmapQ); tma_prefetch_desc(&tmapK); tma_prefetch_desc(&tmapV); }
     pdl_sync();
+    // tiles' heads before tiles, so that CTAs without a tile (the host knows the most there can be) start when no other is left
+    const int tile = blockIdx.x / t.n_split, split = blockIdx.x % t.n_split, hg = tile % t.heads;
     if (warp == 0) {
         const int per = NQ * t.TQ;
-        const Unit u = find_unit(a.seq, (int)blockIdx.x / t.n_split, [per](const SeqRows& s) { return (s.n + per - 1) / per; });
+        const Unit u = find_unit(a.seq, tile / t.heads, [per](const SeqRows& s) { return (s.n + per - 1) / per; });
         if (lane == 0) unit_sm = u;
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    const int split = blockIdx.x % t.n_split, b = unit_sm.b;
+    const int b = unit_sm.b;
     const SeqRows s = unit_sm.s;
-    const int R = a.H / a.G, g = blockIdx.y / t.HC, h0 = g * R + (blockIdx.y % t.HC) * t.RC, heads = min(t.RC, (g + 1) * R - h0);
+    const int R = a.H / a.G, g = hg / t.HC, h0 = g * R + (hg % t.HC) * t.RC, heads = min(t.RC, (g + 1) * R - h0);
     const int i0 = unit_sm.i * NQ * t.TQ;                 // first row of the first tile within the sequence
     // key tiles [t0, t1[q]) of the tiles q; `end`: keys that exist for the last row
     int end = 0, t0 = 0, t1[NQ];
@@ -398,7 +400,7 @@ template <int MODE> int launch_tc(TcArgs& t, long tiles, cudaStream_t st) {
     TRY_RC(make_tmap_2d_u8(&tv, a.v, (uint64_t)a.seq.n_pages * a.G * a.dv, kPage * 2, (uint32_t)t.vr));
     auto kern = attn_paged_tc_kernel<MODE>;
     TRY_RC(allow_shared(kern, o.total));
-    launch_cluster(kern, dim3((unsigned)(tiles * t.n_split), a.G * t.HC), dim3(NT), t.n_split, o.total, st, tq, tk, tv, t);
+    launch_cluster(kern, dim3((unsigned)(tiles * t.n_split * t.heads)), dim3(NT), t.n_split, o.total, st, tq, tk, tv, t);
     return launch_status();
 }
 
@@ -413,8 +415,9 @@ int attn_paged_tc(const PagedAttn& a, cudaStream_t st) {
     t.a2 = a.scale * kLog2e;
     if (t.a2 < 1e-30f) t.a2 = 1e-30f;                     // scale 0: weights all alike, and no infinity times zero
     const long heads = (long)a.G * t.HC, seqs = a.seq.B < a.seq.T ? a.seq.B : a.seq.T;
-    const long pairs = a.seq.T / (2 * t.TQ) + seqs, ones = a.seq.T / t.TQ + seqs;         // at most so many exist
-    if (heads > 65535 || ones * 8 > 0x7fffffffL) return FLEXLLM_ENOTSUP;
+    const long pairs = most_units(a.seq, 2 * t.TQ), ones = most_units(a.seq, t.TQ);
+    t.heads = (int)heads;
+    if (ones * 8 * heads > 0x7fffffffL) return FLEXLLM_ENOTSUP;
     const long sms = gemm_sm_count(), tiles = ((a.seq.T + seqs - 1) / seqs + t.TQ - 1) / t.TQ * seqs * heads;      // if all sequences are of equal length
     const int pages = (a.seq.max_ctx + kPage) / kPage;
     t.n_split = 1;

@@ -70,6 +70,12 @@ template <class Count> __device__ __forceinline__ Unit find_unit(const PackedSeq
     return r;
 }
 
+// At most so many units of `per` rows have T rows of B sequences: the first row of a sequence opens one.
+inline long most_units(const PackedSeqs& p, int per) {
+    const long seqs = p.B < p.T ? p.B : p.T;
+    return seqs + (p.T - seqs) / per;
+}
+
 // The host's checks of those arguments. Positions stay far from the end of 32 bits, so that a sum with a row's index does.
 inline bool table_ok(const PackedSeqs& p) {
     return p.ctx && p.page_table && aligned(p.ctx, 4) && aligned(p.page_table, 4) && p.max_pages > 0 && p.max_ctx >= 0 && p.max_ctx < 1 << 30 &&

@@ -189,8 +189,8 @@ template <class T, int L> __global__ void __launch_bounds__(256, 4) qk_norm_rope
 template <class T, int L> int launch_rope(RopeArgs& a, cudaStream_t st) {
     a.chunks = (a.H + a.G + kRopeHeads - 1) / kRopeHeads;
     const long qk = ((long)a.seq.T * a.chunks + 7) / 8;
-    // a sequence's rows touch at most two pages more than they would fill
-    const long units = (long)a.seq.T / kPage + 2L * (a.seq.B < a.seq.T ? a.seq.B : a.seq.T);
+    // a sequence's first row opens a page, the next one another, and so does every 64th
+    const long seqs = a.seq.B < a.seq.T ? a.seq.B : a.seq.T, next = a.seq.T - seqs, units = seqs + (next + (kPage - 1) * (next < seqs ? next : seqs)) / kPage;
     if (qk + units * a.G > 0x7fffffffL || qk > 0x1fffffffL) return FLEXLLM_ENOTSUP;      // warps are counted in 32 bits
     a.qk_ctas = (int)qk;
     const size_t smem = (size_t)kPage * (a.dv * sizeof(T) + 4);
