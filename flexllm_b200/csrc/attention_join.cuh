@@ -22,34 +22,43 @@ __device__ __forceinline__ void store8f(float* p, const float (&f)[8], bool vec)
 }
 template <class T> __device__ __forceinline__ bool whole_stores(const PagedAttn& a) { return a.ldo % (16 / (int)sizeof(T)) == 0 && aligned16(a.out); }
 
+constexpr int kJoinRows = 144;             // rows of a tile and 16 CTAs, a multiple of their number: up to 15 more
+
+template <class K> inline int allow_cluster(K kern, int size) {
+    return size <= 8 ? FLEXLLM_OK : cuda_status(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+}
+
 // The parts of a tile of 128 rows, STEP of them in each of the n_split CTAs of a cluster, joined by all nt threads of every CTA: maxima (log2 units) and
 // sums at m_at and l_at, [STEP][128], outputs at o_at, [STEP][128][dv + 4], at the same addresses in every CTA and fenced. CTA r of the
-// cluster has rows r, r + n_split, ..: first the parts' weights (over the sums; parts x rows of a CTA are 128 STEP at most), then the outputs.
+// cluster has rows r, r + n_split, ..: first the parts' weights (over the sums; parts x rows of a CTA are kJoinRows STEP at most), then the outputs.
 template <class T, int STEP>
 __device__ __forceinline__ void join_parts(const PagedAttn& a, const SeqRows& s, int i0, int RC, int TQ, int heads, int h0, int n_split, int split, uint32_t o_at,
                                            uint32_t m_at, uint32_t l_at, float* w_sm, unsigned* redo_sm, int nt) {
     using namespace tc;
-    constexpr int MOST = 8 * STEP;                     // parts: set p % STEP of CTA p / STEP
+    constexpr int N = 8 * STEP;                        // parts looked at together: set p % STEP of CTA p / STEP
     const int rows = min(TQ, s.n - i0) * RC, per = a.dv / 8, mine = (rows - split + n_split - 1) / n_split, parts = n_split * STEP;
     for (int e = threadIdx.x; e < mine; e += nt) {
         const int row = split + e * n_split;
-        float top = kNoScore, sum = 0.0f, mk[MOST], lk[MOST];
+        float top = kNoScore, sum = 0.0f;
+        for (int p0 = 0; p0 < parts; p0 += N) {
+            float mk[N], lk[N];
+            const float before = top;
 #pragma unroll
-        for (int p = 0; p < MOST; p++)
-            if (p < parts) {
-                mk[p] = ld_cluster_f32(cluster_addr(m_at + ((p % STEP) * 128 + row) * 4, p / STEP));
-                lk[p] = ld_cluster_f32(cluster_addr(l_at + ((p % STEP) * 128 + row) * 4, p / STEP));
-            }
+            for (int p = 0; p < N; p++)
+                if (p0 + p < parts) {
+                    mk[p] = ld_cluster_f32(cluster_addr(m_at + ((p % STEP) * 128 + row) * 4, (p0 + p) / STEP));
+                    lk[p] = ld_cluster_f32(cluster_addr(l_at + ((p % STEP) * 128 + row) * 4, (p0 + p) / STEP));
+                }
 #pragma unroll
-        for (int p = 0; p < MOST; p++)
-            if (p < parts) top = fmaxf(top, mk[p]);
+            for (int p = 0; p < N; p++)
+                if (p0 + p < parts) top = fmaxf(top, mk[p]);
+            sum *= ex2_fast(before - top);
 #pragma unroll
-        for (int p = 0; p < MOST; p++)
-            if (p < parts) { mk[p] = ex2_fast(mk[p] - top); sum = __fmaf_rn(lk[p], mk[p], sum); }
+            for (int p = 0; p < N; p++)
+                if (p0 + p < parts) { sum = __fmaf_rn(lk[p], ex2_fast(mk[p] - top), sum); w_sm[(p0 + p) * mine + e] = mk[p]; }
+        }
         const float r = sum == 0.0f ? 0.0f : 1.0f / sum;
-#pragma unroll
-        for (int p = 0; p < MOST; p++)
-            if (p < parts) w_sm[p * mine + e] = sum == 0.0f ? 0.0f : mk[p] * r;
+        for (int p = 0; p < parts; p++) w_sm[p * mine + e] = sum == 0.0f ? 0.0f : ex2_fast(w_sm[p * mine + e] - top) * r;
     }
     __syncthreads();
     for (int e = threadIdx.x; e < mine * per; e += nt) {

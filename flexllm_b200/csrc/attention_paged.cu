@@ -274,7 +274,7 @@ template <int RT> int run_simt(const PagedAttn& a, cudaStream_t st) {
     sa.RC = R < RT ? R : RT; sa.HC = (R + sa.RC - 1) / sa.RC; sa.TQ = RT / sa.RC;
     const long seqs = a.seq.B < a.seq.T ? a.seq.B : a.seq.T;
     const long tiles = most_units(a.seq, sa.TQ), real = ((a.seq.T + seqs - 1) / seqs + sa.TQ - 1) / sa.TQ * seqs;      // at most; with sequences of equal length
-    const int splits = key_splits(real * a.G * sa.HC, 2 * gemm_sm_count(), (a.seq.max_ctx + kPage) / kPage, 1);
+    const int splits = key_splits(real * a.G * sa.HC, false, (a.seq.max_ctx + kPage) / kPage, 1, 8);
     if (tiles * splits * a.G * sa.HC > 0x7fffffffL) return FLEXLLM_ENOTSUP;
     if (a.dv <= 64) return launch_simt<RT, 4>(sa, (int)tiles, splits, st);
     if (a.dv <= 128) return launch_simt<RT, 8>(sa, (int)tiles, splits, st);

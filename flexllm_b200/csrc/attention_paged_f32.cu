@@ -76,7 +76,7 @@ __global__ void __launch_bounds__(kF32Threads, 1) attn_paged_f32_kernel(const __
     }
     if (threadIdx.x < 4) redo_sm[threadIdx.x] = 0;
     if (warp == 13) { tmem_alloc(smem_u32(tmem_slot), 512); tmem_relinquish(); }
-    pdl_sync();
+    pdl_wait();
     const int tile = blockIdx.x / t.n_split, split = blockIdx.x % t.n_split, hg = tile % t.heads;
     if (warp == 0) {
         const int TQ = t.TQ;
@@ -86,6 +86,7 @@ __global__ void __launch_bounds__(kF32Threads, 1) attn_paged_f32_kernel(const __
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    pdl_launch();                                         // behind the allocation: no later kernel may hold the TMEM that this one waits for
     const uint32_t tmem = *tmem_slot, tP = tmem + 64, tO = tmem + 192;
     const int b = unit_sm.b;
     const SeqRows s = unit_sm.s;
@@ -378,12 +379,13 @@ int attn_paged_f32(const PagedAttn& a, cudaStream_t st) {
     if (t.a2 < 1e-30f) t.a2 = 1e-30f;                     // scale 0: weights all alike, and no infinity times zero
     const long heads = (long)a.G * t.HC, seqs = a.seq.B < a.seq.T ? a.seq.B : a.seq.T, ones = most_units(a.seq, t.TQ);
     t.heads = (int)heads;
-    if (ones * 8 * heads > 0x7fffffffL) return FLEXLLM_ENOTSUP;
+    if (ones * 16 * heads > 0x7fffffffL) return FLEXLLM_ENOTSUP;
     const long tiles = ((a.seq.T + seqs - 1) / seqs + t.TQ - 1) / t.TQ * seqs * heads;
-    t.n_split = key_splits(tiles, gemm_sm_count(), (a.seq.max_ctx + kPage) / kPage, 2);
+    t.n_split = key_splits(tiles, false, (a.seq.max_ctx + kPage) / kPage, 2, 16);
     const F32Smem o = f32_smem(t.kc, t.vr);
-    if (o.total > 226u * 1024u || (128u * (a.dv + 4) + 384u) * 4u > o.bars) return FLEXLLM_ENOTSUP;
+    if (o.total > 226u * 1024u || (128u * (a.dv + 4) + 256u + kJoinRows) * 4u > o.bars) return FLEXLLM_ENOTSUP;
     TRY_RC(allow_shared(attn_paged_f32_kernel, o.total));
+    TRY_RC(allow_cluster(attn_paged_f32_kernel, t.n_split));
     launch_cluster(attn_paged_f32_kernel, dim3((unsigned)(ones * t.n_split * heads)), dim3(kF32Threads), t.n_split, o.total, st, t);
     return launch_status();
 }

@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(MODE == kOne ? 192 : 320, MODE == kOne ? 2 : 1
     extern __shared__ uint8_t smem_raw[];
     __shared__ Unit unit_sm;
     __shared__ unsigned redo_sm[4 * NQ];
-    __shared__ float m_sm[W * 128], l_sm[W * 128], w_sm[NQ == 2 ? 1 : 128 * STEP];
+    __shared__ float m_sm[W * 128], l_sm[W * 128], w_sm[NQ == 2 ? 1 : kJoinRows * STEP];
     const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
     uint8_t* base_ptr = smem_raw + (base - raw);
     const PagedAttn& a = t.a;
@@ -81,7 +81,7 @@ __global__ void __launch_bounds__(MODE == kOne ? 192 : 320, MODE == kOne ? 2 : 1
     if (threadIdx.x < 4 * NQ) redo_sm[threadIdx.x] = 0;
     if (warp == WM) { tmem_alloc(smem_u32(tmem_slot), t.tmem_cols); tmem_relinquish(); }
     if (warp == WT && lane == 0) { tma_prefetch_desc(&tmapQ); tma_prefetch_desc(&tmapK); tma_prefetch_desc(&tmapV); }
-    pdl_sync();
+    pdl_wait();
     // tiles' heads before tiles, so that CTAs without a tile (the host knows the most there can be) start when no other is left
     const int tile = blockIdx.x / t.n_split, split = blockIdx.x % t.n_split, hg = tile % t.heads;
     if (warp == 0) {
@@ -92,6 +92,7 @@ __global__ void __launch_bounds__(MODE == kOne ? 192 : 320, MODE == kOne ? 2 : 1
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    pdl_launch();                                         // behind the allocation: no later kernel may hold the TMEM that this one waits for
     const uint32_t tmem = *tmem_slot;
     const int b = unit_sm.b;
     const SeqRows s = unit_sm.s;
@@ -400,11 +401,37 @@ template <int MODE> int launch_tc(TcArgs& t, long tiles, cudaStream_t st) {
     TRY_RC(make_tmap_2d_u8(&tv, a.v, (uint64_t)a.seq.n_pages * a.G * a.dv, kPage * 2, (uint32_t)t.vr));
     auto kern = attn_paged_tc_kernel<MODE>;
     TRY_RC(allow_shared(kern, o.total));
+    TRY_RC(allow_cluster(kern, t.n_split));
     launch_cluster(kern, dim3((unsigned)(tiles * t.n_split * t.heads)), dim3(NT), t.n_split, o.total, st, tq, tk, tv, t);
     return launch_status();
 }
 
+int most_clusters(int size) {
+    auto kern = attn_paged_tc_kernel<kTurns>;
+    const size_t smem = kWholeSm - 4096;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = size; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(size); cfg.blockDim = dim3(320); cfg.dynamicSmemBytes = smem; cfg.attrs = at; cfg.numAttrs = 1;
+    int n = 0;
+    if (allow_shared(kern, smem) || allow_cluster(kern, size) || cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) {
+        cudaGetLastError();                               // not known: keys are not cut
+        return 0;
+    }
+    return n;
+}
+
 }  // namespace
+
+int cluster_slots(int size, bool two) {
+    struct Table {
+        int n[17];
+        Table() { for (int s = 1; s <= 16; s++) n[s] = most_clusters(s); }
+    };
+    static const Table table;
+    return two ? (size == 1 ? 2 * table.n[1] : table.n[(size + 1) / 2]) : table.n[size];
+}
 
 int attn_paged_tc(const PagedAttn& a, cudaStream_t st) {
     TcArgs t = {};
@@ -417,20 +444,37 @@ int attn_paged_tc(const PagedAttn& a, cudaStream_t st) {
     const long heads = (long)a.G * t.HC, seqs = a.seq.B < a.seq.T ? a.seq.B : a.seq.T;
     const long pairs = most_units(a.seq, 2 * t.TQ), ones = most_units(a.seq, t.TQ);
     t.heads = (int)heads;
-    if (ones * 8 * heads > 0x7fffffffL) return FLEXLLM_ENOTSUP;
+    if (ones * 16 * heads > 0x7fffffffL) return FLEXLLM_ENOTSUP;
     const long sms = gemm_sm_count(), tiles = ((a.seq.T + seqs - 1) / seqs + t.TQ - 1) / t.TQ * seqs * heads;      // if all sequences are of equal length
     const int pages = (a.seq.max_ctx + kPage) / kPage;
     t.n_split = 1;
     if (a.dk <= 128 && a.dv <= 128) {
         if (tiles <= sms) {
-            t.n_split = key_splits(tiles, sms, pages, 2 * KT / kPage);
-            return launch_tc<kTurns>(t, ones, st);
+            // What the call takes in microseconds, cut into s parts, by one CTA of kTurns or two of kOne per SM: a time per key tile, one for the call, and
+            // one per part for joining rows (a tree of 26 over 1000, kTurns and kOne: 17.6 and 15.2; 16 of 31 over 8000: 103 and 89; 9 of 10
+            // over 4000: 34 and 44; one token over 100000: 62 and 157)
+            const float rows = (float)((a.seq.T + seqs - 1) / seqs < t.TQ ? (a.seq.T + seqs - 1) / seqs * t.RC : 128) / 128;
+            const int n = (pages + 1) / 2;
+            float best = 3e38f;
+            bool turns = true;
+            for (int s = 1; s <= 16 && s <= n; s++) {
+                const float each = (float)((n + s - 1) / s);
+                const int alone = cluster_slots(s, false);
+                const float two_sets = 1.1f * each + 11.0f + 1.6f * s * rows;
+                const float one_set = (alone >= tiles ? 1.85f * each + 8.0f : 2.1f * each + 9.0f) + (s > 1 ? 2.5f + 0.8f * s * rows : 0.0f);
+                if (two_sets < best && alone >= tiles) { best = two_sets; turns = true; t.n_split = s; }
+                if (one_set < best && cluster_slots(s, true) >= tiles) { best = one_set; turns = false; t.n_split = s; }
+            }
+            return turns ? launch_tc<kTurns>(t, ones, st) : launch_tc<kOne>(t, ones, st);
         }
         // pairs where sequences fill them and every SM has one
         if ((long)a.seq.T >= 2L * t.TQ * seqs && tiles >= 2 * sms) return launch_tc<kPair>(t, pairs, st);
+        // long ones are cut although each has its place: sequences differ (20 trees of 20 over 6000: 105 us against 112, 32 of 28 over 8000: 199 against
+        // 228, 32 single tokens over 8000: 154 against 152, over 2000: 56 against 48)
+        if (tiles <= 4 * sms && pages >= 80) t.n_split = 2;
         return launch_tc<kOne>(t, ones, st);
     }
-    t.n_split = key_splits(tiles, sms, pages, KT / kPage);
+    t.n_split = key_splits(tiles, false, pages, KT / kPage, 16);
     return launch_tc<kOne>(t, ones, st);
 }
 

@@ -63,7 +63,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_w4_tc_kernel(const __gri
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
-    pdl_sync();
+    pdl_sync();                                           // behind the allocation: no later kernel may hold the TMEM that this one waits for
     const int split = blockIdx.x % t.n_split, n0 = blockIdx.x / t.n_split * 128, m0 = blockIdx.y * 64;
     const int s0 = (int)((long)t.steps * split / t.n_split), s1 = (int)((long)t.steps * (split + 1) / t.n_split);
     // all lanes look: one that looks for the others and tells them takes twice as long

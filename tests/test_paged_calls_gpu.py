@@ -309,3 +309,20 @@ def test_library_owned_pages(ops):
     kv = ops.PagedKV(2, [(1, 64, 64)])
     assert kv.k[0].dtype == BF and math.isfinite(float(kv.v[0].float().sum()))
     kv.close()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF], ids=["f32", "bf16"])
+@pytest.mark.parametrize("H,G,dim,new,ctx", [(8, 1, 128, [1], [30000]), (8, 1, 64, [33], [12000]), (8, 2, 128, [40, 7], [3000, 10]), (12, 3, 64, [5], [5000]), (4, 4, 128, [1, 1, 0, 1], [2500, 0, 90, 700]),
+                                             (16, 8, 128, [9, 2], [1500, 1501]), (10, 5, 96, [17], [20000]), (8, 8, 64, [3, 3, 3], [640, 639, 0]), (3, 1, 256, [20], [9000])],
+                         ids=lambda v: str(v).replace(" ", ""))
+def test_keys_cut_into_any_number_of_parts(ops, dtype, H, G, dim, new, ctx):
+    table, start, cx, n_pages = pc.layout(new, ctx, seed=3)
+    g = torch.Generator(device="cuda").manual_seed(4)
+    r = lambda *n: torch.randn(n, generator=g, device="cuda").to(dtype)
+    k, v, q = r(n_pages, G, 64, dim), r(n_pages, G, dim, 64), r(sum(new), H, dim)
+    mask = pc.tree_masks(new, 7)
+    for m in (None, mask):
+        args = (k, v, table.cuda(), start.cuda(), cx.cuda())
+        got = ops.attn_packed(q, *args) if m is None else ops.attn_tree(q, m.cuda(), *args)
+        want, far = pc.attention(q, k, v, table, start, cx, dim ** -0.5, m)
+        assert ((got.double() - want).abs() <= far).all()
