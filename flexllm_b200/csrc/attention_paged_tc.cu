@@ -207,6 +207,7 @@ __global__ void __launch_bounds__(MODE == kOne ? 192 : 320, MODE == kOne ? 2 : 1
         const uint32_t lane_addr = (uint32_t)((warp & 3) * 32) << 16;
         const int i = i0 + q * t.TQ + row / t.RC, hr = row % t.RC;
         const bool live = row < t.TQ * t.RC && i < s.n && hr < heads;
+        const bool busy = __any_sync(0xffffffffu, live);                                  // other warps' rows are nowhere read
         const int sure = live ? sure_keys(a, s, i) : 0x40000000;                          // rows of the tile without a token mask nothing
         const unsigned long long bits = live ? mask_bits(a, s, i) : 0ull;
         const uint32_t tO = tmem + W * KT + w * t.o_stride + lane_addr;
@@ -221,6 +222,9 @@ __global__ void __launch_bounds__(MODE == kOne ? 192 : 320, MODE == kOne ? 2 : 1
             if (!wait_bar(bar_s + 8 * w, (uint32_t)(turn & 1))) { ok = false; break; }
             tc_fence_after();
             const uint32_t tS = tmem + w * KT + lane_addr;
+            if (!busy) {
+                if (lane == 0) mbar_arrive(bar_h + 8 * w);
+            } else {
             uint32_t v[4][32];
 #pragma unroll
             for (int c = 0; c < 4; c++) tmem_ld_32x32(tS + 32 * c, v[c]);
@@ -281,6 +285,7 @@ __global__ void __launch_bounds__(MODE == kOne ? 192 : 320, MODE == kOne ? 2 : 1
                     __syncwarp();
                     if (lane == 0) mbar_arrive(bar_h + 8 * w);
                 }
+            }
             }
             if (left < KT) {                              // the sequence ends inside the tile: zeros for the values behind its end
                 const int sv = n % t.vs, c0 = left >> 3;
