@@ -26,6 +26,7 @@ constexpr int KT = 128;                    // keys per tile
 struct TcArgs {
     PagedAttn a;
     int RC, HC, TQ, heads;                 // heads per tile, head chunks per group, tokens per tile, head chunks
+    uint32_t q_block;                      // bytes of a 128-byte block of the rows of Q. The products take 128 rows, so those of a short tile read on into K
     int kc, vr;                            // 128-byte blocks of a Q or K row, rows of a V^T tile (dv rounded up to 16)
     int ks, vs;                            // stages of K and V
     float a2;                              // scale * log2 e
@@ -39,9 +40,9 @@ struct Ring {
     __device__ __forceinline__ void next() { if (++st == n) { st = 0; ph ^= 1u; } }
 };
 struct TcSmem { uint32_t k, v, bars, total; };
-__host__ __device__ inline TcSmem tc_smem(int NQ, int kc, int vr, int ks, int vs) {
+__host__ __device__ inline TcSmem tc_smem(int NQ, uint32_t q_block, int kc, int vr, int ks, int vs) {
     TcSmem o;
-    o.k = (uint32_t)(NQ * kc) * 16384u;
+    o.k = (uint32_t)(NQ * kc) * q_block;
     o.v = o.k + (uint32_t)(ks * kc) * 16384u;
     o.bars = o.v + (uint32_t)(vs * vr) * 256u;
     o.total = o.bars + 256u + 1024u;
@@ -64,7 +65,7 @@ __global__ void __launch_bounds__(MODE == kOne ? 192 : 320, MODE == kOne ? 2 : 1
     const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
     uint8_t* base_ptr = smem_raw + (base - raw);
     const PagedAttn& a = t.a;
-    const TcSmem o = tc_smem(NQ, t.kc, t.vr, t.ks, t.vs);
+    const TcSmem o = tc_smem(NQ, t.q_block, t.kc, t.vr, t.ks, t.vs);
     uint64_t* bars = reinterpret_cast<uint64_t*>(base_ptr + o.bars);
     const uint32_t bar_q = smem_u32(bars), bar_kf = bar_q + 8, bar_ke = bar_kf + 8 * kMaxStages, bar_vf = bar_ke + 8 * kMaxStages,
                    bar_ve = bar_vf + 8 * kMaxStages, bar_s = bar_ve + 8 * kMaxStages, bar_p = bar_s + 16, bar_o = bar_p + 16, bar_f = bar_o + 16, bar_h = bar_f + 16;
@@ -117,7 +118,7 @@ __global__ void __launch_bounds__(MODE == kOne ? 192 : 320, MODE == kOne ? 2 : 1
         if (lane == 0 && t0 < t_last) {
             mbar_expect_tx(bar_q, (uint32_t)(NQ * t.kc * t.TQ * t.RC) * 128u);
             for (int q = 0; q < NQ; q++)
-                for (int i = 0; i < t.kc; i++) tma_load_3d(base + (uint32_t)(q * t.kc + i) * 16384u, &tmapQ, bar_q, i * 128, h0, s.row0 + i0 + q * t.TQ);
+                for (int i = 0; i < t.kc; i++) tma_load_3d(base + (uint32_t)(q * t.kc + i) * t.q_block, &tmapQ, bar_q, i * 128, h0, s.row0 + i0 + q * t.TQ);
         }
         const int n_pg = (end + kPage - 1) / kPage;
         int ids = 0;
@@ -162,12 +163,12 @@ __global__ void __launch_bounds__(MODE == kOne ? 192 : 320, MODE == kOne ? 2 : 1
             const int q = NQ == 2 ? w : 0;
             if (!wait(bar_kf + 8 * r.st, r.ph)) return false;
             tc_fence_after();
-            const uint32_t a_at = q_lo + (uint32_t)(q * t.kc) * 1024u, b_at = k_lo + (uint32_t)(r.st * t.kc) * 1024u, d_at = u_tmem + w * KT;
+            const uint32_t q_step = t.q_block >> 4, a_at = q_lo + (uint32_t)(q * t.kc) * q_step, b_at = k_lo + (uint32_t)(r.st * t.kc) * 1024u, d_at = u_tmem + w * KT;
             for (int blk = 0; blk < ksteps >> 2; blk++)
 #pragma unroll
-                for (uint32_t k = 0; k < 4; k++) umma_bf16_lo(leader, d_at, a_at + blk * 1024u + 2 * k, b_at + blk * 1024u + 2 * k, idesc_qk, blk + k > 0);
+                for (uint32_t k = 0; k < 4; k++) umma_bf16_lo(leader, d_at, a_at + blk * q_step + 2 * k, b_at + blk * 1024u + 2 * k, idesc_qk, blk + k > 0);
             for (int k = ksteps & ~3; k < ksteps; k++)
-                umma_bf16_lo(leader, d_at, a_at + (k >> 2) * 1024u + 2 * (k & 3), b_at + (k >> 2) * 1024u + 2 * (k & 3), idesc_qk, k > 0);
+                umma_bf16_lo(leader, d_at, a_at + (k >> 2) * q_step + 2 * (k & 3), b_at + (k >> 2) * 1024u + 2 * (k & 3), idesc_qk, k > 0);
             umma_commit_by(leader, bar_s + 8 * w);
             if (q == NQ - 1 || j >= u1[NQ - 1]) umma_commit_by(leader, bar_ke + 8 * r.st);      // the last product with K_j
             return true;
@@ -248,7 +249,7 @@ __global__ void __launch_bounds__(MODE == kOne ? 192 : 320, MODE == kOne ? 2 : 1
                 for (int x = 2; x < 32; x += 2) mx[c] = max3(mx[c], __uint_as_float(v[c][x]), __uint_as_float(v[c][x + 1]));
             }
             const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * t.a2;
-            const bool grow = top > m + kSlack;
+            const bool grow = live && top > m + kSlack;
             if (__any_sync(0xffffffffu, grow)) {
                 const float m_new = grow ? top : m, al = ex2_fast(m - m_new);
                 m = m_new;
@@ -388,15 +389,15 @@ template <int MODE> int launch_tc(TcArgs& t, long tiles, cudaStream_t st) {
     const PagedAttn& a = t.a;
     constexpr int NQ = MODE == kPair ? 2 : 1, W = MODE == kOne ? 1 : 2, NT = W * 128 + 64;
     // stages while they fit, of K and V in turn; kOne: two CTAs per SM where that is possible
-    const bool two = MODE == kOne && KT + t.o_stride <= 256 && tc_smem(1, t.kc, t.vr, 1, 1).total <= kHalfSm;
+    const bool two = MODE == kOne && KT + t.o_stride <= 256 && tc_smem(1, t.q_block, t.kc, t.vr, 1, 1).total <= kHalfSm;
     t.tmem_cols = two ? 256 : 512;
     t.ks = t.vs = 1;
     for (int i = 0; i < 2 * (kMaxStages - 1); i++) {
         int& n = i & 1 ? t.vs : t.ks;
         n++;
-        if (tc_smem(NQ, t.kc, t.vr, t.ks, t.vs).total > (two ? kHalfSm : kWholeSm)) { n--; break; }
+        if (tc_smem(NQ, t.q_block, t.kc, t.vr, t.ks, t.vs).total > (two ? kHalfSm : kWholeSm)) { n--; break; }
     }
-    TcSmem o = tc_smem(NQ, t.kc, t.vr, t.ks, t.vs);
+    TcSmem o = tc_smem(NQ, t.q_block, t.kc, t.vr, t.ks, t.vs);
     // the parts of a tile go over the operands, not over the barriers
     const uint32_t parts = MODE == kTurns || t.n_split > 1 ? (uint32_t)(W * 128 * (a.dv + 4) * 4) : 0;
     if (o.total > kWholeSm || parts > o.bars) return FLEXLLM_ENOTSUP;
@@ -442,15 +443,20 @@ int attn_paged_tc(const PagedAttn& a, cudaStream_t st) {
     TcArgs t = {};
     const int R = a.H / a.G;
     t.a = a;
-    t.RC = R < 128 ? R : 128; t.HC = (R + t.RC - 1) / t.RC; t.TQ = 128 / t.RC;
+    t.RC = R < 128 ? R : 128; t.HC = (R + t.RC - 1) / t.RC;
     t.kc = (a.dk + 63) / 64; t.vr = (a.dv + 15) / 16 * 16; t.o_stride = (t.vr + 31) / 32 * 32;
     t.a2 = a.scale * kLog2e;
     if (t.a2 < 1e-30f) t.a2 = 1e-30f;                     // scale 0: weights all alike, and no infinity times zero
-    const long heads = (long)a.G * t.HC, seqs = a.seq.B < a.seq.T ? a.seq.B : a.seq.T;
+    const long heads = (long)a.G * t.HC, seqs = a.seq.B < a.seq.T ? a.seq.B : a.seq.T, each = (a.seq.T + seqs - 1) / seqs;
+    // short tiles where two of them would hold what sequences have on average: shared memory for Q becomes stages (one token over 100000, 8 key/value
+    // heads: 105 us and 81)
+    const int most = each * t.RC <= 16 ? 32 : 128;
+    t.TQ = most / t.RC;
+    t.q_block = most * 128u;
     const long pairs = most_units(a.seq, 2 * t.TQ), ones = most_units(a.seq, t.TQ);
     t.heads = (int)heads;
     if (ones * 16 * heads > 0x7fffffffL) return FLEXLLM_ENOTSUP;
-    const long sms = gemm_sm_count(), tiles = ((a.seq.T + seqs - 1) / seqs + t.TQ - 1) / t.TQ * seqs * heads;      // if all sequences are of equal length
+    const long sms = gemm_sm_count(), tiles = (each + t.TQ - 1) / t.TQ * seqs * heads;      // if all sequences are of equal length
     const int pages = (a.seq.max_ctx + kPage) / kPage;
     t.n_split = 1;
     if (a.dk <= 128 && a.dv <= 128) {
@@ -458,15 +464,15 @@ int attn_paged_tc(const PagedAttn& a, cudaStream_t st) {
             // What the call takes in microseconds, cut into s parts, by one CTA of kTurns or two of kOne per SM: a time per key tile, one for the call, and
             // one per part for joining rows (a tree of 26 over 1000, kTurns and kOne: 17.6 and 15.2; 16 of 31 over 8000: 103 and 89; 9 of 10
             // over 4000: 34 and 44; one token over 100000: 62 and 157)
-            const float rows = (float)((a.seq.T + seqs - 1) / seqs < t.TQ ? (a.seq.T + seqs - 1) / seqs * t.RC : 128) / 128;
+            const float rows = (float)((each < t.TQ ? each : t.TQ) * t.RC) / 128;
             const int n = (pages + 1) / 2;
             float best = 3e38f;
             bool turns = true;
             for (int s = 1; s <= 16 && s <= n; s++) {
-                const float each = (float)((n + s - 1) / s);
+                const float part = (float)((n + s - 1) / s);
                 const int alone = cluster_slots(s, false);
-                const float two_sets = 1.1f * each + 11.0f + 1.6f * s * rows;
-                const float one_set = (alone >= tiles ? 1.85f * each + 8.0f : 2.1f * each + 9.0f) + (s > 1 ? 2.5f + 0.8f * s * rows : 0.0f);
+                const float two_sets = 1.1f * part + 11.0f + 1.6f * s * rows;
+                const float one_set = (alone >= tiles ? 1.85f * part + 8.0f : 2.1f * part + 9.0f) + (s > 1 ? 2.5f + 0.8f * s * rows : 0.0f);
                 if (two_sets < best && alone >= tiles) { best = two_sets; turns = true; t.n_split = s; }
                 if (one_set < best && cluster_slots(s, true) >= tiles) { best = one_set; turns = false; t.n_split = s; }
             }
