@@ -2,11 +2,12 @@
 //   y[m][n] = sum_groups s[n][g] * sum_{k in g} a[m][k] (q[n][k] - z[n][g])
 // Weights are on the 128-row side, up to 64 tokens on the other. A CTA walks K in steps of 128:
 //   warp 12        brings words (eight steps ahead) and activations by TMA
-//   warps 4 .. 11  put q - z, exact in bf16, into swizzled shared memory. They load nothing from memory themselves: their fence towards the
+//   warps 4 .. 11  put q - z, exact in bf16, into swizzled shared memory, four of them a step, the others the next (all eight a step: 13.2 us for 48 tokens,
+//                  16384 x 2048; by fours 11.7; three teams of four leave too few registers for the sums: 12.9). They load nothing from memory themselves: their fence towards the
 //                  tensor core would wait for it (words in registers, asked for four steps ahead: 18.8 us for 48 x 16384 x 2048)
 //   warp 13        issues the MMAs, accumulators of their own for each group of a step, two steps' worth
 //   warps 0 .. 3   take a step's sums out of TMEM and add them up in fp32 registers, times the groups' scales: no weight is ever rounded;
-//                  they also hand the zero points to the converting warps
+//                  they also hand the zero points to the converting warps, six steps ahead
 // Few rows: the CTAs of a cluster cut K, and their sums meet in shared memory, in a fixed order.
 // Bound by the chain of a step: one thread's waits and eight MMAs, beside it the conversion, about two instructions for half a byte.
 #include "linear_w4.h"
@@ -18,7 +19,8 @@ using namespace tc;
 
 namespace {
 
-constexpr int kStepK = 128, kStages = 3, kWords = 8, kTcThreads = 448;
+constexpr int kStepK = 128, kStages = 3, kWords = 8, kTeams = 2, kTmaWarp = 4 + 4 * kTeams, kMmaWarp = kTmaWarp + 1, kTcThreads = (kMmaWarp + 1) * 32;
+constexpr int kZeros = 8, kZerosAhead = 6;      // zero points: slots, steps ahead of the sums
 
 struct W4Tc {
     W4Call c;
@@ -26,11 +28,11 @@ struct W4Tc {
     int* error_flag;
     int per_group; uint32_t magic;         // blocks of a group, and 2^32 / per_group rounded up: the quotient of block numbers below 2^16
 };
-// shared memory: A [stage][2][128 rows][128 bytes], activations [stage][2][NT][128 bytes], words [kWords][128 rows][64 bytes], zero points [stage][4][128]
+// shared memory: A [stage][2][128 rows][128 bytes], activations [stage][2][NT][128 bytes], words [kWords][128 rows][64 bytes], zero points [kZeros][4][128]
 constexpr uint32_t kXAt = kStages * 32768u;
 template <int NT> constexpr uint32_t kWAt = kXAt + kStages * NT * 256u;
 template <int NT> constexpr uint32_t kZAt = kWAt<NT> + kWords * 8192u;
-template <int NT> constexpr uint32_t kBarsAt = kZAt<NT> + kStages * 512u;
+template <int NT> constexpr uint32_t kBarsAt = kZAt<NT> + kZeros * 512u;
 template <int NT> constexpr uint32_t kTcSmem = kBarsAt<NT> + 512u + 1024u;
 
 // U groups (or parts of one) per step
@@ -51,14 +53,15 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_w4_tc_kernel(const __gri
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     constexpr uint32_t need = 2 * U * NT, cols = need <= 32 ? 32 : need <= 64 ? 64 : need <= 128 ? 128 : need <= 256 ? 256 : 512;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < kStages; i++) { mbar_init(bar_a + 8 * i, 9); mbar_init(bar_e + 8 * i, 1); mbar_init(bar_z + 8 * i, 4); }
+        for (int i = 0; i < kStages; i++) { mbar_init(bar_a + 8 * i, 5); mbar_init(bar_e + 8 * i, 1); }
         for (int i = 0; i < 2; i++) { mbar_init(bar_d + 8 * i, 1); mbar_init(bar_de + 8 * i, 4); }
         for (int i = 0; i < kWords; i++) mbar_init(bar_w + 8 * i, 1);
+        for (int i = 0; i < kZeros; i++) mbar_init(bar_z + 8 * i, 4);
         *abort_flag = 0;
         fence_barrier_init();
     }
-    if (warp == 13) { tmem_alloc(smem_u32(tmem_slot), cols); tmem_relinquish(); }
-    if (warp == 12 && lane == 0) { tma_prefetch_desc(&tmapX); tma_prefetch_desc(&tmapW); }
+    if (warp == kMmaWarp) { tmem_alloc(smem_u32(tmem_slot), cols); tmem_relinquish(); }
+    if (warp == kTmaWarp && lane == 0) { tma_prefetch_desc(&tmapX); tma_prefetch_desc(&tmapW); }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -71,7 +74,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_w4_tc_kernel(const __gri
     float acc[NT];
 #pragma unroll
     for (int x = 0; x < NT; x++) acc[x] = 0.0f;
-    if (warp == 12) {
+    if (warp == kTmaWarp) {
         if (lane == 0) {
             // the words of step n lie where those of step n - kWords were, which the conversion has read when the products of that step are done
             auto words = [&](int n) {
@@ -89,7 +92,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_w4_tc_kernel(const __gri
                 if (n >= kStages) words(n - kStages + kWords);
             }
         }
-    } else if (warp == 13) {
+    } else if (warp == kMmaWarp) {
         const uint32_t leader = elect_leader(), u_tmem = (uint32_t)uniform_max((int)tmem);
         const uint32_t idesc = umma_idesc_bf16(128, NT), a_lo = umma_desc_lo(base), x_lo = umma_desc_lo(base + kXAt);
         for (int n = 0; s0 + n < s1; n++) {
@@ -105,31 +108,32 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_w4_tc_kernel(const __gri
             umma_commit_by(leader, bar_e + 8 * st);
         }
     } else if (warp >= 4) {
-        // lane: bits 0 - 2 and 4 the row, bit 3 the half of the step, so that eight lanes in a row meet eight different 16-byte columns
-        const int h = lane >> 3 & 1, r = (warp - 4) * 16 + (lane & 7) + (lane >> 4) * 8;
-        uint8_t* to = base_ptr + h * 16384 + r * 128;
-        for (int n = 0; s0 + n < s1; n++) {
+        // a row per lane: eight lanes in a row meet eight different 16-byte columns, in the words as in the operand
+        const int r = (warp & 3) * 32 + lane;
+        for (int n = (warp - 4) >> 2; s0 + n < s1; n += kTeams) {
             const int st = n % kStages, sw = n % kWords;
+            uint8_t* to = base_ptr + st * 32768 + r * 128;
             if (!wait_warp(bar_w + 8 * sw, (uint32_t)(n / kWords & 1))) break;
-            uint4 v[2];
+            uint4 v[4];
 #pragma unroll
-            for (int x = 0; x < 2; x++) v[x] = *reinterpret_cast<const uint4*>(base_ptr + kWAt<NT> + sw * 8192 + r * 64 + (((h * 2 + x) ^ (r >> 1 & 3)) << 4));
+            for (int x = 0; x < 4; x++) v[x] = *reinterpret_cast<const uint4*>(base_ptr + kWAt<NT> + sw * 8192 + r * 64 + ((x ^ (r >> 1 & 3)) << 4));
             if (!wait_warp(bar_e + 8 * st, (uint32_t)(n / kStages & 1) ^ 1u)) break;
-            uint32_t z[2] = {8u, 8u};
+            uint32_t z2[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) z2[u] = zero2(8u);
             if (c.zero) {
-                if (!wait_warp(bar_z + 8 * st, (uint32_t)(n / kStages & 1))) break;
-                const uint8_t* zs = base_ptr + kZAt<NT> + st * 512 + r;
-                z[0] = zs[h * U / 2 * 128];
-                z[1] = U == 4 ? zs[(h * 2 + 1) * 128] : z[0];
+                if (!wait_warp(bar_z + 8 * (n % kZeros), (uint32_t)(n / kZeros & 1))) break;
+#pragma unroll
+                for (int u = 0; u < U; u++) z2[u] = zero2(base_ptr[kZAt<NT> + n % kZeros * 512 + u * 128 + r]);
             }
 #pragma unroll
-            for (int x = 0; x < 2; x++) {
-                const uint32_t z2 = zero2(z[x]);
+            for (int x = 0; x < 4; x++) {
+                const uint32_t z = z2[x * U / 4];
                 const uint32_t word[4] = {v[x].x, v[x].y, v[x].z, v[x].w};
 #pragma unroll
                 for (int y = 0; y < 4; y++) {
-                    const uint32_t p0 = weights2(word[y], 0, z2), p1 = weights2(word[y], 1, z2), p2 = weights2(word[y], 2, z2), p3 = weights2(word[y], 3, z2);
-                    *reinterpret_cast<uint4*>(to + st * 32768 + (((x * 4 + y) ^ (r & 7)) << 4)) =
+                    const uint32_t p0 = weights2(word[y], 0, z), p1 = weights2(word[y], 1, z), p2 = weights2(word[y], 2, z), p3 = weights2(word[y], 3, z);
+                    *reinterpret_cast<uint4*>(to + (x >> 1) * 16384 + ((((x & 1) * 4 + y) ^ (r & 7)) << 4)) =
                         make_uint4(pick(p0, p1, 0x5410), pick(p2, p3, 0x5410), pick(p0, p1, 0x7632), pick(p2, p3, 0x7632));
                 }
             }
@@ -145,30 +149,34 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_w4_tc_kernel(const __gri
             const int kb = min(i * U + u, c.K / BK - 1);
             return g0 + (t.per_group == 1 ? kb : (int)__umulhi(kb, t.magic));
         };
-        uint32_t next[U], zero[U];
+        uint32_t next[U];
         auto fetch = [&](int i) {
 #pragma unroll
             for (int u = 0; u < U; u++) next[u] = c.scale_f32 ? ((const uint32_t*)c.scale)[group_at(i, u)] : (uint32_t)((const uint16_t*)c.scale)[group_at(i, u)];
         };
-        auto fetch_zero = [&](int i) {
+        // zero points of step n into a slot that the conversion of step n - kZeros has left: its products are among the sums
+        struct Zeros { uint32_t v[U]; } zero;
+        auto fetch_zero = [&](int n) {
+            Zeros z;
 #pragma unroll
-            for (int u = 0; u < U; u++) zero[u] = c.zero[group_at(i, u)];
+            for (int u = 0; u < U; u++) z.v[u] = c.zero[group_at(s0 + n, u)];
+            return z;
         };
-        // zero points of step n, asked for a step ahead, into its slot, which the conversion of step n - kStages has left
-        auto hand_zero = [&](int n) {
-            if (!wait_warp(bar_e + 8 * (n % kStages), (uint32_t)(n / kStages & 1) ^ 1u)) return false;
+        auto hand_zero = [&](int n, const Zeros& z) {
 #pragma unroll
-            for (int u = 0; u < U; u++) base_ptr[kZAt<NT> + n % kStages * 512 + u * 128 + rr] = (uint8_t)zero[u];
-            fetch_zero(s0 + n + 1);
+            for (int u = 0; u < U; u++) base_ptr[kZAt<NT> + n % kZeros * 512 + u * 128 + rr] = (uint8_t)z.v[u];
             __syncwarp();
-            if (lane == 0) mbar_arrive(bar_z + 8 * (n % kStages));
-            return true;
+            if (lane == 0) mbar_arrive(bar_z + 8 * (n % kZeros));
         };
         bool ok = s0 < s1;
         if (ok) fetch(s0);
         if (ok && c.zero) {
-            fetch_zero(s0);
-            for (int n = 0; ok && n < 2 && s0 + n < s1; n++) ok = hand_zero(n);
+            Zeros first[kZerosAhead];
+#pragma unroll
+            for (int n = 0; n < kZerosAhead; n++) first[n] = fetch_zero(n);
+#pragma unroll
+            for (int n = 0; n < kZerosAhead; n++) if (s0 + n < s1) hand_zero(n, first[n]);
+            zero = fetch_zero(kZerosAhead);
         }
         for (int n = 0; ok && s0 + n < s1; n++) {
             float sc[U];
@@ -189,7 +197,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_w4_tc_kernel(const __gri
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(bar_de + 8 * (n & 1));
-            if (c.zero && s0 + n + 2 < s1) ok = hand_zero(n + 2);
+            if (c.zero && s0 + n + kZerosAhead < s1) {
+                hand_zero(n + kZerosAhead, zero);
+                zero = fetch_zero(n + kZerosAhead + 1);
+            }
         }
     }
     // the sums into shared memory (every product has been waited for), [token][132]; the CTAs of the cluster join the tokens in turn
@@ -236,7 +247,7 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_w4_tc_kernel(const __gri
         if (threadIdx.x == 0 && t.error_flag) atomicOr(t.error_flag, 1);
         __syncthreads();
     }
-    if (warp == 13) { tc_fence_after(); tmem_dealloc(tmem, cols); }
+    if (warp == kMmaWarp) { tc_fence_after(); tmem_dealloc(tmem, cols); }
 }
 
 template <int NT, int U> int launch_tc(W4Tc& t, cudaStream_t st) {
