@@ -67,10 +67,6 @@ template <class T> __device__ __noinline__ void attn_row_by_key(const PagedAttn&
 __device__ __forceinline__ bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 __device__ __forceinline__ bool not_finite(float v) { return !(fabsf(v) <= 3.402823466e38f); }
 
-// Clusters of `size` CTAs, up to 16, that the device runs at once where an SM takes one CTA, or two of them. Fewer than the SMs would do, since a cluster
-// stays within a part of the device: of 148 SMs (one CTA each) 33 clusters of 4, 22 of 6, 15 of 8, 7 of 16.
-int cluster_slots(int size, bool two);
-
 // CTAs of a cluster among which a tile's keys are cut, for `tiles` (tile, head) pairs of up to `pages` key pages each: as many as all run at once
 // while each part keeps `least` pages, and 16 in clusters of more than 8.
 inline int key_splits(long tiles, bool two, int pages, int least, int most) {

@@ -208,4 +208,11 @@ void attn_layout(AttnShape* s, bool gate, bool own_kv = true);
 void attn_bias_table(const AttnShape& s, const float* table, int rows, int bias_max, float* out);
 inline size_t attn_bias_floats(const AttnShape& s) { return (size_t)s.H * (2 * kBiasPad + s.window); }
 
+// Clusters of `size` CTAs, up to 16, that the device runs at once where an SM takes one CTA, or two of them. Fewer than the SMs would do, since a cluster
+// stays within a part of the device: of 148 SMs (one CTA each) 33 clusters of 4, 22 of 6, 15 of 8, 7 of 16. Beyond 8 a kernel has to ask for it.
+int cluster_slots(int size, bool two);
+template <class K> inline int allow_cluster(K kern, int size) {
+    return size <= 8 ? FLEXLLM_OK : cuda_status(cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+}
+
 }  // namespace flexllm

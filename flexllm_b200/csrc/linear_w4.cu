@@ -362,7 +362,9 @@ extern "C" int flexllm_linear_w4(int dtype, const void* a, long lda, const uint8
                     aligned(y, y_f32 || dtype == FLEXLLM_F32 ? 4 : 2));
     const W4Call c = {a, lda, w, scale, scale_dtype == FLEXLLM_F32, zero, group, bias, M, N, K, y, ldy, y_f32 != 0};
     const SetUpEarly early;
-    if (dtype == FLEXLLM_BF16 && M > 8) return linear_w4_tc(c, (cudaStream_t)stream);
+    // the tensor cores for more than 8 tokens (16 x 8192 x 2048: 9.1 us), and for more than 2 where K is long and one wave has all rows: each CTA there has a
+    // part of K (4 x 2048 x 8192: 10.6 us against 13.6; 8 x 8192 x 8192: 21.2 against 26.6; 8 x 128256 x 2048: 79 against 49)
+    if (dtype == FLEXLLM_BF16 && (M > 8 || (M > 2 && K >= 4096 && N <= 128L * gemm_sm_count()))) return linear_w4_tc(c, (cudaStream_t)stream);
     W4Args p = {};
     static_cast<W4Call&>(p) = c;
     return dtype == FLEXLLM_BF16 ? pick_w4<bf16>(p, (cudaStream_t)stream) : pick_w4<float>(p, (cudaStream_t)stream);

@@ -255,14 +255,16 @@ template <int NT, int U> int launch_tc(W4Tc& t, cudaStream_t st) {
     t.steps = (c.K + kStepK - 1) / kStepK;
     t.per_group = c.group / (kStepK / U);
     t.magic = (uint32_t)(((1ull << 32) + t.per_group - 1) / t.per_group);
-    const long tiles = (c.N + 127) / 128, sms = gemm_sm_count();
+    const long tiles = (c.N + 127) / 128;
     t.n_split = 1;
-    while (t.n_split < 8 && tiles * t.n_split * 2 <= sms && t.steps >= 4 * t.n_split) t.n_split *= 2;
+    for (int k = 2; k <= 16 && t.steps >= k * (k > 8 ? 4 : 2); k++)
+        if (cluster_slots(k, false) >= tiles * ((c.M + 63) / 64)) t.n_split = k;
     CUtensorMap tx, tw;
     TRY_RC(make_tmap_2d_u8_ld(&tx, c.a, (uint64_t)c.M, (uint64_t)c.K * 2, NT, (uint64_t)c.lda * 2));
     TRY_RC(make_tmap_2d_u8_box(&tw, c.w, (uint64_t)c.N, (uint64_t)c.K / 2, 64, 128, 64));
     auto kern = linear_w4_tc_kernel<NT, U>;
     TRY_RC(allow_shared(kern, kTcSmem<NT>));
+    TRY_RC(allow_cluster(kern, t.n_split));
     launch_cluster(kern, dim3((unsigned)(tiles * t.n_split), (c.M + 63) / 64), dim3(kTcThreads), t.n_split, kTcSmem<NT>, st, tx, tw, t);
     return launch_status();
 }
