@@ -205,20 +205,23 @@ template <class T> int run_rope(RopeArgs& a, cudaStream_t st) {
     return launch_rope<T, 32>(a, st);
 }
 
-// new[ctx + i] = old[ctx + keep[i]], i < count: one CTA per (sequence, key/value head, layer). All old entries are in shared memory before the
-// first new one is written, so the indices may come in any order. Latency bound: a few KB per CTA; entries that stay are not touched.
+// new[ctx + i] = old[ctx + keep[i]], i < count: one CTA per (sequence, key/value head, several layers of like shape, where there are enough CTAs). All old
+// entries are in shared memory before the first new one is written, so the indices may come in any order. Bound by latency (counts, indices, page
+// table, entries, one after the other) and by the sectors of V^T: an element of two bytes is read and written with its 32.
 struct KeepLayer { void *k, *v; int hkv, dk, dv, n_pages; };
 constexpr int kKeepLayers = 64;
 struct KeepArgs {
     PackedSeqs seq;                        // cu unused
     const int32_t *keep, *count;
-    int most;
+    int most, layers, per;                 // per: layers of a CTA
     KeepLayer layer[kKeepLayers];
 };
+
 template <class T> __global__ void __launch_bounds__(256) kv_keep_kernel(const __grid_constant__ KeepArgs a) {
     extern __shared__ __align__(16) uint8_t raw[];
     __shared__ int src_page[64], src_slot[64], dst_page[64], dst_slot[64], n_moves;
-    const KeepLayer& y = a.layer[blockIdx.z];
+    const int l0 = blockIdx.z * a.per, layers = min(a.per, a.layers - l0);
+    const KeepLayer& y = a.layer[l0];      // the shape of all of them
     const int b = blockIdx.x, g = blockIdx.y, tid = threadIdx.x;
     pdl_sync();
     if (g >= y.hkv) return;
@@ -240,35 +243,47 @@ template <class T> __global__ void __launch_bounds__(256) kv_keep_kernel(const _
     }
     __syncthreads();
     const int n = n_moves;
-    T* ks = reinterpret_cast<T*>(raw);                    // [n][dk]
-    T* vs = ks + (long)n * y.dk;                          // [dv][n]
-    auto k_at = [&](int page, int slot) { return (T*)y.k + (((long)page * y.hkv + g) * kPage + slot) * y.dk; };
-    auto v_at = [&](int page, int slot) { return (T*)y.v + ((long)page * y.hkv + g) * y.dv * kPage + slot; };
-    const int vec = y.dk * (int)sizeof(T) / 16;
-    for (int e = tid; e < n * vec; e += 256) {
-        const int i = e / vec, c = e % vec;
-        reinterpret_cast<uint4*>(ks + (long)i * y.dk)[c] = reinterpret_cast<const uint4*>(k_at(src_page[i], src_slot[i]))[c];
-    }
-    for (int e = tid; e < n * y.dv; e += 256) {
-        const int d = e / n, i = e - d * n;
-        vs[e] = v_at(src_page[i], src_slot[i])[(long)d * kPage];
+    if (n == 0) return;
+    const int vec = y.dk * (int)sizeof(T) / 16, kn = n * vec, vn = n * y.dv;
+    T* ks = reinterpret_cast<T*>(raw);                    // [layer][n][dk]
+    T* vs = ks + (long)layers * n * y.dk;                 // [layer][dv][n]
+    // quotients of numbers below 2^17 by numbers below 2^15 (1 apart), as they are needed for every element
+    struct Quotient {
+        uint32_t by, magic;
+        __device__ Quotient(int d) : by(d), magic(d > 1 ? 0xffffffffu / (uint32_t)d + 1u : 0u) {}
+        __device__ __forceinline__ uint32_t operator()(uint32_t x) const { return by > 1 ? __umulhi(x, magic) : x; }
+    };
+    const Quotient by_kn(kn), by_vec(vec), by_vn(vn), by_n(n);
+    auto k_at = [&](uint32_t e, const int* page, const int* slot) {
+        const uint32_t l = by_kn(e), r = e - l * kn, i = by_vec(r), c = r - i * vec;
+        return reinterpret_cast<uint4*>((T*)a.layer[l0 + l].k + (((long)page[i] * y.hkv + g) * kPage + slot[i]) * y.dk) + c;
+    };
+    auto v_at = [&](uint32_t e, const int* page, const int* slot) {
+        const uint32_t l = by_vn(e), r = e - l * vn, d = by_n(r), i = r - d * n;
+        return (T*)a.layer[l0 + l].v + ((long)page[i] * y.hkv + g) * y.dv * kPage + (long)d * kPage + slot[i];
+    };
+    for (int e = tid; e < layers * kn; e += 256) reinterpret_cast<uint4*>(ks)[e] = *k_at(e, src_page, src_slot);
+    for (int e0 = tid; e0 < layers * vn; e0 += 8 * 256) {      // eight loads under way
+        T x[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) if (e0 + j * 256 < layers * vn) x[j] = *v_at(e0 + j * 256, src_page, src_slot);
+#pragma unroll
+        for (int j = 0; j < 8; j++) if (e0 + j * 256 < layers * vn) vs[e0 + j * 256] = x[j];
     }
     __syncthreads();
-    for (int e = tid; e < n * vec; e += 256) {
-        const int i = e / vec, c = e % vec;
-        reinterpret_cast<uint4*>(k_at(dst_page[i], dst_slot[i]))[c] = reinterpret_cast<const uint4*>(ks + (long)i * y.dk)[c];
-    }
-    for (int e = tid; e < n * y.dv; e += 256) {
-        const int d = e / n, i = e - d * n;
-        v_at(dst_page[i], dst_slot[i])[(long)d * kPage] = vs[e];
-    }
+    for (int e = tid; e < layers * kn; e += 256) *k_at(e, dst_page, dst_slot) = reinterpret_cast<const uint4*>(ks)[e];
+    for (int e = tid; e < layers * vn; e += 256) *v_at(e, dst_page, dst_slot) = vs[e];
 }
 
-template <class T> int run_keep(const KeepArgs& a, int layers, int heads, int widest, cudaStream_t st) {
-    const size_t smem = (size_t)a.most * widest * sizeof(T);
+template <class T> int run_keep(KeepArgs& a, int heads, int widest, bool alike, cudaStream_t st) {
+    // several layers per CTA, up to 4, while every SM has its eight CTAs (48 sequences, 8 heads, 16 layers: 20.1 us with one, 16.2 with 4)
+    const long all = (long)a.seq.B * heads * a.layers, room = 8L * gemm_sm_count();
+    a.per = 1;
+    while (alike && a.per < 4 && all >= 2 * a.per * room && 2 * a.per * a.most * widest * (int)sizeof(T) <= 24 * 1024) a.per *= 2;
+    const size_t smem = (size_t)a.per * a.most * widest * sizeof(T);
     auto kern = kv_keep_kernel<T>;
     TRY_RC(allow_shared(kern, smem));
-    launch_k(kern, dim3(a.seq.B, heads, layers), dim3(256), smem, st, a);
+    launch_k(kern, dim3(a.seq.B, heads, (a.layers + a.per - 1) / a.per), dim3(256), smem, st, a);
     return launch_status();
 }
 
@@ -333,15 +348,18 @@ extern "C" int flexllm_kv_keep(int dtype, const flexllm_kv_pages* layers_host, i
         const int n = layers - l0 < kKeepLayers ? layers - l0 : kKeepLayers;
         KeepArgs a = {};
         a.seq = seq;
-        a.keep = keep; a.count = count; a.most = most;
+        a.keep = keep; a.count = count; a.most = most; a.layers = n;
         int heads = 0, widest = 0;
+        bool alike = true;
         for (int i = 0; i < n; i++) {
             const flexllm_kv_pages& p = layers_host[l0 + i];
+            const flexllm_kv_pages& o = layers_host[l0];
             a.layer[i] = {p.k, p.v, p.hkv, p.kdim, p.vdim, p.n_pages};
+            alike = alike && p.hkv == o.hkv && p.kdim == o.kdim && p.vdim == o.vdim && p.n_pages == o.n_pages;
             heads = p.hkv > heads ? p.hkv : heads;
             widest = p.kdim + p.vdim > widest ? p.kdim + p.vdim : widest;
         }
-        TRY_RC(dtype == FLEXLLM_BF16 ? run_keep<bf16>(a, n, heads, widest, (cudaStream_t)stream) : run_keep<float>(a, n, heads, widest, (cudaStream_t)stream));
+        TRY_RC(dtype == FLEXLLM_BF16 ? run_keep<bf16>(a, heads, widest, alike, (cudaStream_t)stream) : run_keep<float>(a, heads, widest, alike, (cudaStream_t)stream));
     }
     return FLEXLLM_OK;
 }
