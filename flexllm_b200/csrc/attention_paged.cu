@@ -1,10 +1,12 @@
-// Attention of packed rows over their sequences' pages on the CUDA cores, for the 32-bit mode. A CTA of 256 threads takes RT rows
+// Attention of packed rows over their sequences' pages on the CUDA cores, for the 32-bit mode with heads of more than 128 (others:
+// attention_paged_f32.cu). A CTA of 256 threads takes RT rows
 // (TQ tokens x the query heads of one key/value head) and walks the sequence's pages, one page of 64 keys per step: S = Q K^T and
 // O += P V are both dot products of rows in shared memory (Q and K along the head, P and V^T along the keys), RT/16 x 4 and RT/16 x dv/16
 // of them per thread, two partial sums each (even and odd elements) in packed fp32 pairs. A row's 16 threads are half a warp, so that its weights
-// change hands without a barrier; the next page comes in under this one's products where shared memory holds two (heads up to 128).
+// change hands without a barrier; the next page comes in under this one's products where shared memory holds two.
 // Few tiles: a cluster of CTAs cuts the keys, and its partial maxima, sums and outputs meet in shared memory.
-// Bound by the fp32 units, at half their rate: FIGURES
+// Bound by the fp32 units and the reads of shared memory that feed them: 8 / 2 heads of 256, two prompts of 750 behind 500: 399 us, 26 TFLOP/s; four trees
+// of 25 over 3000: 153 us.
 #include "attention_paged.cuh"
 #include "tc_common.cuh"
 

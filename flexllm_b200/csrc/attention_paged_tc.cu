@@ -5,11 +5,15 @@
 //   O += P V takes P from TMEM and V^T from the pages as they lie (keys along the inner index)
 // m is lazy: only a row whose maximum exceeds it by more than kSlack moves it and rescales its O in TMEM.
 //   kPair   two tiles per CTA, so that one tile's softmax runs under the other's products: prompts
-//   kOne    one tile per CTA, two CTAs per SM: more tiles than SMs, but not long ones; and heads of more than 128
+//   kOne    one tile per CTA, two CTAs per SM: more tiles than SMs; and heads of more than 128
 //   kTurns  one tile per CTA with two sets of scores, outputs and softmax warps that take the key tiles in turn: fewer tiles than SMs (trees,
 //           decoding), whose keys are also cut among the CTAs of a cluster
 // Where a tile's keys are cut, the parts' maxima, sums and outputs meet in shared memory, in a fixed order.
 // Warps 0 .. 4 W - 1 softmax (W sets, one row per thread), then one for TMA, one for the MMAs.
+// Bound by, and measured: prompts (kPair) by the chain from scores to weights and back, the tensor cores busy 42 % (16384 tokens, 32 / 8 heads of 128: 2.0 ms,
+// 1.08 PFLOP/s, 66 % of the measured bf16 rate; 4000 tokens 151 us, 0.87 PFLOP/s); trees (kOne) by that chain and the differences
+// between sequences (16 of 25 tokens over 8000: 89 us, 4.2 TB/s); single tokens by the products, which take 128 rows for a few (one over 84500: 81 us,
+// 4.3 TB/s, the tensor cores busy 73 % on 80 SMs); short calls by latency (26 tokens over 1000: 14 us, eight prompts of 143: 11.6 us).
 // Keys behind a sequence's last one were never written: their scores are replaced, their values zeroed in shared memory. Any other value
 // that a row does not see meets a weight of zero; a row whose result is not finite is computed again, key by key.
 #include "attention_join.cuh"
@@ -448,7 +452,7 @@ int attn_paged_tc(const PagedAttn& a, cudaStream_t st) {
     t.a2 = a.scale * kLog2e;
     if (t.a2 < 1e-30f) t.a2 = 1e-30f;                     // scale 0: weights all alike, and no infinity times zero
     const long heads = (long)a.G * t.HC, seqs = a.seq.B < a.seq.T ? a.seq.B : a.seq.T, each = (a.seq.T + seqs - 1) / seqs;
-    // short tiles where two of them would hold what sequences have on average: shared memory for Q becomes stages (one token over 100000, 8 key/value
+    // short tiles where two of them would hold what sequences have on average: shared memory for Q becomes stages (one token over 84500, 8 key/value
     // heads: 105 us and 81)
     const int most = each * t.RC <= 16 ? 32 : 128;
     t.TQ = most / t.RC;
@@ -462,8 +466,8 @@ int attn_paged_tc(const PagedAttn& a, cudaStream_t st) {
     if (a.dk <= 128 && a.dv <= 128) {
         if (tiles <= sms) {
             // What the call takes in microseconds, cut into s parts, by one CTA of kTurns or two of kOne per SM: a time per key tile, one for the call, and
-            // one per part for joining rows (a tree of 26 over 1000, kTurns and kOne: 17.6 and 15.2; 16 of 31 over 8000: 103 and 89; 9 of 10
-            // over 4000: 34 and 44; one token over 100000: 62 and 157)
+            // one per part for joining rows (a tree of 26 over 1000, kTurns and kOne: 17.6 and 15.2; 16 of 25 over 8000: 103 and 89; 9 of 10
+            // over 4000: 34 and 44; one token over 84500, one head: 62 and 157; where several sequences are named, their lengths are 0.4 to 1 of the figure)
             const float rows = (float)((each < t.TQ ? each : t.TQ) * t.RC) / 128;
             const int n = (pages + 1) / 2;
             float best = 3e38f;

@@ -2,14 +2,15 @@
 //   y[m][n] = sum_groups s[n][g] * sum_{k in g} a[m][k] (q[n][k] - z[n][g])
 // Weights are on the 128-row side, up to 64 tokens on the other. A CTA walks K in steps of 128:
 //   warp 12        brings words (eight steps ahead) and activations by TMA
-//   warps 4 .. 11  put q - z, exact in bf16, into swizzled shared memory, four of them a step, the others the next (all eight a step: 13.2 us for 48 tokens,
-//                  16384 x 2048; by fours 11.7; three teams of four leave too few registers for the sums: 12.9). They load nothing from memory themselves: their fence towards the
-//                  tensor core would wait for it (words in registers, asked for four steps ahead: 18.8 us for 48 x 16384 x 2048)
+//   warps 4 .. 11  put q - z, exact in bf16, into swizzled shared memory, four of them a step, the others the next (48 tokens, 16384 x 2048: all eight a
+//                  step 13.2 us, by fours 11.7; three teams of four leave too few registers for the sums: 12.9). They load nothing from memory
+//                  themselves: their fence towards the tensor core would wait for it (words in registers, asked for four steps ahead: 18.8 us)
 //   warp 13        issues the MMAs, accumulators of their own for each group of a step, two steps' worth
 //   warps 0 .. 3   take a step's sums out of TMEM and add them up in fp32 registers, times the groups' scales: no weight is ever rounded;
 //                  they also hand the zero points to the converting warps, six steps ahead
 // Few rows: the CTAs of a cluster cut K, and their sums meet in shared memory, in a fixed order.
-// Bound by the chain of a step: one thread's waits and eight MMAs, beside it the conversion, about two instructions for half a byte.
+// Bound by the chain of a step: words from shared memory, unpacked and put back (about 600 clocks), their fence, eight MMAs. 48 tokens, 16384 x 2048: 11.8 us;
+// 64 tokens, 8192 x 8192: 21.7 us, 396 TFLOP/s, 1.5 TB/s; 64 tokens, 128256 x 2048: 83 us.
 #include "linear_w4.h"
 #include "tc_common.cuh"
 
