@@ -24,15 +24,14 @@ constexpr uint32_t kPieceBytes = 8192;
 struct F32Args {
     PagedAttn a;
     int RC, HC, TQ, heads;                 // heads per tile, head chunks per group, tokens per tile, head chunks
-    int kc, vr, o_stride, n_split;         // 128-byte blocks of a part's Q or K row, rows of a V^T part, columns of O
+    int kc, kq, vr, n_split;               // 128-byte blocks of a part's K row, 32-element chunks of a Q row, rows of a V^T part
     float a2;                              // scale * log2 e
 };
-struct F32Smem { uint32_t k, v, raw, bars, total; };
+struct F32Smem { uint32_t v, raw, bars, total; };      // two stages of K's parts, of V's, pieces
 __host__ __device__ inline F32Smem f32_smem(int kc, int vr) {
     F32Smem o;
-    o.k = 3u * kc * 16384u;
-    o.v = o.k + 3u * kc * 8192u;
-    o.raw = o.v + 3u * vr * 128u;
+    o.v = 2u * 3u * kc * 8192u;
+    o.raw = o.v + 2u * 3u * vr * 128u;
     o.bars = o.raw + kPieces * kPieceBytes;
     o.total = o.bars + 256u + 1024u;
     return o;
@@ -65,15 +64,15 @@ __global__ void __launch_bounds__(kF32Threads, 1) attn_paged_f32_kernel(const __
     const PagedAttn& a = t.a;
     const F32Smem o = f32_smem(t.kc, t.vr);
     uint64_t* bars = reinterpret_cast<uint64_t*>(base_ptr + o.bars);
-    const uint32_t bar_rf = smem_u32(bars), bar_re = bar_rf + 8 * kPieces, bar_q = bar_re + 8 * kPieces, bar_k = bar_q + 8, bar_ke = bar_k + 8, bar_v = bar_ke + 8,
-                   bar_ve = bar_v + 8, bar_s = bar_ve + 8, bar_p = bar_s + 8, bar_o = bar_p + 8, bar_f = bar_o + 8;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 20);
+    const uint32_t bar_rf = smem_u32(bars), bar_re = bar_rf + 8 * kPieces, bar_q = bar_re + 8 * kPieces, bar_k = bar_q + 8, bar_ke = bar_k + 16, bar_v = bar_ke + 16,
+                   bar_ve = bar_v + 16, bar_s = bar_ve + 16, bar_r = bar_s + 8, bar_p = bar_r + 8, bar_o = bar_p + 8, bar_f = bar_o + 8;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 24);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < kPieces; i++) { mbar_init(bar_rf + 8 * i, 1); mbar_init(bar_re + 8 * i, 8); }
-        mbar_init(bar_q, 8); mbar_init(bar_k, 8); mbar_init(bar_ke, 1); mbar_init(bar_v, 8); mbar_init(bar_ve, 1);
-        mbar_init(bar_s, 1); mbar_init(bar_p, 4); mbar_init(bar_o, 1); mbar_init(bar_f, 1);
+        for (int i = 0; i < 2; i++) { mbar_init(bar_k + 8 * i, 8); mbar_init(bar_ke + 8 * i, 1); mbar_init(bar_v + 8 * i, 8); mbar_init(bar_ve + 8 * i, 1); }
+        mbar_init(bar_q, 8); mbar_init(bar_s, 1); mbar_init(bar_r, 4); mbar_init(bar_p, 4); mbar_init(bar_o, 1); mbar_init(bar_f, 1);
         *abort_flag = 0;
         fence_barrier_init();
     }
@@ -90,7 +89,7 @@ __global__ void __launch_bounds__(kF32Threads, 1) attn_paged_f32_kernel(const __
     __syncthreads();
     tc_fence_after();
     pdl_launch();                                         // behind the allocation: no later kernel may hold the TMEM that this one waits for
-    const uint32_t tmem = *tmem_slot, tP = tmem + 64, tO = tmem + 192;
+    const uint32_t tmem = *tmem_slot, tP = tmem + 64, tO = tmem + 192, tQ = tmem + 320;      // S at the start
     const int b = unit_sm.b;
     const SeqRows s = unit_sm.s;
     const int R = a.H / a.G, g = hg / t.HC, h0 = g * R + (hg % t.HC) * t.RC, heads = min(t.RC, (g + 1) * R - h0);
@@ -122,31 +121,34 @@ __global__ void __launch_bounds__(kF32Threads, 1) attn_paged_f32_kernel(const __
         const int u0 = uniform_max(t0), u1 = uniform_max(t1);
         const uint32_t idesc_qk = umma_idesc_bf16(128, kPage), idesc_pv = umma_idesc_bf16(128, t.vr);
         const int ksteps = (a.dk + 15) / 16;
-        const uint32_t q_lo = umma_desc_lo(base), k_lo = umma_desc_lo(base + o.k), v_lo = umma_desc_lo(base + o.v);
+        const uint32_t k_lo = umma_desc_lo(base), v_lo = umma_desc_lo(base + o.v), k_stage = 3u * t.kc * 512u, v_stage = 3u * t.vr * 8u;
         // products of parts, the small ones first
         auto parts = [](int x, uint32_t& pa, uint32_t& pb) {
             pa = x == 1 ? 2u : x == 2 || x == 4 ? 1u : 0u;
             pb = x == 0 ? 2u : x == 2 || x == 3 ? 1u : 0u;
         };
         auto qk = [&](int n) {
-            if (!wait(bar_k, (uint32_t)(n & 1))) return false;
+            const uint32_t st = n & 1;
+            if (!wait(bar_k + 8 * st, (uint32_t)(n >> 1 & 1))) return false;
+            if (n > 0 && !wait(bar_r, (uint32_t)(n - 1 & 1))) return false;      // the scores in front have been read
             tc_fence_after();
 #pragma unroll
             for (int x = 0; x < 6; x++) {
                 uint32_t pa, pb;
                 parts(x, pa, pb);
-                const uint32_t qa = q_lo + pa * (uint32_t)t.kc * 1024u, ka = k_lo + pb * (uint32_t)t.kc * 512u;
-                for (int k = 0; k < ksteps; k++)
-                    umma_bf16_lo(leader, u_tmem, qa + (k >> 2) * 1024u + 2 * (k & 3), ka + (k >> 2) * 512u + 2 * (k & 3), idesc_qk, x > 0 || k > 0);
+                const uint32_t qa = u_tmem + 320 + pa * (uint32_t)t.kq * 16u, ka = k_lo + st * k_stage + pb * (uint32_t)t.kc * 512u;
+                for (int k = 0; k < ksteps; k++) umma_bf16_ts_lo(leader, u_tmem, qa + 8 * k, ka + (k >> 2) * 512u + 2 * (k & 3), idesc_qk, x > 0 || k > 0);
             }
             umma_commit_by(leader, bar_s);
-            umma_commit_by(leader, bar_ke);
+            umma_commit_by(leader, bar_ke + 8 * st);
             return true;
         };
         bool ok = u0 < u1 && wait(bar_q, 0) && qk(0);
         for (int j = u0; ok && j < u1; j++) {
             const int n = j - u0;
-            ok = wait(bar_v, (uint32_t)(n & 1)) && wait(bar_p, (uint32_t)(n & 1));
+            const uint32_t st = n & 1;
+            if (j + 1 < u1 && !qk(n + 1)) break;          // under this page's softmax
+            ok = wait(bar_v + 8 * st, (uint32_t)(n >> 1 & 1)) && wait(bar_p, (uint32_t)(n & 1));
             if (!ok) break;
             tc_fence_after();
 #pragma unroll
@@ -155,11 +157,10 @@ __global__ void __launch_bounds__(kF32Threads, 1) attn_paged_f32_kernel(const __
                 parts(x, pa, pb);
 #pragma unroll
                 for (uint32_t k = 0; k < 4; k++)
-                    umma_bf16_ts_lo(leader, u_tmem + 192, u_tmem + 64 + 32 * pa + 8 * k, v_lo + pb * (uint32_t)t.vr * 8u + 2 * k, idesc_pv, n > 0 || x > 0 || k > 0);
+                    umma_bf16_ts_lo(leader, u_tmem + 192, u_tmem + 64 + 32 * pa + 8 * k, v_lo + st * v_stage + pb * (uint32_t)t.vr * 8u + 2 * k, idesc_pv, n > 0 || x > 0 || k > 0);
             }
             umma_commit_by(leader, j + 1 < u1 ? bar_o : bar_f);           // the last one has a barrier of its own
-            umma_commit_by(leader, bar_ve);
-            if (j + 1 < u1) ok = qk(n + 1);
+            umma_commit_by(leader, bar_ve + 8 * st);
         }
     } else if (warp >= 4) {
         // ---- numbers into parts: 8 of them per thread and piece
@@ -169,21 +170,33 @@ __global__ void __launch_bounds__(kF32Threads, 1) attn_paged_f32_kernel(const __
 #pragma unroll
             for (int p = 0; p < 3; p++) *reinterpret_cast<uint4*>(base_ptr + at + p * stride + row * 128 + (((c ^ row) & 7) << 4)) = part[p];
         };
-        const uint32_t q_part = (uint32_t)t.kc * 16384u, k_part = (uint32_t)t.kc * 8192u, v_part = (uint32_t)t.vr * 128u;
+        const uint32_t k_part = (uint32_t)t.kc * 8192u, v_part = (uint32_t)t.vr * 128u;
         if (t0 < t1) {
-            for (int e = ct; e < 128 * per; e += 256) {
-                const int row = e / per, c = e - row * per, i = i0 + row / t.RC;
-                float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-                if (row < t.TQ * t.RC && i < s.n && row % t.RC < heads) load8((const float*)a.q + (long)(s.row0 + i) * a.ldq + (long)(h0 + row % t.RC) * a.dk + c * 8, f);
-                cut8(f, part);
-                put((uint32_t)(c >> 3) * 16384u, q_part, row, c);
+            // Q's parts into TMEM, two elements per column: warps w and w + 4 have the same rows, and 32-element chunks in turn
+            const int row = threadIdx.x & 127, i = i0 + row / t.RC;
+            const bool live = row < t.TQ * t.RC && i < s.n && row % t.RC < heads;
+            const float* src = (const float*)a.q + (long)(s.row0 + i) * a.ldq + (long)(h0 + row % t.RC) * a.dk;
+            for (int c = (warp - 4) >> 2; c < t.kq; c += 2) {
+                uint32_t pk[3][16];
+#pragma unroll
+                for (int x = 0; x < 4; x++) {
+                    float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                    if (live && 32 * c + 8 * x < a.dk) load8(src + 32 * c + 8 * x, f);
+                    cut8(f, part);
+#pragma unroll
+                    for (int p = 0; p < 3; p++) { pk[p][4 * x] = part[p].x; pk[p][4 * x + 1] = part[p].y; pk[p][4 * x + 2] = part[p].z; pk[p][4 * x + 3] = part[p].w; }
+                }
+                __syncwarp();
+#pragma unroll
+                for (int p = 0; p < 3; p++) tmem_st_32x16(tQ + (uint32_t)(p * t.kq + c) * 16u + ((uint32_t)((warp & 3) * 32) << 16), pk[p]);
             }
-            if (per & 1) {                                // the last 16 elements of a product reach beyond the row: zeros in Q and K
+            if ((per & 1) && ct < kPage) {                // the last 16 elements of a product reach beyond the row: zeros in K
                 part[0] = part[1] = part[2] = make_uint4(0, 0, 0, 0);
-                if (ct < 128) put((uint32_t)(per >> 3) * 16384u, q_part, ct, per);
-                if (ct < kPage) put(o.k + (uint32_t)(per >> 3) * 8192u, k_part, ct, per);
+                for (uint32_t st = 0; st < 2; st++) put(st * 3 * k_part + (uint32_t)(per >> 3) * 8192u, k_part, ct, per);
             }
             fence_proxy_async_smem();
+            tmem_st_wait();
+            tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(bar_q);
         }
@@ -200,20 +213,21 @@ __global__ void __launch_bounds__(kF32Threads, 1) attn_paged_f32_kernel(const __
         };
         for (int j = t0; ok && j < t1; j++) {
             const int n = j - t0, left = end - j * kPage;
-            ok = wait(bar_ke, (uint32_t)(n & 1) ^ 1u);
+            const uint32_t st = n & 1, free = (uint32_t)(n >> 1 & 1) ^ 1u, k_at = st * 3 * k_part, v_at = o.v + st * 3 * v_part;
+            ok = wait(bar_ke + 8 * st, free);
             for (int c = 0; ok && c < 4; c++)
                 next_piece([&](const float* src) {
                     if (key >= 16) return;
                     float f[8];
                     load8(src + key * a.dk + col * 8, f);
                     cut8(f, part);
-                    put(o.k + (uint32_t)(col >> 3) * 8192u, k_part, c * 16 + key, col);
+                    put(k_at + (uint32_t)(col >> 3) * 8192u, k_part, c * 16 + key, col);
                 });
             if (!ok) break;
             fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive(bar_k);
-            ok = wait(bar_ve, (uint32_t)(n & 1) ^ 1u);
+            if (lane == 0) mbar_arrive(bar_k + 8 * st);
+            ok = wait(bar_ve + 8 * st, free);
             for (int c = 0; ok && c < v_pieces; c++)
                 next_piece([&](const float* src) {
                     const int d = ct >> 3, k8 = (ct & 7) * 8;
@@ -226,12 +240,12 @@ __global__ void __launch_bounds__(kF32Threads, 1) attn_paged_f32_kernel(const __
                         for (int x = 0; x < 8; x++)
                             if (k8 + x >= left) f[x] = 0.0f;
                     cut8(f, part);
-                    put(o.v, v_part, 32 * c + d, k8 >> 3);
+                    put(v_at, v_part, 32 * c + d, k8 >> 3);
                 });
             if (!ok) break;
             fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive(bar_v);
+            if (lane == 0) mbar_arrive(bar_v + 8 * st);
         }
     } else {
         // ---- one row per thread
@@ -251,6 +265,9 @@ __global__ void __launch_bounds__(kF32Threads, 1) attn_paged_f32_kernel(const __
             tmem_ld_32x32(tmem + lane_addr, v[0]);
             tmem_ld_32x32(tmem + 32 + lane_addr, v[1]);
             tmem_ld_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_r);
             if (!__all_sync(0xffffffffu, sure - j * kPage >= kPage))
 #pragma unroll
                 for (int c = 0; c < 2; c++) {
@@ -298,9 +315,14 @@ __global__ void __launch_bounds__(kF32Threads, 1) attn_paged_f32_kernel(const __
                         e0 -= bf_lo(pk[p][x >> 1]); e1 -= bf_hi(pk[p][x >> 1]);
                     }
                 }
+                if (c == 0 && n > 0) {                    // the weights in front have been read
+                    if (!wait(bar_o, (uint32_t)((n - 1) & 1))) { ok = false; break; }
+                    tc_fence_after();
+                }
 #pragma unroll
                 for (int p = 0; p < 3; p++) tmem_st_32x16(tP + 32 * p + 16 * c + lane_addr, pk[p]);
             }
+            if (!ok) break;
             l += sum[0] + sum[1];
             tmem_st_wait();
             tc_fence_before();
@@ -377,7 +399,7 @@ int attn_paged_f32(const PagedAttn& a, cudaStream_t st) {
     const int R = a.H / a.G;
     t.a = a;
     t.RC = R < 128 ? R : 128; t.HC = (R + t.RC - 1) / t.RC; t.TQ = 128 / t.RC;
-    t.kc = (a.dk + 63) / 64; t.vr = (a.dv + 15) / 16 * 16; t.o_stride = (t.vr + 31) / 32 * 32;
+    t.kc = (a.dk + 63) / 64; t.kq = (a.dk + 31) / 32; t.vr = (a.dv + 15) / 16 * 16;
     t.a2 = a.scale * kLog2e;
     if (t.a2 < 1e-30f) t.a2 = 1e-30f;                     // scale 0: weights all alike, and no infinity times zero
     const long heads = (long)a.G * t.HC, seqs = a.seq.B < a.seq.T ? a.seq.B : a.seq.T, ones = most_units(a.seq, t.TQ);
