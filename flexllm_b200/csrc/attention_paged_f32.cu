@@ -18,37 +18,40 @@ using namespace tc;
 
 namespace {
 
-constexpr int kPieces = 4, kF32Threads = 448;
+constexpr int kPieces = 16, kF32Threads = 448;      // of a page: four of K, four of V, for a warp each; two pages
 constexpr uint32_t kPieceBytes = 8192;
 
 struct F32Args {
     PagedAttn a;
     int RC, HC, TQ, heads;                 // heads per tile, head chunks per group, tokens per tile, head chunks
     int kc, kq, vr, n_split;               // 128-byte blocks of a part's K row, 32-element chunks of a Q row, rows of a V^T part
+    int v_rows;                            // rows of a piece of V^T
     float a2;                              // scale * log2 e
 };
-struct F32Smem { uint32_t v, raw, bars, total; };      // two stages of K's parts, of V's, pieces
+struct F32Smem { uint32_t v, raw, bars, total; };      // K's parts, V's parts, pieces
 __host__ __device__ inline F32Smem f32_smem(int kc, int vr) {
     F32Smem o;
-    o.v = 2u * 3u * kc * 8192u;
-    o.raw = o.v + 2u * 3u * vr * 128u;
+    o.v = 3u * kc * 8192u;
+    o.raw = o.v + 3u * vr * 128u;
     o.bars = o.raw + kPieces * kPieceBytes;
-    o.total = o.bars + 256u + 1024u;
+    o.total = o.bars + 512u + 1024u;
     return o;
 }
 
-// 8 numbers as their three parts, pairs in order. The first part carries an infinity or NaN.
+// 8 numbers as their three parts, pairs in order: twice what is nearest in eight bits and the rest, all exact (bits are added and cut; a number up to half
+// a step short of 2^128 becomes an infinity). Where an infinity or a NaN is among them, a NaN is in some part.
 __device__ __forceinline__ void cut8(float (&f)[8], uint4 (&part)[3]) {
 #pragma unroll
     for (int p = 0; p < 3; p++) {
-        const uint32_t w[4] = {bf_pack(f[0], f[1]), bf_pack(f[2], f[3]), bf_pack(f[4], f[5]), bf_pack(f[6], f[7])};
-        part[p] = make_uint4(w[0], w[1], w[2], w[3]);
-        if (p < 2)
+        uint32_t h[8];
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                f[2 * j] = fabsf(f[2 * j]) <= 3.0e38f ? f[2 * j] - bf_lo(w[j]) : 0.0f;
-                f[2 * j + 1] = fabsf(f[2 * j + 1]) <= 3.0e38f ? f[2 * j + 1] - bf_hi(w[j]) : 0.0f;
-            }
+        for (int j = 0; j < 8; j++) {
+            h[j] = __float_as_uint(f[j]);
+            if (p == 2) continue;                         // eight bits are left
+            h[j] = (h[j] + 0x8000u) & 0xffff0000u;
+            f[j] -= __uint_as_float(h[j]);
+        }
+        part[p] = make_uint4(__byte_perm(h[0], h[1], 0x7632), __byte_perm(h[2], h[3], 0x7632), __byte_perm(h[4], h[5], 0x7632), __byte_perm(h[6], h[7], 0x7632));
     }
 }
 __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
@@ -64,15 +67,14 @@ __global__ void __launch_bounds__(kF32Threads, 1) attn_paged_f32_kernel(const __
     const PagedAttn& a = t.a;
     const F32Smem o = f32_smem(t.kc, t.vr);
     uint64_t* bars = reinterpret_cast<uint64_t*>(base_ptr + o.bars);
-    const uint32_t bar_rf = smem_u32(bars), bar_re = bar_rf + 8 * kPieces, bar_q = bar_re + 8 * kPieces, bar_k = bar_q + 8, bar_ke = bar_k + 16, bar_v = bar_ke + 16,
-                   bar_ve = bar_v + 16, bar_s = bar_ve + 16, bar_r = bar_s + 8, bar_p = bar_r + 8, bar_o = bar_p + 8, bar_f = bar_o + 8;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 24);
+    const uint32_t bar_rf = smem_u32(bars), bar_re = bar_rf + 8 * kPieces, bar_q = bar_re + 8 * kPieces, bar_k = bar_q + 8, bar_ke = bar_k + 8, bar_v = bar_ke + 8,
+                   bar_ve = bar_v + 8, bar_s = bar_ve + 8, bar_r = bar_s + 8, bar_p = bar_r + 8, bar_o = bar_p + 8, bar_f = bar_o + 8;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 48);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < kPieces; i++) { mbar_init(bar_rf + 8 * i, 1); mbar_init(bar_re + 8 * i, 8); }
-        for (int i = 0; i < 2; i++) { mbar_init(bar_k + 8 * i, 8); mbar_init(bar_ke + 8 * i, 1); mbar_init(bar_v + 8 * i, 8); mbar_init(bar_ve + 8 * i, 1); }
-        mbar_init(bar_q, 8); mbar_init(bar_s, 1); mbar_init(bar_r, 4); mbar_init(bar_p, 4); mbar_init(bar_o, 1); mbar_init(bar_f, 1);
+        for (int i = 0; i < kPieces; i++) { mbar_init(bar_rf + 8 * i, 1); mbar_init(bar_re + 8 * i, 1); }
+        mbar_init(bar_q, 8); mbar_init(bar_k, 4); mbar_init(bar_ke, 1); mbar_init(bar_v, 4); mbar_init(bar_ve, 1); mbar_init(bar_s, 1); mbar_init(bar_r, 4); mbar_init(bar_p, 4); mbar_init(bar_o, 1); mbar_init(bar_f, 1);
         *abort_flag = 0;
         fence_barrier_init();
     }
@@ -97,58 +99,56 @@ __global__ void __launch_bounds__(kF32Threads, 1) attn_paged_f32_kernel(const __
     const int end = b < 0 ? 0 : a.mask ? s.ctx + s.n : min(s.ctx + i0 + t.TQ, s.ctx + s.n), n_pg = (end + kPage - 1) / kPage;
     const int t0 = (int)((long)n_pg * split / t.n_split), t1 = (int)((long)n_pg * (split + 1) / t.n_split);
     auto wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_spin(bar, parity, abort_flag)) != 0; };
-    const int v_pieces = (a.dv + 31) / 32;
     if (b >= 0) {
     if (warp == 12) {
-        int ids = 0, piece = 0;
-        bool ok = true;
-        for (int j = t0; ok && j < t1; j++) {
-            const int n = j - t0;
+        // lane w brings the pieces of the cutting warp w
+        const int c = lane & 3, rows = min(t.v_rows, a.dv - c * t.v_rows);
+        const uint32_t bytes = lane < 4 ? 16u * a.dk * 4u : (uint32_t)(rows * 256);
+        bool ok = lane < 4 || (lane < 8 && rows > 0);
+        int ids = 0;
+        for (int j = t0; j < t1; j++) {
+            const int n = j - t0, st = lane * 2 + (n & 1);
             if ((n & 31) == 0) ids = j + lane < t1 ? page_of(a.seq, b, j + lane) : 0;
             const long at = ((long)__shfl_sync(0xffffffffu, ids, n & 31) * a.G + g) * kPage;
-            for (int c = 0; ok && c < 4 + v_pieces; c++, piece++) {
-                const int st = piece % kPieces;
-                ok = wait(bar_re + 8 * st, (uint32_t)(piece / kPieces & 1) ^ 1u);
-                if (!ok || lane != 0) continue;
-                const uint32_t bytes = c < 4 ? 16u * a.dk * 4u : (uint32_t)min(32, a.dv - 32 * (c - 4)) * 256u;
-                const float* src = c < 4 ? (const float*)a.k + at * a.dk + (long)c * 16 * a.dk : (const float*)a.v + at * a.dv + (long)(c - 4) * 32 * kPage;
+            ok = ok && mbar_spin(bar_re + 8 * st, (uint32_t)(n >> 1 & 1) ^ 1u, abort_flag);
+            if (ok) {
                 mbar_expect_tx(bar_rf + 8 * st, bytes);
-                bulk_copy(base + o.raw + st * kPieceBytes, src, bytes, bar_rf + 8 * st);
+                bulk_copy(base + o.raw + st * kPieceBytes, lane < 4 ? (const float*)a.k + (at + c * 16) * a.dk : (const float*)a.v + at * a.dv + (long)c * t.v_rows * kPage, bytes,
+                          bar_rf + 8 * st);
             }
+            __syncwarp();
         }
     } else if (warp == 13) {
         const uint32_t leader = elect_leader(), u_tmem = (uint32_t)uniform_max((int)tmem);
         const int u0 = uniform_max(t0), u1 = uniform_max(t1);
         const uint32_t idesc_qk = umma_idesc_bf16(128, kPage), idesc_pv = umma_idesc_bf16(128, t.vr);
         const int ksteps = (a.dk + 15) / 16;
-        const uint32_t k_lo = umma_desc_lo(base), v_lo = umma_desc_lo(base + o.v), k_stage = 3u * t.kc * 512u, v_stage = 3u * t.vr * 8u;
+        const uint32_t k_lo = umma_desc_lo(base), v_lo = umma_desc_lo(base + o.v);
         // products of parts, the small ones first
         auto parts = [](int x, uint32_t& pa, uint32_t& pb) {
             pa = x == 1 ? 2u : x == 2 || x == 4 ? 1u : 0u;
             pb = x == 0 ? 2u : x == 2 || x == 3 ? 1u : 0u;
         };
         auto qk = [&](int n) {
-            const uint32_t st = n & 1;
-            if (!wait(bar_k + 8 * st, (uint32_t)(n >> 1 & 1))) return false;
+            if (!wait(bar_k, (uint32_t)(n & 1))) return false;
             if (n > 0 && !wait(bar_r, (uint32_t)(n - 1 & 1))) return false;      // the scores in front have been read
             tc_fence_after();
 #pragma unroll
             for (int x = 0; x < 6; x++) {
                 uint32_t pa, pb;
                 parts(x, pa, pb);
-                const uint32_t qa = u_tmem + 320 + pa * (uint32_t)t.kq * 16u, ka = k_lo + st * k_stage + pb * (uint32_t)t.kc * 512u;
+                const uint32_t qa = u_tmem + 320 + pa * (uint32_t)t.kq * 16u, ka = k_lo + pb * (uint32_t)t.kc * 512u;
                 for (int k = 0; k < ksteps; k++) umma_bf16_ts_lo(leader, u_tmem, qa + 8 * k, ka + (k >> 2) * 512u + 2 * (k & 3), idesc_qk, x > 0 || k > 0);
             }
             umma_commit_by(leader, bar_s);
-            umma_commit_by(leader, bar_ke + 8 * st);
+            umma_commit_by(leader, bar_ke);
             return true;
         };
         bool ok = u0 < u1 && wait(bar_q, 0) && qk(0);
         for (int j = u0; ok && j < u1; j++) {
             const int n = j - u0;
-            const uint32_t st = n & 1;
             if (j + 1 < u1 && !qk(n + 1)) break;          // under this page's softmax
-            ok = wait(bar_v + 8 * st, (uint32_t)(n >> 1 & 1)) && wait(bar_p, (uint32_t)(n & 1));
+            ok = wait(bar_v, (uint32_t)(n & 1)) && wait(bar_p, (uint32_t)(n & 1));
             if (!ok) break;
             tc_fence_after();
 #pragma unroll
@@ -157,10 +157,10 @@ __global__ void __launch_bounds__(kF32Threads, 1) attn_paged_f32_kernel(const __
                 parts(x, pa, pb);
 #pragma unroll
                 for (uint32_t k = 0; k < 4; k++)
-                    umma_bf16_ts_lo(leader, u_tmem + 192, u_tmem + 64 + 32 * pa + 8 * k, v_lo + st * v_stage + pb * (uint32_t)t.vr * 8u + 2 * k, idesc_pv, n > 0 || x > 0 || k > 0);
+                    umma_bf16_ts_lo(leader, u_tmem + 192, u_tmem + 64 + 32 * pa + 8 * k, v_lo + pb * (uint32_t)t.vr * 8u + 2 * k, idesc_pv, n > 0 || x > 0 || k > 0);
             }
             umma_commit_by(leader, j + 1 < u1 ? bar_o : bar_f);           // the last one has a barrier of its own
-            umma_commit_by(leader, bar_ve + 8 * st);
+            umma_commit_by(leader, bar_ve);
         }
     } else if (warp >= 4) {
         // ---- numbers into parts: 8 of them per thread and piece
@@ -192,7 +192,7 @@ __global__ void __launch_bounds__(kF32Threads, 1) attn_paged_f32_kernel(const __
             }
             if ((per & 1) && ct < kPage) {                // the last 16 elements of a product reach beyond the row: zeros in K
                 part[0] = part[1] = part[2] = make_uint4(0, 0, 0, 0);
-                for (uint32_t st = 0; st < 2; st++) put(st * 3 * k_part + (uint32_t)(per >> 3) * 8192u, k_part, ct, per);
+                put((uint32_t)(per >> 3) * 8192u, k_part, ct, per);
             }
             fence_proxy_async_smem();
             tmem_st_wait();
@@ -200,52 +200,46 @@ __global__ void __launch_bounds__(kF32Threads, 1) attn_paged_f32_kernel(const __
             __syncwarp();
             if (lane == 0) mbar_arrive(bar_q);
         }
-        const int key = ct / per, col = ct - key * per;   // of a piece of K: 16 keys
-        int piece = 0;
+        // warps 4 .. 7: 16 keys of K each, 8 .. 11: rows of V^T; each has its pieces to itself and goes through them without the others
+        const int w = warp - 4, c = w & 3, rows = min(t.v_rows, a.dv - c * t.v_rows), count = w < 4 ? 16 * per : rows * 8;
+        const uint32_t inv = 65535u / (uint32_t)per + 1u;         // e / per for e < 256
         bool ok = true;
-        auto next_piece = [&](auto f) {
-            const int st = piece % kPieces;
-            ok = ok && wait(bar_rf + 8 * st, (uint32_t)(piece / kPieces & 1));
-            if (ok) f((const float*)(base_ptr + o.raw + st * kPieceBytes));
-            __syncwarp();
-            if (ok && lane == 0) mbar_arrive(bar_re + 8 * st);
-            piece++;
-        };
-        for (int j = t0; ok && j < t1; j++) {
-            const int n = j - t0, left = end - j * kPage;
-            const uint32_t st = n & 1, free = (uint32_t)(n >> 1 & 1) ^ 1u, k_at = st * 3 * k_part, v_at = o.v + st * 3 * v_part;
-            ok = wait(bar_ke + 8 * st, free);
-            for (int c = 0; ok && c < 4; c++)
-                next_piece([&](const float* src) {
-                    if (key >= 16) return;
-                    float f[8];
-                    load8(src + key * a.dk + col * 8, f);
-                    cut8(f, part);
-                    put(k_at + (uint32_t)(col >> 3) * 8192u, k_part, c * 16 + key, col);
-                });
+        for (int j = t0; j < t1; j++) {
+            const int n = j - t0, left = end - j * kPage, st = w * 2 + (n & 1);
+            ok = wait(w < 4 ? bar_ke : bar_ve, (uint32_t)(n & 1) ^ 1u) && (count <= 0 || wait(bar_rf + 8 * st, (uint32_t)(n >> 1 & 1)));
             if (!ok) break;
-            fence_proxy_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar_k + 8 * st);
-            ok = wait(bar_ve + 8 * st, free);
-            for (int c = 0; ok && c < v_pieces; c++)
-                next_piece([&](const float* src) {
-                    const int d = ct >> 3, k8 = (ct & 7) * 8;
-                    if (32 * c + d >= a.dv) return;
-                    float f[8];
-                    load8(src + d * kPage + k8, f);
-                    // keys behind the sequence's last one were never written: zeros, so that a weight of zero stays without effect
-                    if (k8 + 8 > left)
+            const float* src = (const float*)(base_ptr + o.raw + st * kPieceBytes);
+            for (int e0 = lane; e0 < count; e0 += 64) {
+                float f[2][8];
 #pragma unroll
-                        for (int x = 0; x < 8; x++)
-                            if (k8 + x >= left) f[x] = 0.0f;
-                    cut8(f, part);
-                    put(v_at, v_part, 32 * c + d, k8 >> 3);
-                });
-            if (!ok) break;
+                for (int x = 0; x < 2; x++)
+                    if (e0 + 32 * x < count) load8(src + (e0 + 32 * x) * 8, f[x]);
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    const int e = e0 + 32 * x;
+                    if (e >= count) break;
+                    if (w < 4) {
+                        const int key = (int)(e * inv >> 16), col = e - key * per;
+                        cut8(f[x], part);
+                        put((uint32_t)(col >> 3) * 8192u, k_part, c * 16 + key, col);
+                    } else {
+                        // keys behind the sequence's last one were never written: zeros, so that a weight of zero stays without effect
+                        const int k8 = (e & 7) * 8;
+                        if (k8 + 8 > left)
+#pragma unroll
+                            for (int y = 0; y < 8; y++)
+                                if (k8 + y >= left) f[x][y] = 0.0f;
+                        cut8(f[x], part);
+                        put(o.v, v_part, c * t.v_rows + (e >> 3), k8 >> 3);
+                    }
+                }
+            }
             fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0) mbar_arrive(bar_v + 8 * st);
+            if (lane == 0) {
+                if (count > 0) mbar_arrive(bar_re + 8 * st);
+                mbar_arrive(w < 4 ? bar_k : bar_v);
+            }
         }
     } else {
         // ---- one row per thread
@@ -400,6 +394,7 @@ int attn_paged_f32(const PagedAttn& a, cudaStream_t st) {
     t.a = a;
     t.RC = R < 128 ? R : 128; t.HC = (R + t.RC - 1) / t.RC; t.TQ = 128 / t.RC;
     t.kc = (a.dk + 63) / 64; t.kq = (a.dk + 31) / 32; t.vr = (a.dv + 15) / 16 * 16;
+    t.v_rows = (a.dv + 31) / 32 * 8;
     t.a2 = a.scale * kLog2e;
     if (t.a2 < 1e-30f) t.a2 = 1e-30f;                     // scale 0: weights all alike, and no infinity times zero
     const long heads = (long)a.G * t.HC, seqs = a.seq.B < a.seq.T ? a.seq.B : a.seq.T, ones = most_units(a.seq, t.TQ);
