@@ -18,41 +18,56 @@ using namespace tc;
 
 namespace {
 
-constexpr int kPieces = 16, kF32Threads = 448;      // of a page: four of K, four of V, for a warp each; two pages
-constexpr uint32_t kPieceBytes = 8192;
+constexpr int kF32Threads = 448, kMostSlots = 4;     // slots for pieces per cutting warp: 4, 2 or 1, as shared memory has room
+constexpr uint32_t kPieceBytes = 4096;
 
 struct F32Args {
     PagedAttn a;
     int RC, HC, TQ, heads;                 // heads per tile, head chunks per group, tokens per tile, head chunks
     int kc, kq, vr, n_split;               // 128-byte blocks of a part's K row, 32-element chunks of a Q row, rows of a V^T part
-    int v_rows;                            // rows of a piece of V^T
+    int v_rows, slots_log, two;            // rows of V^T of a cutting warp; its slots; K's and V's parts have two stages (1) or one (0)
     float a2;                              // scale * log2 e
 };
-struct F32Smem { uint32_t v, raw, bars, total; };      // K's parts, V's parts, pieces
-__host__ __device__ inline F32Smem f32_smem(int kc, int vr) {
+struct F32Smem { uint32_t v, raw, bars, total; };      // K's parts, V's, pieces
+__host__ __device__ inline F32Smem f32_smem(int kc, int vr, int slots_log, int two) {
     F32Smem o;
-    o.v = 3u * kc * 8192u;
-    o.raw = o.v + 3u * vr * 128u;
-    o.bars = o.raw + kPieces * kPieceBytes;
-    o.total = o.bars + 512u + 1024u;
+    o.v = (3u << two) * kc * 8192u;
+    o.raw = o.v + (3u << two) * vr * 128u;
+    o.bars = o.raw + (8u << slots_log) * kPieceBytes;
+    o.total = o.bars + 1024u + 1024u;
     return o;
 }
 
-// 8 numbers as their three parts, pairs in order: twice what is nearest in eight bits and the rest, all exact (bits are added and cut; a number up to half
-// a step short of 2^128 becomes an infinity). Where an infinity or a NaN is among them, a NaN is in some part.
-__device__ __forceinline__ void cut8(float (&f)[8], uint4 (&part)[3]) {
+// Two numbers less what is nearest to them in bf16, which is `w`: exact
+__device__ __forceinline__ f32x2 rest2(f32x2 f, uint32_t w) { return fma2(pack2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)), pack2(-1.0f, -1.0f), f); }
+__device__ __forceinline__ uint32_t near2(f32x2 f) {
+    float x, y;
+    unpack2(f, x, y);
+    return bf_pack(x, y);
+}
+// 8 numbers as their three parts: twice what is nearest in eight bits, and the rest. Where an infinity or a NaN is among them, a NaN is in some part.
+__device__ __forceinline__ void cut8(const float (&f)[8], uint4 (&part)[3]) {
+    f32x2 v[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) v[j] = pack2(f[2 * j], f[2 * j + 1]);
 #pragma unroll
     for (int p = 0; p < 3; p++) {
-        uint32_t h[8];
+        const uint32_t w[4] = {near2(v[0]), near2(v[1]), near2(v[2]), near2(v[3])};
+        part[p] = make_uint4(w[0], w[1], w[2], w[3]);
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            h[j] = __float_as_uint(f[j]);
-            if (p == 2) continue;                         // eight bits are left
-            h[j] = (h[j] + 0x8000u) & 0xffff0000u;
-            f[j] -= __uint_as_float(h[j]);
-        }
-        part[p] = make_uint4(__byte_perm(h[0], h[1], 0x7632), __byte_perm(h[2], h[3], 0x7632), __byte_perm(h[4], h[5], 0x7632), __byte_perm(h[6], h[7], 0x7632));
+        for (int j = 0; j < 4; j++) v[j] = rest2(v[j], w[j]);
     }
+}
+// 32 bytes per lane, the lanes' side by side. Every other four lanes read their second half first (flip 16), so that eight lanes meet all banks once.
+__device__ __forceinline__ void load8_shared(uint32_t at, uint32_t flip, float (&f)[8]) {
+    float x[4], y[4];
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]) : "r"(at + flip));
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(y[0]), "=f"(y[1]), "=f"(y[2]), "=f"(y[3]) : "r"(at + (flip ^ 16u)));
+#pragma unroll
+    for (int i = 0; i < 4; i++) { f[i] = flip ? y[i] : x[i]; f[4 + i] = flip ? x[i] : y[i]; }
+}
+__device__ __forceinline__ void store_shared(uint32_t at, const uint4& v) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
@@ -65,16 +80,17 @@ __global__ void __launch_bounds__(kF32Threads, 1) attn_paged_f32_kernel(const __
     const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
     uint8_t* base_ptr = smem_raw + (base - raw);
     const PagedAttn& a = t.a;
-    const F32Smem o = f32_smem(t.kc, t.vr);
+    const F32Smem o = f32_smem(t.kc, t.vr, t.slots_log, t.two);
     uint64_t* bars = reinterpret_cast<uint64_t*>(base_ptr + o.bars);
-    const uint32_t bar_rf = smem_u32(bars), bar_re = bar_rf + 8 * kPieces, bar_q = bar_re + 8 * kPieces, bar_k = bar_q + 8, bar_ke = bar_k + 8, bar_v = bar_ke + 8,
-                   bar_ve = bar_v + 8, bar_s = bar_ve + 8, bar_r = bar_s + 8, bar_p = bar_r + 8, bar_o = bar_p + 8, bar_f = bar_o + 8;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 48);
+    const uint32_t bar_rf = smem_u32(bars), bar_re = bar_rf + 64 * kMostSlots, bar_q = bar_re + 64 * kMostSlots, bar_k = bar_q + 8, bar_ke = bar_k + 16, bar_v = bar_ke + 16,
+                   bar_ve = bar_v + 16, bar_s = bar_ve + 16, bar_r = bar_s + 8, bar_p = bar_r + 8, bar_o = bar_p + 8, bar_f = bar_o + 8;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 96);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
-        for (int i = 0; i < kPieces; i++) { mbar_init(bar_rf + 8 * i, 1); mbar_init(bar_re + 8 * i, 1); }
-        mbar_init(bar_q, 8); mbar_init(bar_k, 4); mbar_init(bar_ke, 1); mbar_init(bar_v, 4); mbar_init(bar_ve, 1); mbar_init(bar_s, 1); mbar_init(bar_r, 4); mbar_init(bar_p, 4); mbar_init(bar_o, 1); mbar_init(bar_f, 1);
+        for (int i = 0; i < 8 * kMostSlots; i++) { mbar_init(bar_rf + 8 * i, 1); mbar_init(bar_re + 8 * i, 1); }
+        for (int i = 0; i < 2; i++) { mbar_init(bar_k + 8 * i, 4); mbar_init(bar_ke + 8 * i, 1); mbar_init(bar_v + 8 * i, 4); mbar_init(bar_ve + 8 * i, 1); }
+        mbar_init(bar_q, 8); mbar_init(bar_s, 1); mbar_init(bar_r, 4); mbar_init(bar_p, 4); mbar_init(bar_o, 1); mbar_init(bar_f, 1);
         *abort_flag = 0;
         fence_barrier_init();
     }
@@ -101,20 +117,24 @@ __global__ void __launch_bounds__(kF32Threads, 1) attn_paged_f32_kernel(const __
     auto wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_spin(bar, parity, abort_flag)) != 0; };
     if (b >= 0) {
     if (warp == 12) {
-        // lane w brings the pieces of the cutting warp w
-        const int c = lane & 3, rows = min(t.v_rows, a.dv - c * t.v_rows);
-        const uint32_t bytes = lane < 4 ? 16u * a.dk * 4u : (uint32_t)(rows * 256);
-        bool ok = lane < 4 || (lane < 8 && rows > 0);
-        int ids = 0;
+        // lane w brings what the cutting warp w has of a page, in two pieces
+        const int c = lane & 3, rows = lane < 4 ? 16 : lane < 8 ? max(min(t.v_rows, a.dv - c * t.v_rows), 0) : 0, half = lane < 4 ? 8 : t.v_rows / 2;
+        const int width = lane < 4 ? a.dk : kPage;
+        const float* from = lane < 4 ? (const float*)a.k + (long)c * 16 * a.dk : (const float*)a.v + (long)c * t.v_rows * kPage;
+        const long page_size = (long)a.G * kPage * (lane < 4 ? a.dk : a.dv), head = (long)g * kPage * (lane < 4 ? a.dk : a.dv);
+        bool ok = true;
+        int ids = 0, u = 0;
         for (int j = t0; j < t1; j++) {
-            const int n = j - t0, st = lane * 2 + (n & 1);
+            const int n = j - t0;
             if ((n & 31) == 0) ids = j + lane < t1 ? page_of(a.seq, b, j + lane) : 0;
-            const long at = ((long)__shfl_sync(0xffffffffu, ids, n & 31) * a.G + g) * kPage;
-            ok = ok && mbar_spin(bar_re + 8 * st, (uint32_t)(n >> 1 & 1) ^ 1u, abort_flag);
-            if (ok) {
-                mbar_expect_tx(bar_rf + 8 * st, bytes);
-                bulk_copy(base + o.raw + st * kPieceBytes, lane < 4 ? (const float*)a.k + (at + c * 16) * a.dk : (const float*)a.v + at * a.dv + (long)c * t.v_rows * kPage, bytes,
-                          bar_rf + 8 * st);
+            const float* src = from + __shfl_sync(0xffffffffu, ids, n & 31) * page_size + head;
+            for (int r = 0; r < rows; r += half, u++) {
+                const int slot = (lane << t.slots_log) + (u & ((1 << t.slots_log) - 1));
+                ok = ok && mbar_spin(bar_re + 8 * slot, (uint32_t)(u >> t.slots_log & 1) ^ 1u, abort_flag);
+                if (!ok) continue;
+                const uint32_t bytes = (uint32_t)(min(half, rows - r) * width) * 4u;
+                mbar_expect_tx(bar_rf + 8 * slot, bytes);
+                bulk_copy(base + o.raw + slot * kPieceBytes, src + r * width, bytes, bar_rf + 8 * slot);
             }
             __syncwarp();
         }
@@ -130,25 +150,27 @@ __global__ void __launch_bounds__(kF32Threads, 1) attn_paged_f32_kernel(const __
             pb = x == 0 ? 2u : x == 2 || x == 3 ? 1u : 0u;
         };
         auto qk = [&](int n) {
-            if (!wait(bar_k, (uint32_t)(n & 1))) return false;
+            const uint32_t st = n & t.two;
+            if (!wait(bar_k + 8 * st, (uint32_t)(n >> t.two & 1))) return false;
             if (n > 0 && !wait(bar_r, (uint32_t)(n - 1 & 1))) return false;      // the scores in front have been read
             tc_fence_after();
 #pragma unroll
             for (int x = 0; x < 6; x++) {
                 uint32_t pa, pb;
                 parts(x, pa, pb);
-                const uint32_t qa = u_tmem + 320 + pa * (uint32_t)t.kq * 16u, ka = k_lo + pb * (uint32_t)t.kc * 512u;
+                const uint32_t qa = u_tmem + 320 + pa * (uint32_t)t.kq * 16u, ka = k_lo + (st * 3u + pb) * (uint32_t)t.kc * 512u;
                 for (int k = 0; k < ksteps; k++) umma_bf16_ts_lo(leader, u_tmem, qa + 8 * k, ka + (k >> 2) * 512u + 2 * (k & 3), idesc_qk, x > 0 || k > 0);
             }
             umma_commit_by(leader, bar_s);
-            umma_commit_by(leader, bar_ke);
+            umma_commit_by(leader, bar_ke + 8 * st);
             return true;
         };
         bool ok = u0 < u1 && wait(bar_q, 0) && qk(0);
         for (int j = u0; ok && j < u1; j++) {
             const int n = j - u0;
+            const uint32_t st = n & t.two;
             if (j + 1 < u1 && !qk(n + 1)) break;          // under this page's softmax
-            ok = wait(bar_v, (uint32_t)(n & 1)) && wait(bar_p, (uint32_t)(n & 1));
+            ok = wait(bar_v + 8 * st, (uint32_t)(n >> t.two & 1)) && wait(bar_p, (uint32_t)(n & 1));
             if (!ok) break;
             tc_fence_after();
 #pragma unroll
@@ -157,10 +179,10 @@ __global__ void __launch_bounds__(kF32Threads, 1) attn_paged_f32_kernel(const __
                 parts(x, pa, pb);
 #pragma unroll
                 for (uint32_t k = 0; k < 4; k++)
-                    umma_bf16_ts_lo(leader, u_tmem + 192, u_tmem + 64 + 32 * pa + 8 * k, v_lo + pb * (uint32_t)t.vr * 8u + 2 * k, idesc_pv, n > 0 || x > 0 || k > 0);
+                    umma_bf16_ts_lo(leader, u_tmem + 192, u_tmem + 64 + 32 * pa + 8 * k, v_lo + (st * 3u + pb) * (uint32_t)t.vr * 8u + 2 * k, idesc_pv, n > 0 || x > 0 || k > 0);
             }
             umma_commit_by(leader, j + 1 < u1 ? bar_o : bar_f);           // the last one has a barrier of its own
-            umma_commit_by(leader, bar_ve);
+            umma_commit_by(leader, bar_ve + 8 * st);
         }
     } else if (warp >= 4) {
         // ---- numbers into parts: 8 of them per thread and piece
@@ -168,7 +190,7 @@ __global__ void __launch_bounds__(kF32Threads, 1) attn_paged_f32_kernel(const __
         uint4 part[3];
         auto put = [&](uint32_t at, uint32_t stride, int row, int c) {         // the 16 bytes c of a row of all parts; `at` the row's block
 #pragma unroll
-            for (int p = 0; p < 3; p++) *reinterpret_cast<uint4*>(base_ptr + at + p * stride + row * 128 + (((c ^ row) & 7) << 4)) = part[p];
+            for (int p = 0; p < 3; p++) store_shared(base + at + p * stride + row * 128 + (((c ^ row) & 7) << 4), part[p]);
         };
         const uint32_t k_part = (uint32_t)t.kc * 8192u, v_part = (uint32_t)t.vr * 128u;
         if (t0 < t1) {
@@ -192,7 +214,7 @@ __global__ void __launch_bounds__(kF32Threads, 1) attn_paged_f32_kernel(const __
             }
             if ((per & 1) && ct < kPage) {                // the last 16 elements of a product reach beyond the row: zeros in K
                 part[0] = part[1] = part[2] = make_uint4(0, 0, 0, 0);
-                put((uint32_t)(per >> 3) * 8192u, k_part, ct, per);
+                for (uint32_t st = 0; st <= (uint32_t)t.two; st++) put((st * 3u * t.kc + (uint32_t)(per >> 3)) * 8192u, k_part, ct, per);
             }
             fence_proxy_async_smem();
             tmem_st_wait();
@@ -200,46 +222,49 @@ __global__ void __launch_bounds__(kF32Threads, 1) attn_paged_f32_kernel(const __
             __syncwarp();
             if (lane == 0) mbar_arrive(bar_q);
         }
-        // warps 4 .. 7: 16 keys of K each, 8 .. 11: rows of V^T; each has its pieces to itself and goes through them without the others
-        const int w = warp - 4, c = w & 3, rows = min(t.v_rows, a.dv - c * t.v_rows), count = w < 4 ? 16 * per : rows * 8;
-        const uint32_t inv = 65535u / (uint32_t)per + 1u;         // e / per for e < 256
+        // warps 4 .. 7: 16 keys of K each, 8 .. 11: rows of V^T. A warp goes through its pieces without the others; a piece is in registers when the next
+        // one is asked for
+        const int w = warp - 4, c = w & 3, rows = w < 4 ? 16 : max(min(t.v_rows, a.dv - c * t.v_rows), 0), half = w < 4 ? 8 : t.v_rows / 2, wide = w < 4 ? per : 8;
+        const uint32_t inv = 65535u / (uint32_t)wide + 1u, raw_at = base + o.raw, flip = (uint32_t)(lane >> 2 & 1) * 16u;
+        const uint32_t full = w < 4 ? bar_k : bar_v, empty = w < 4 ? bar_ke : bar_ve;
         bool ok = true;
-        for (int j = t0; j < t1; j++) {
-            const int n = j - t0, left = end - j * kPage, st = w * 2 + (n & 1);
-            ok = wait(w < 4 ? bar_ke : bar_ve, (uint32_t)(n & 1) ^ 1u) && (count <= 0 || wait(bar_rf + 8 * st, (uint32_t)(n >> 1 & 1)));
-            if (!ok) break;
-            const float* src = (const float*)(base_ptr + o.raw + st * kPieceBytes);
-            for (int e0 = lane; e0 < count; e0 += 64) {
-                float f[2][8];
+        int u = 0;
+        for (int j = t0; ok && j < t1; j++) {
+            const int n = j - t0, left = end - j * kPage;
+            const uint32_t st = n & t.two, before = (uint32_t)(n >> t.two & 1) ^ 1u, to = w < 4 ? st * 3 * k_part : o.v + st * 3 * v_part;
+            if (rows == 0) ok = wait(empty + 8 * st, before);
+            for (int r = 0; ok && r < rows; r += half, u++) {
+                const int count = min(half, rows - r) * wide;      // of 8 numbers, at most 128
+                const int slot = (w << t.slots_log) + (u & ((1 << t.slots_log) - 1));
+                ok = wait(bar_rf + 8 * slot, (uint32_t)(u >> t.slots_log & 1));
+                if (!ok) break;
+                float f[4][8];
 #pragma unroll
-                for (int x = 0; x < 2; x++)
-                    if (e0 + 32 * x < count) load8(src + (e0 + 32 * x) * 8, f[x]);
+                for (int x = 0; x < 4; x++)
+                    if (lane + 32 * x < count) load8_shared(raw_at + slot * kPieceBytes + (lane + 32 * x) * 32, flip, f[x]);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar_re + 8 * slot);
+                if (r == 0) ok = wait(empty + 8 * st, before);
+                if (!ok) break;
 #pragma unroll
-                for (int x = 0; x < 2; x++) {
-                    const int e = e0 + 32 * x;
-                    if (e >= count) break;
-                    if (w < 4) {
-                        const int key = (int)(e * inv >> 16), col = e - key * per;
-                        cut8(f[x], part);
-                        put((uint32_t)(col >> 3) * 8192u, k_part, c * 16 + key, col);
-                    } else {
-                        // keys behind the sequence's last one were never written: zeros, so that a weight of zero stays without effect
-                        const int k8 = (e & 7) * 8;
-                        if (k8 + 8 > left)
+                for (int x = 0; x < 4; x++) {
+                    const int e = lane + 32 * x;
+                    if (e >= count) continue;
+                    const int row = (int)(e * inv >> 16), col = e - row * wide;
+                    // keys behind the sequence's last one were never written: zeros, so that a weight of zero stays without effect
+                    if (w >= 4 && col * 8 + 8 > left)
 #pragma unroll
-                            for (int y = 0; y < 8; y++)
-                                if (k8 + y >= left) f[x][y] = 0.0f;
-                        cut8(f[x], part);
-                        put(o.v, v_part, c * t.v_rows + (e >> 3), k8 >> 3);
-                    }
+                        for (int y = 0; y < 8; y++)
+                            if (col * 8 + y >= left) f[x][y] = 0.0f;
+                    cut8(f[x], part);
+                    if (w < 4) put(to + (uint32_t)(col >> 3) * 8192u, k_part, c * 16 + r + row, col);
+                    else put(to, v_part, c * t.v_rows + r + row, col);
                 }
             }
+            if (!ok) break;
             fence_proxy_async_smem();
             __syncwarp();
-            if (lane == 0) {
-                if (count > 0) mbar_arrive(bar_re + 8 * st);
-                mbar_arrive(w < 4 ? bar_k : bar_v);
-            }
+            if (lane == 0) mbar_arrive(full + 8 * st);
         }
     } else {
         // ---- one row per thread
@@ -295,18 +320,19 @@ __global__ void __launch_bounds__(kF32Threads, 1) attn_paged_f32_kernel(const __
                     }
                 }
             }
-            float sum[2] = {0.0f, 0.0f};
+            f32x2 sum = pack2(0.0f, 0.0f);
 #pragma unroll
             for (int c = 0; c < 2; c++) {
                 uint32_t pk[3][16];
 #pragma unroll
                 for (int x = 0; x < 32; x += 2) {
-                    float e0 = ex2_fast(__fmaf_rn(__uint_as_float(v[c][x]), t.a2, -m)), e1 = ex2_fast(__fmaf_rn(__uint_as_float(v[c][x + 1]), t.a2, -m));
-                    sum[0] += e0; sum[1] += e1;
+                    const float e0 = ex2_fast(__fmaf_rn(__uint_as_float(v[c][x]), t.a2, -m)), e1 = ex2_fast(__fmaf_rn(__uint_as_float(v[c][x + 1]), t.a2, -m));
+                    f32x2 e = pack2(e0, e1);
+                    sum = add2(sum, e);
 #pragma unroll
                     for (int p = 0; p < 3; p++) {
-                        pk[p][x >> 1] = bf_pack(e0, e1);
-                        e0 -= bf_lo(pk[p][x >> 1]); e1 -= bf_hi(pk[p][x >> 1]);
+                        pk[p][x >> 1] = near2(e);
+                        e = rest2(e, pk[p][x >> 1]);
                     }
                 }
                 if (c == 0 && n > 0) {                    // the weights in front have been read
@@ -317,7 +343,9 @@ __global__ void __launch_bounds__(kF32Threads, 1) attn_paged_f32_kernel(const __
                 for (int p = 0; p < 3; p++) tmem_st_32x16(tP + 32 * p + 16 * c + lane_addr, pk[p]);
             }
             if (!ok) break;
-            l += sum[0] + sum[1];
+            float s0, s1;
+            unpack2(sum, s0, s1);
+            l += s0 + s1;
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
@@ -402,7 +430,12 @@ int attn_paged_f32(const PagedAttn& a, cudaStream_t st) {
     if (ones * 16 * heads > 0x7fffffffL) return FLEXLLM_ENOTSUP;
     const long tiles = ((a.seq.T + seqs - 1) / seqs + t.TQ - 1) / t.TQ * seqs * heads;
     t.n_split = key_splits(tiles, false, (a.seq.max_ctx + kPage) / kPage, 2, 16);
-    const F32Smem o = f32_smem(t.kc, t.vr);
+    // two stages while four slots fit beside them, or two; heads of more than 96: one stage, and four slots, since what is on its way counts more
+    // (32 single tokens over 2000, heads of 128: 201 us against 211 with two stages and one slot)
+    auto fits = [&](int slots_log, int two) { return f32_smem(t.kc, t.vr, slots_log, two).total <= 226u * 1024u; };
+    t.two = fits(1, 1);
+    t.slots_log = fits(2, t.two) ? 2 : 1;
+    const F32Smem o = f32_smem(t.kc, t.vr, t.slots_log, t.two);
     if (o.total > 226u * 1024u || (128u * (a.dv + 4) + 256u + kJoinRows) * 4u > o.bars) return FLEXLLM_ENOTSUP;
     TRY_RC(allow_shared(attn_paged_f32_kernel, o.total));
     TRY_RC(allow_cluster(attn_paged_f32_kernel, t.n_split));
