@@ -2,14 +2,15 @@
 // each, which hold it to the last bit; a product is the six of nine products of parts that reach 2^-24 of it, summed in fp32. Six bf16 MMAs
 // are a quarter of what the same product takes the fp32 units.
 // A tile is 128 rows (tokens x the query heads of one key/value head), walked page by page with the running softmax of the bf16 kernel:
-//   warp 12        brings K and V^T of a page in pieces of 8 KB
-//   warps 4 .. 11  cut them into parts, in swizzled shared memory (Q at the start)
-//   warp 13        S = Q K^T and O += P V, P from TMEM
+//   warp 12        brings K and V^T of a page in pieces of up to 4 KB, a lane for each cutting warp
+//   warps 4 .. 11  cut them into parts, in swizzled shared memory (Q at the start, into TMEM)
+//   warp 13        S = Q K^T of the next page, then O += P V of this one; Q and P come from TMEM
 //   warps 0 .. 3   one row per thread: maximum, weights 2^(S scale log2 e - m) in three parts, sum
 // Few tiles: a cluster of CTAs cuts the keys.
-// A page's chain bounds it (pieces, parts, six MMAs per product, softmax; K and V have one place each, since three parts of two heads of 128 fill
-// shared memory), not the tensor cores, which run a fifth of the time: 16 tokens of four sequences over 3000, 16 / 4 heads of 128: 45 us; three prompts
-// of 380 behind 700, 8 / 2 heads of 64: 36 us; 4000 tokens, 32 / 8 heads of 128: 1.0 ms, 127 TFLOP/s, nearly twice what the fp32 units could.
+// Shared memory bounds it: for a page of heads of 128, 512 clocks of copies, 512 of reads and 768 of writes to cut it, 1536 of reads by the MMAs, and the cutting
+// waits for its turn in between; the tensor cores run a fifth of the time. 66 tokens of four sequences over 1350 to 3000, 16 / 4 heads of 128: 40 us;
+// three prompts of 380 behind 700, 8 / 2 heads of 64: 30 us; one token over 84500, one head of 128: 270 us; 1500 tokens behind 1000, 32 / 8 heads of 128:
+// 282 us, 139 TFLOP/s, nearly twice what the fp32 units could.
 #include "attention_join.cuh"
 
 namespace flexllm {
@@ -18,7 +19,7 @@ using namespace tc;
 
 namespace {
 
-constexpr int kF32Threads = 448, kMostSlots = 4;     // slots for pieces per cutting warp: 4, 2 or 1, as shared memory has room
+constexpr int kF32Threads = 448, kMostSlots = 4;     // slots for pieces per cutting warp: 4 or 2
 constexpr uint32_t kPieceBytes = 4096;
 
 struct F32Args {
