@@ -46,7 +46,7 @@ __global__ void __launch_bounds__(256, RT * NV <= 256 ? 2 : 1) attn_paged_simt_k
     pdl_sync();
     if (tid < 32) {
         const int TQ = sa.TQ;
-        const Unit u = find_unit(a.seq, tile / all, [TQ](const SeqRows& s) { return (s.n + TQ - 1) / TQ; });
+        const Unit u = find_unit(a.seq, tile / all, TQ, 1, [TQ](const SeqRows& s) { return (s.n + TQ - 1) / TQ; });
         if (tid == 0) { unit_sm = u; redo_sm[0] = redo_sm[1] = 0; }
     }
     __syncthreads();

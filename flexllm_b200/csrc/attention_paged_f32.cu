@@ -101,7 +101,7 @@ __global__ void __launch_bounds__(kF32Threads, 1) attn_paged_f32_kernel(const __
     const int tile = blockIdx.x / t.n_split, split = blockIdx.x % t.n_split, hg = tile % t.heads;
     if (warp == 0) {
         const int TQ = t.TQ;
-        const Unit u = find_unit(a.seq, tile / t.heads, [TQ](const SeqRows& s) { return (s.n + TQ - 1) / TQ; });
+        const Unit u = find_unit(a.seq, tile / t.heads, TQ, 1, [TQ](const SeqRows& s) { return (s.n + TQ - 1) / TQ; });
         if (lane == 0) unit_sm = u;
     }
     tc_fence_before();

@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(MODE == kOne ? 192 : 320, MODE == kOne ? 2 : 1
     const int tile = blockIdx.x / t.n_split, split = blockIdx.x % t.n_split, hg = tile % t.heads;
     if (warp == 0) {
         const int per = NQ * t.TQ;
-        const Unit u = find_unit(a.seq, tile / t.heads, [per](const SeqRows& s) { return (s.n + per - 1) / per; });
+        const Unit u = find_unit(a.seq, tile / t.heads, per, 1, [per](const SeqRows& s) { return (s.n + per - 1) / per; });
         if (lane == 0) unit_sm = u;
     }
     tc_fence_before();

@@ -75,8 +75,7 @@ template <class T, int L> __device__ __forceinline__ void rope_warp(const RopeAr
     };
     load(h0);
     // the sequence of the row: the last one that starts at or before it
-    int b = -1;
-    for (int b0 = 0; b0 < a.seq.B; b0 += 32) b += __popc(__ballot_sync(0xffffffffu, b0 + lane < a.seq.B && a.seq.cu[b0 + lane] <= t));
+    const int b = count_below(a.seq.B, [&](int i) { return a.seq.cu[i] <= t; }) - 1;
     Four co = all_four(1.0f), si = all_four(0.0f);         // the other elements do not turn
     bool outside = false;                                  // an error only if the row is a sequence's
     if (turns) {
@@ -149,7 +148,7 @@ template <class T, int L> __global__ void __launch_bounds__(256, 4) qk_norm_rope
     }
     const int id = blockIdx.x - a.qk_ctas, g = id % a.G, tid = threadIdx.x;
     if (tid < 32) {
-        const Unit u = find_unit(a.seq, id / a.G, [](const SeqRows& s) { return (s.ctx + s.n - 1) / kPage - s.ctx / kPage + 1; });
+        const Unit u = find_unit(a.seq, id / a.G, kPage, 2, [](const SeqRows& s) { return (s.ctx + s.n - 1) / kPage - s.ctx / kPage + 1; });
         if (tid == 0) unit_sm = u;
     }
     __syncthreads();
@@ -191,7 +190,8 @@ template <class T, int L> int launch_rope(RopeArgs& a, cudaStream_t st) {
     a.chunks = (a.H + a.G + kRopeHeads - 1) / kRopeHeads;
     const long qk = ((long)a.seq.T * a.chunks + 7) / 8;
     // a sequence's first row opens a page, the next one another, and so does every 64th
-    const long seqs = a.seq.B < a.seq.T ? a.seq.B : a.seq.T, next = a.seq.T - seqs, units = seqs + (next + (kPage - 1) * (next < seqs ? next : seqs)) / kPage;
+    const long seqs = a.seq.B < a.seq.T ? a.seq.B : a.seq.T, next = a.seq.T - seqs,
+               units = a.seq.B > kLookThrough ? a.seq.T / kPage + 2L * a.seq.B : seqs + (next + (kPage - 1) * (next < seqs ? next : seqs)) / kPage;
     if (qk + units * a.G > 0x7fffffffL || qk > 0x1fffffffL) return FLEXLLM_ENOTSUP;      // warps are counted in 32 bits
     a.qk_ctas = (int)qk;
     const size_t smem = (size_t)kPage * (a.dv * sizeof(T) + 4);

@@ -326,3 +326,57 @@ def test_keys_cut_into_any_number_of_parts(ops, dtype, H, G, dim, new, ctx):
         got = ops.attn_packed(q, *args) if m is None else ops.attn_tree(q, m.cuda(), *args)
         want, far = pc.attention(q, k, v, table, start, cx, dim ** -0.5, m)
         assert ((got.double() - want).abs() <= far).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF], ids=["f32", "bf16"])
+@pytest.mark.parametrize("B,most,H,G", [(65, 1, 4, 2), (300, 3, 8, 2), (130, 70, 3, 1), (1500, 2, 2, 1)])
+def test_many_sequences(ops, dtype, B, most, H, G):
+    """More sequences than are looked through one by one: with and without rows, over pages that are begun, full and crossed."""
+    g = torch.Generator().manual_seed(B)
+    new = [int(x) for x in torch.randint(0, most + 1, (B,), generator=g)] if most > 1 else [1] * B
+    ctx = [int(x) for x in torch.randint(0, 130, (B,), generator=g)]
+    table, start, cx, n_pages = pc.layout(new, ctx, seed=1)
+    T, dim = sum(new) + 3, 64                                           # three rows that are nobody's
+    gd = torch.Generator(device="cuda").manual_seed(2)
+    r = lambda *n: torch.randn(n, generator=gd, device="cuda").to(dtype)
+    k, v, proj = r(n_pages, G, 64, dim), r(n_pages, G, dim, 64), r(T, (H + 2 * G) * dim)
+    one = torch.ones((1, dim // 2), device="cuda")
+    args = (table.cuda(), start.cuda(), cx.cuda())
+    k0, v0 = k.clone(), v.clone()
+    q = ops.qk_norm_rope(proj, H, torch.zeros(T, dtype=torch.int32, device="cuda"), one, one * 0, k, v, *args)
+    x = proj.view(T, -1, dim)
+    assert torch.equal(q[:T - 3], x[:T - 3, :H].reshape(T - 3, -1))
+    row = 0
+    for b in range(B):
+        for i in range(new[b]):
+            page, slot = int(table[b, (ctx[b] + i) // 64]), (ctx[b] + i) % 64
+            k0[page, :, slot], v0[page, :, :, slot] = x[row, H:H + G], x[row, H + G:]
+            row += 1
+    assert torch.equal(k, k0) and torch.equal(v, v0)
+    out = torch.full((T, H * dim), 7.0, device="cuda", dtype=dtype)
+    ops.attn_packed(q.view(T, H, dim), k, v, *args, out=out)
+    want, far = pc.attention(q.view(T, H, dim), k, v, table, start, cx, dim ** -0.5)
+    assert ((out.double() - want).abs() <= far)[:T - 3].all() and (out[T - 3:] == 7).all()
+    from flexllm_b200 import lib
+    assert lib().flexllm_device_status() == 0
+    bad = start.clone()
+    bad[B // 2] = T + 40                                                # a start behind the rows, then one that falls
+    ops.attn_packed(q.view(T, H, dim), k, v, args[0], bad.cuda(), args[2])
+    assert lib().flexllm_device_status() == -7
+
+
+def test_captured_first_and_in_many_parts(ops):
+    """A call in 16 parts, captured and replayed for another context than it was captured with."""
+    g = torch.Generator(device="cuda").manual_seed(1)
+    k, v = torch.randn((300, 1, 64, 128), generator=g, device="cuda").to(BF), torch.randn((300, 1, 128, 64), generator=g, device="cuda").to(BF)
+    q = torch.randn((1, 8, 128), generator=g, device="cuda").to(BF)
+    table, cu, ctx = torch.arange(300, device="cuda", dtype=torch.int32)[None].contiguous(), i32(0, 1), i32(19000)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        y = ops.attn_packed(q, k, v, table, cu, ctx)
+    for c in (19000, 5, 12345, 0):
+        ctx.fill_(c)
+        graph.replay()
+        want, far = pc.attention(q, k, v, table.cpu(), cu.cpu(), ctx.cpu(), 128 ** -0.5)
+        assert ((y.double() - want).abs() <= far).all()
