@@ -1,4 +1,4 @@
-// Products with 4-bit weights, one scale and zero point per group of the inner index:
+// Products with 4-bit weights, one scale and zero point per group of the inner index, for up to 8 tokens:
 //   y[m][n] = sum_groups s[n][g] * sum_{k in g} a[m][k] (q[n][k] - z[n][g])
 // HBM bound for few tokens: half a byte per weight. Weights stream from memory into the registers of the lanes that multiply them: a warp has
 // 16 rows on the 16-row side of bf16 warp MMAs and 8 tokens per MMA on the other. q - z is an integer of five bits, exact in bf16, and sums
@@ -9,7 +9,7 @@
 // subtraction of 128 + z). The inner index may go through the MMA in any order, the same one in both operands: a lane's words are as they lie
 // in memory, and the activations follow (16 bytes at a time on their way into shared memory, pairs when they are read).
 // Measured: one token, 8192 x 2048, 7.1 us (launch, first words, joining K); 128256 x 2048, 43 us, 3.0 TB/s, where unpacking fills the math pipes; fp32
-// activations: one token 8192 x 2048 9.0 us, 16 tokens 19 us, 64 tokens 68 us.
+// activations: one token 8192 x 2048 9.0 us.
 #include "linear_w4.h"
 
 namespace flexllm {
@@ -23,8 +23,7 @@ struct W4Args : W4Call {
     int steps, chunks;                     // steps of kStep elements per staged chunk of activations (a multiple of ks), chunks
 };
 constexpr int kStep = 128;
-// warps of a CTA: with many tokens fewer of them, with more registers each
-template <int MT> constexpr int kWarps = MT <= 2 ? 16 : 8;
+constexpr int kWarps = 16;                 // of a CTA
 
 template <int VW> struct Words { uint32_t v[VW]; };
 template <int VW> __device__ __forceinline__ Words<VW> load_words(const uint8_t* p) {
@@ -38,25 +37,6 @@ template <int VW> __device__ __forceinline__ Words<VW> load_words(const uint8_t*
 // 8 bf16 activations k .. k + 7 as the pairs (0,4) (1,5) (2,6) (3,7)
 __device__ __forceinline__ uint4 pairs(const uint4& v) {
     return make_uint4(pick(v.x, v.z, 0x5410), pick(v.x, v.z, 0x7632), pick(v.y, v.w, 0x5410), pick(v.y, v.w, 0x7632));
-}
-// 8 fp32 activations as such pairs of their three parts
-struct Eight { uint4 part[3]; };
-__device__ __forceinline__ Eight eight(const float* p) {
-    float f[8];
-    load8(p, f);
-    Eight r;
-#pragma unroll
-    for (int k = 0; k < 3; k++) {
-        r.part[k] = make_uint4(bf_pack(f[0], f[4]), bf_pack(f[1], f[5]), bf_pack(f[2], f[6]), bf_pack(f[3], f[7]));
-        const uint32_t w[4] = {r.part[k].x, r.part[k].y, r.part[k].z, r.part[k].w};
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-            // what the part leaves; nothing of an infinity or NaN (the first part carries it)
-            f[j] = fabsf(f[j]) <= 3.0e38f ? f[j] - bf_lo(w[j]) : 0.0f;
-            f[j + 4] = fabsf(f[j + 4]) <= 3.0e38f ? f[j + 4] - bf_hi(w[j]) : 0.0f;
-        }
-    }
-    return r;
 }
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
@@ -72,20 +52,19 @@ __device__ __forceinline__ void mma_bf16_first(float (&d)[4], uint32_t a0, uint3
 // A step is 128 elements of 32 rows (two MMA tiles, which share the activations' operands): four words per lane and row, U blocks of VW words (a quad of lanes covers the 32 VW elements of a block, which
 // are of one group). A CTA's warps are ks along K, the others along the rows; the tokens' activations are staged in chunks, two in shared
 // memory, and serve all its rows. Where one chunk holds them all, a CTA goes on with further rows. Weights, scales and zero points are asked
-// for D steps ahead, over the end of a chunk and of the rows. MT tiles of 8 tokens.
-// In shared memory 32 elements, those of one word of a quad's lanes, lie together for all tokens: [chunk][8 MT tokens][64 bytes], so that eight
+// for D steps ahead, over the end of a chunk and of the rows.
+// In shared memory 32 elements, those of one word of a quad's lanes, lie together for all tokens: [chunk][8 tokens][64 bytes], so that eight
 // lanes read 128 bytes in a row and every address but the step's is a constant.
 // PACKED: K of whole steps, a group per block, bf16 scales: a step's scales and zero points come in one load each.
-template <class T, int VW, int MT, bool PACKED>
-__global__ void __launch_bounds__(kWarps<MT> * 32, 1) linear_w4_kernel(const __grid_constant__ W4Args p) {
-    constexpr int PL = sizeof(T) == 2 ? 1 : 3, NW = kWarps<MT>;
+template <class T, int VW, bool PACKED>
+__global__ void __launch_bounds__(kWarps * 32, 1) linear_w4_kernel(const __grid_constant__ W4Args p) {
+    constexpr int PL = sizeof(T) == 2 ? 1 : 3, NW = kWarps;
     constexpr int BK = 32 * VW, U = 4 / VW;                // elements of a block, blocks per step
     constexpr int D = 2;
-    constexpr int XC = 8 * MT * 64, XS = 4 * XC;           // bytes of 32 elements of all tokens, of a step
+    constexpr int XC = 8 * 64, XS = 4 * XC;           // bytes of 32 elements of all tokens, of a step
     constexpr int SW = PACKED ? (U + 1) / 2 : U, ZW = PACKED ? 1 : U;
     extern __shared__ __align__(16) uint8_t x_sm[];        // [2][PL][steps] XS
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, lr = lane >> 2, lc = lane & 3;
-    const int m0 = blockIdx.y * 64, Mb = min(p.M - m0, 8 * MT);
     const int kw = warp & (p.ks - 1), per_cta = NW / p.ks, rows = 32 * per_cta, r0 = 32 * (warp / p.ks);
     const int groups = p.K / p.group, plane = p.steps * XS;
     // a step's words, scales and zero points of this lane's four rows, as they are in memory: a conversion here would wait for the load
@@ -160,17 +139,19 @@ __global__ void __launch_bounds__(kWarps<MT> * 32, 1) linear_w4_kernel(const __g
         const int n = min(kc, p.K - chunk * kc) / BK, piece = lane % LT, c = piece / VW, j = piece % VW;
         uint8_t* to = x_sm + (chunk & 1) * PL * plane + j * XC + (lane / LT) * 64 + c * 16;
         const int k = chunk * kc + piece * 8;
-        for (int e = warp; e < n * (8 * MT / TW); e += NW) {
-            const int b = e / (8 * MT / TW), mt = (e - b * (8 * MT / TW)) * TW, m = mt + lane / LT;
-            if (m < Mb) f(to + b * VW * XC + mt * 64, m, k + b * BK);
+        for (int e = warp; e < n * (8 / TW); e += NW) {
+            const int b = e / (8 / TW), mt = (e - b * (8 / TW)) * TW, m = mt + lane / LT;
+            if (m < p.M) f(to + b * VW * XC + mt * 64, m, k + b * BK);
         }
     };
     auto stage = [&](int chunk) {
         pieces(chunk, [&](uint8_t* to, int m, int k) {
-            const T* src = (const T*)p.a + (long)(m0 + m) * p.lda + k;
+            const T* src = (const T*)p.a + (long)m * p.lda + k;
             if (PL == 1) copy16((uint32_t)__cvta_generic_to_shared(to), src);
             else {
-                const Eight x = eight((const float*)src);
+                float f[8];
+                load8((const float*)src, f);
+                const Eight x = eight(f);
 #pragma unroll
                 for (int q = 0; q < 3; q++) *reinterpret_cast<uint4*>(to + q * plane) = x.part[q];
             }
@@ -182,21 +163,19 @@ __global__ void __launch_bounds__(kWarps<MT> * 32, 1) linear_w4_kernel(const __g
         asm volatile("cp.async.wait_group 0;" ::: "memory");
         if (PL == 1) pieces(chunk, [&](uint8_t* at, int, int) { *reinterpret_cast<uint4*>(at) = pairs(*reinterpret_cast<const uint4*>(at)); });
     };
-    float acc[2][MT][4];
+    float acc[2][4];
     auto clear = [&] {
 #pragma unroll
         for (int h = 0; h < 2; h++)
 #pragma unroll
-            for (int t = 0; t < MT; t++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) acc[h][t][i] = 0.0f;
+            for (int i = 0; i < 4; i++) acc[h][i] = 0.0f;
     };
     // one step of the warp: elements k0 .. of its rows, activations at xb
     auto multiply = [&](const Step& cur, int k0, const uint8_t* xb) {
 #pragma unroll
         for (int u = 0; u < U; u++) {
             if (!PACKED && k0 + u * BK >= p.K) break;
-            float sc[4], part[2][MT][4];
+            float sc[4], part[2][4];
             uint32_t z[4];
 #pragma unroll
             for (int r = 0; r < 4; r++) { z[r] = zero_of(cur.z[r], u); sc[r] = scale_of(cur.s[r], u); }
@@ -207,33 +186,22 @@ __global__ void __launch_bounds__(kWarps<MT> * 32, 1) linear_w4_kernel(const __g
                 for (int r = 0; r < 4; r++)
 #pragma unroll
                     for (int i = 0; i < 4; i++) a[r][i] = weights2(cur.w[r][u].v[j], i, z[r]);
-                // all tiles of tokens in turn, so that a product does not wait for the one in front
 #pragma unroll
-                for (int q = 0; q < PL; q++)
+                for (int q = 0; q < PL; q++) {
+                    const uint4 x = *reinterpret_cast<const uint4*>(xb + q * plane + (u * VW + j) * XC);
 #pragma unroll
-                    for (int t0 = 0; t0 < MT; t0 += 4) {
-                        uint4 x[4];
-#pragma unroll
-                        for (int t = t0; t < t0 + 4 && t < MT; t++) x[t - t0] = *reinterpret_cast<const uint4*>(xb + q * plane + (u * VW + j) * XC + t * 512);
-#pragma unroll
-                        for (int t = t0; t < t0 + 4 && t < MT; t++)
-#pragma unroll
-                            for (int h = 0; h < 2; h++) {
-                                if (j == 0 && q == 0) mma_bf16_first(part[h][t], a[2 * h][0], a[2 * h + 1][0], a[2 * h][1], a[2 * h + 1][1], x[t - t0].x, x[t - t0].y);
-                                else mma_bf16(part[h][t], a[2 * h][0], a[2 * h + 1][0], a[2 * h][1], a[2 * h + 1][1], x[t - t0].x, x[t - t0].y);
-                            }
-#pragma unroll
-                        for (int t = t0; t < t0 + 4 && t < MT; t++)
-#pragma unroll
-                            for (int h = 0; h < 2; h++) mma_bf16(part[h][t], a[2 * h][2], a[2 * h + 1][2], a[2 * h][3], a[2 * h + 1][3], x[t - t0].z, x[t - t0].w);
+                    for (int h = 0; h < 2; h++) {
+                        if (j == 0 && q == 0) mma_bf16_first(part[h], a[2 * h][0], a[2 * h + 1][0], a[2 * h][1], a[2 * h + 1][1], x.x, x.y);
+                        else mma_bf16(part[h], a[2 * h][0], a[2 * h + 1][0], a[2 * h][1], a[2 * h + 1][1], x.x, x.y);
                     }
+#pragma unroll
+                    for (int h = 0; h < 2; h++) mma_bf16(part[h], a[2 * h][2], a[2 * h + 1][2], a[2 * h][3], a[2 * h + 1][3], x.z, x.w);
+                }
             }
 #pragma unroll
-            for (int t = 0; t < MT; t++)
+            for (int h = 0; h < 2; h++)
 #pragma unroll
-                for (int h = 0; h < 2; h++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) acc[h][t][i] = __fmaf_rn(part[h][t][i], sc[2 * h + (i >> 1)], acc[h][t][i]);
+                for (int i = 0; i < 4; i++) acc[h][i] = __fmaf_rn(part[h][i], sc[2 * h + (i >> 1)], acc[h][i]);
         }
     };
     // the warps' parts of K, joined in their order; [ks][tokens][rows of the CTA + 4], behind the activations when these are needed again
@@ -244,27 +212,25 @@ __global__ void __launch_bounds__(kWarps<MT> * 32, 1) linear_w4_kernel(const __g
 #pragma unroll
         for (int h = 0; h < 2; h++)
 #pragma unroll
-            for (int t = 0; t < MT; t++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int m = t * 8 + 2 * lc + (i & 1);
-                    if (m < Mb) red[(kw * Mb + m) * red_row + r0 + 16 * h + lr + 8 * (i >> 1)] = acc[h][t][i];
-                }
+            for (int i = 0; i < 4; i++) {
+                const int m = 2 * lc + (i & 1);
+                if (m < p.M) red[(kw * p.M + m) * red_row + r0 + 16 * h + lr + 8 * (i >> 1)] = acc[h][i];
+            }
         __syncthreads();
-        for (int e0 = tid; e0 < Mb * rows; e0 += 4 * NW * 32) {
+        for (int e0 = tid; e0 < p.M * rows; e0 += 4 * NW * 32) {
             float v[4];
 #pragma unroll
             for (int x = 0; x < 4; x++) {
-                const int e = min(e0 + x * NW * 32, Mb * rows - 1), at = (e >> p.rows_log) * red_row + (e & (rows - 1));
+                const int e = min(e0 + x * NW * 32, p.M * rows - 1), at = (e >> p.rows_log) * red_row + (e & (rows - 1));
                 v[x] = 0.0f;
-                for (int k = 0; k < p.ks; k++) v[x] += red[k * Mb * red_row + at];
+                for (int k = 0; k < p.ks; k++) v[x] += red[k * p.M * red_row + at];
             }
 #pragma unroll
             for (int x = 0; x < 4; x++) {
                 const int e = e0 + x * NW * 32, m = e >> p.rows_log, n = tile * rows + (e & (rows - 1));
-                if (m >= Mb || n >= p.N) continue;
+                if (m >= p.M || n >= p.N) continue;
                 if (p.bias) v[x] += p.bias[n];
-                const long at = (long)(m0 + m) * p.ldy + n;
+                const long at = (long)m * p.ldy + n;
                 if (p.y_f32) ((float*)p.y)[at] = v[x];
                 else ((T*)p.y)[at] = from_f<T>(v[x]);
             }
@@ -305,8 +271,8 @@ __global__ void __launch_bounds__(kWarps<MT> * 32, 1) linear_w4_kernel(const __g
         }
 }
 
-template <class T, int VW, int MT, bool PACKED> int launch_w4(W4Args& p, cudaStream_t st) {
-    constexpr int NW = kWarps<MT>, PL = sizeof(T) == 2 ? 1 : 3, per_step = PL * 8 * MT * 2 * kStep;       // bytes of activations
+template <class T, int VW, bool PACKED> int launch_w4(W4Args& p, cudaStream_t st) {
+    constexpr int NW = kWarps, PL = sizeof(T) == 2 ? 1 : 3, per_step = PL * 8 * 2 * kStep;       // bytes of activations
     const int all = (p.K + kStep - 1) / kStep;             // steps of a row
     p.per_group = p.group / (32 * VW);
     p.magic = (uint32_t)(((1ull << 32) + p.per_group - 1) / p.per_group);
@@ -315,7 +281,7 @@ template <class T, int VW, int MT, bool PACKED> int launch_w4(W4Args& p, cudaStr
     const long tiles = (p.N + 31) / 32, sms = gemm_sm_count();
     while (p.ks < NW && 2 * p.ks <= all && (tiles * 2 * p.ks + NW - 1) / NW <= sms) p.ks *= 2;
     // all activations at once, or two chunks in turn
-    const int tokens = p.M < 8 * MT ? p.M : 8 * MT, red = NW * 36 * tokens * 4, room = 220 * 1024;
+    const int red = NW * 36 * p.M * 4, room = 220 * 1024;
     int steps = (room - red) / per_step;
     if (steps < all) steps = room / 2 / per_step;
     while (p.ks > steps) p.ks /= 2;
@@ -326,26 +292,19 @@ template <class T, int VW, int MT, bool PACKED> int launch_w4(W4Args& p, cudaStr
     const size_t smem = p.chunks > 1 ? (2 * x_bytes > red ? 2 * x_bytes : red) : x_bytes + red;
     const int per_cta = NW / p.ks;
     for (p.rows_log = 5; 32 * per_cta > 1 << p.rows_log;) p.rows_log++;
-    auto kern = linear_w4_kernel<T, VW, MT, PACKED>;
+    auto kern = linear_w4_kernel<T, VW, PACKED>;
     TRY_RC(allow_shared(kern, smem));
     long ctas = (tiles + per_cta - 1) / per_cta;
     if (p.chunks == 1 && ctas > sms) ctas = sms;
-    launch_k(kern, dim3((unsigned)ctas, (p.M + 63) / 64), dim3(NW * 32), smem, st, p);
+    launch_k(kern, dim3((unsigned)ctas), dim3(NW * 32), smem, st, p);
     return launch_status();
 }
 bool packed_groups(const W4Args& p, int block) { return !p.scale_f32 && p.group == block && p.K % kStep == 0 && aligned(p.scale, 8) && aligned(p.zero, 4); }
-template <int VW> int run_w4(W4Args& p, const bf16*, cudaStream_t st) {
-    return packed_groups(p, 32 * VW) ? launch_w4<bf16, VW, 1, true>(p, st) : launch_w4<bf16, VW, 1, false>(p, st);
-}
-template <int VW> int run_w4(W4Args& p, const float*, cudaStream_t st) {
-    if (p.M <= 8) return packed_groups(p, 32 * VW) ? launch_w4<float, VW, 1, true>(p, st) : launch_w4<float, VW, 1, false>(p, st);
-    if (p.M <= 32) return launch_w4<float, VW, 4, false>(p, st);
-    return launch_w4<float, VW, 8, false>(p, st);
-}
+template <class T, int VW> int run_w4(W4Args& p, cudaStream_t st) { return packed_groups(p, 32 * VW) ? launch_w4<T, VW, true>(p, st) : launch_w4<T, VW, false>(p, st); }
 template <class T> int pick_w4(W4Args& p, cudaStream_t st) {
-    if (p.group % 128 == 0) return run_w4<4>(p, (const T*)p.a, st);
-    if (p.group % 64 == 0) return run_w4<2>(p, (const T*)p.a, st);
-    return run_w4<1>(p, (const T*)p.a, st);
+    if (p.group % 128 == 0) return run_w4<T, 4>(p, st);
+    if (p.group % 64 == 0) return run_w4<T, 2>(p, st);
+    return run_w4<T, 1>(p, st);
 }
 
 }  // namespace
@@ -358,16 +317,19 @@ extern "C" int flexllm_linear_w4(int dtype, const void* a, long lda, const uint8
                                  const float* bias, int M, int N, int K, void* y, long ldy, int y_f32, void* stream) {
     FLEXLLM_REQUIRE((dtype == FLEXLLM_F32 || dtype == FLEXLLM_BF16) && (scale_dtype == FLEXLLM_F32 || scale_dtype == FLEXLLM_BF16));
     FLEXLLM_REQUIRE(M >= 0 && N > 0 && K > 0 && group > 0 && group % 32 == 0 && K % group == 0 && lda >= K && lda % 8 == 0 && ldy >= N);
-    if ((M + 63) / 64 > 65535 || K > 1 << 20) return FLEXLLM_ENOTSUP;
+    if ((M + 31) / 32 > 65535 || K > 1 << 20) return FLEXLLM_ENOTSUP;
     if (M == 0) return FLEXLLM_OK;
     FLEXLLM_REQUIRE(a && w && scale && y && aligned(a, 16) && aligned(w, 16) && aligned(scale, scale_dtype == FLEXLLM_F32 ? 4 : 2) && aligned(bias, 4) &&
                     aligned(y, y_f32 || dtype == FLEXLLM_F32 ? 4 : 2));
     const W4Call c = {a, lda, w, scale, scale_dtype == FLEXLLM_F32, zero, group, bias, M, N, K, y, ldy, y_f32 != 0};
     const SetUpEarly early;
-    // the tensor cores for more than 8 tokens (16 x 8192 x 2048: 9.1 us), and for more than 2 where K is long and one wave has all rows: each CTA there has a
-    // part of K (4 x 2048 x 8192: 10.6 us against 13.6; 8 x 8192 x 8192: 21.2 against 26.6; 8 x 128256 x 2048: 79 against 49)
-    if (dtype == FLEXLLM_BF16 && (M > 8 || (M > 2 && K >= 4096 && N <= 128L * gemm_sm_count()))) return linear_w4_tc(c, (cudaStream_t)stream);
+    // the tensor cores for more than 8 tokens (16 x 8192 x 2048: 9.1 us, fp32 11.8), and for more than 2 (fp32: any) where K is long and one wave has all rows: each CTA
+    // there has a part of K (4 x 2048 x 8192: 10.6 us against 13.6, fp32 13.9 against 17.8; 1 x 1024 x 4096 in fp32: 8.2
+    // against 17.3; 8 x 8192 x 8192: 21.2 against 26.6, but fp32 31 against 28;
+    // 8 x 128256 x 2048: 79 against 49)
+    const bool f32 = dtype == FLEXLLM_F32;
+    if (M > 8 || ((M > 2 || f32) && K >= 4096 && N <= (f32 ? 32L : 128L) * gemm_sm_count())) return linear_w4_tc(c, f32, (cudaStream_t)stream);
     W4Args p = {};
     static_cast<W4Call&>(p) = c;
-    return dtype == FLEXLLM_BF16 ? pick_w4<bf16>(p, (cudaStream_t)stream) : pick_w4<float>(p, (cudaStream_t)stream);
+    return f32 ? pick_w4<float>(p, (cudaStream_t)stream) : pick_w4<bf16>(p, (cudaStream_t)stream);
 }

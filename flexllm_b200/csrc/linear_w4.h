@@ -1,4 +1,4 @@
-// Products with 4-bit weights: the call, shared by its kernels (linear_w4.cu: few tokens and fp32, linear_w4_tc.cu: tensor cores).
+// Products with 4-bit weights: the call, shared by its kernels (linear_w4.cu: few tokens, linear_w4_tc.cu: tensor cores).
 #pragma once
 #include "float_common.cuh"
 
@@ -14,7 +14,25 @@ struct W4Call {
     int M, N, K;
     void* y; long ldy; int y_f32;
 };
-int linear_w4_tc(const W4Call& c, cudaStream_t st);      // bf16
+int linear_w4_tc(const W4Call& c, bool f32, cudaStream_t st);
+
+// 8 fp32 activations as the pairs (0,4) (1,5) (2,6) (3,7) of their three bf16 parts
+struct Eight { uint4 part[3]; };
+__device__ __forceinline__ Eight eight(float (&f)[8]) {
+    Eight r;
+#pragma unroll
+    for (int k = 0; k < 3; k++) {
+        r.part[k] = make_uint4(bf_pack(f[0], f[4]), bf_pack(f[1], f[5]), bf_pack(f[2], f[6]), bf_pack(f[3], f[7]));
+        const uint32_t w[4] = {r.part[k].x, r.part[k].y, r.part[k].z, r.part[k].w};
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            // what the part leaves; nothing of an infinity or NaN (the first part carries it)
+            f[j] = fabsf(f[j]) <= 3.0e38f ? f[j] - bf_lo(w[j]) : 0.0f;
+            f[j + 4] = fabsf(f[j + 4]) <= 3.0e38f ? f[j + 4] - bf_hi(w[j]) : 0.0f;
+        }
+    }
+    return r;
+}
 
 __device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t mask, uint32_t bits) {
     uint32_t r;
