@@ -459,7 +459,8 @@ int attn_paged_tc(const PagedAttn& a, cudaStream_t st) {
     t.q_block = most * 128u;
     const long pairs = most_units(a.seq, 2 * t.TQ), ones = most_units(a.seq, t.TQ);
     t.heads = (int)heads;
-    if (ones * 16 * heads > 0x7fffffffL) return FLEXLLM_ENOTSUP;
+    // rows of the pages are counted in 31 bits
+    if (ones * 16 * heads > 0x7fffffffL || (long)a.seq.n_pages * a.G * (a.dv > kPage ? a.dv : kPage) > 0x7fffffffL) return FLEXLLM_ENOTSUP;
     const long sms = gemm_sm_count(), tiles = (each + t.TQ - 1) / t.TQ * seqs * heads;      // if all sequences are of equal length
     const int pages = (a.seq.max_ctx + kPage) / kPage;
     t.n_split = 1;

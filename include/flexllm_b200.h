@@ -481,8 +481,9 @@ FLEXLLM_API int flexllm_qk_norm_rope(int dtype, const flexllm_kv_pages* kv, int 
                                      int T, void* q, long ldq, void* stream);
 
 /* Causal attention of the packed rows over their sequences' pages, which hold the keys and values of all their positions (the new ones
- * included): row i of sequence b sees the positions 0 .. ctx[b] + i. heads a multiple of hkv. q [T][ldq] (heads side by side, row stride a
- * multiple of 16 bytes), out [T][ldo], scale >= 0. What a row does not see has no influence on it, not finite values included. */
+ * included): row i of sequence b sees the positions 0 .. ctx[b] + i. heads a multiple of hkv; in bf16 n_pages * hkv *
+ * the larger of 64 and vdim below 2^31. q [T][ldq] (heads side by side, row stride a multiple of 16 bytes), out [T][ldo], scale >= 0. What a
+ * row does not see has no influence on it, not finite values included. */
 FLEXLLM_API int flexllm_attn_packed(int dtype, const flexllm_kv_pages* kv, int heads, float scale, const void* q, long ldq, const int32_t* cu,
                                     const int32_t* ctx, const int32_t* page_table, int max_pages, int max_ctx, int B, int T, void* out, long ldo,
                                     void* stream);

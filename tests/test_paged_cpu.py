@@ -53,6 +53,7 @@ def test_attention_sizes(lib):
     assert lib.flexllm_attn_tree(_lib.BF16, C.byref(pages()), 4, 0.125, P, 256, None, P, P, P, 4, 255, 2, 3, P, 256, None) == EINVAL
     for kdim, vdim in ((60, 64), (64, 60), (264, 64), (64, 264)):
         assert attention(lib, kv=pages(kdim=kdim, vdim=vdim), ldq=4096, ldo=4096) == ENOTSUP
+    assert attention(lib, T=3, kv=pages(n_pages=1 << 26)) == ENOTSUP                   # rows of pages beyond 31 bits
 
 
 def rope(lib, **change):
