@@ -698,7 +698,8 @@ extern "C" int flexllm_kv_cache_create(flexllm_kv_cache** out, int layers, int n
         return e == cudaErrorMemoryAllocation ? FLEXLLM_ENOMEM : FLEXLLM_ECUDA;
     }
     *out = c;
-    return flexllm_kv_cache_reset(c, nullptr);
+    TRY_RC(flexllm_kv_cache_reset(c, nullptr));
+    return wait_cleared();
 }
 
 // Floating-point flavour: one pool pair per layer, each with its own shape (256-byte aligned inside two allocations).
@@ -728,7 +729,8 @@ extern "C" int flexllm_kv_cache_create_float(flexllm_kv_cache** out, int layers,
         return e == cudaErrorMemoryAllocation ? FLEXLLM_ENOMEM : FLEXLLM_ECUDA;
     }
     *out = c;
-    return flexllm_kv_cache_reset(c, nullptr);
+    TRY_RC(flexllm_kv_cache_reset(c, nullptr));
+    return wait_cleared();
 }
 
 int flexllm::kv_cache_add_states(flexllm_kv_cache* c, int slots, const std::vector<size_t>& slot_bytes) {
@@ -742,7 +744,8 @@ int flexllm::kv_cache_add_states(flexllm_kv_cache* c, int slots, const std::vect
     if (n == 0) return FLEXLLM_OK;
     const cudaError_t e = cudaMalloc(&c->states, n);
     if (e != cudaSuccess) { g_last_cuda_error = (int)e; return e == cudaErrorMemoryAllocation ? FLEXLLM_ENOMEM : FLEXLLM_ECUDA; }
-    return cuda_status(cudaMemset(c->states, 0, n));
+    FLEXLLM_CHECK_CUDA(cudaMemset(c->states, 0, n));
+    return wait_cleared();
 }
 
 extern "C" int flexllm_kv_cache_destroy(flexllm_kv_cache* c) {

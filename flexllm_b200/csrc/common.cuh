@@ -32,6 +32,8 @@ inline int cuda_status(cudaError_t e) {
     g_last_cuda_error = (int)e;
     return FLEXLLM_ECUDA;
 }
+// Memory that the library makes is cleared on the null stream, which has no order with a caller's non-blocking streams: its maker returns when it is clear.
+inline int wait_cleared() { return cuda_status(cudaStreamSynchronize(nullptr)); }
 // Lets launches of `kern` ask for `bytes` of dynamic shared memory. A function's limit belongs to the (function, device) and so to every host thread
 // and every model of the process: it is raised once, to the most that the device has, and never set to the size of one call, which would lower it
 // between another thread's setting and its launch, or under a plan made earlier. Up to 40 KB need nothing (48 KB with the static part).

@@ -1009,6 +1009,7 @@ int mega_create(const MegaModelView& v, MegaPlan** out) {
         e = cudaMalloc(&p->dev_trace, p->trace_bytes);
         if (e == cudaSuccess) e = cudaMemset(p->dev_trace, 0, p->trace_bytes);
     }
+    if (e == cudaSuccess) e = cudaStreamSynchronize(nullptr);      // the step's counters are zero before any stream's kernel counts
     if (e != cudaSuccess) {
         mega_destroy(p);
         g_last_cuda_error = (int)e;

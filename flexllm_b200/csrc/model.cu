@@ -232,6 +232,7 @@ int flexllm::runner_create(flexllm_model** out, const flexllm_model_config& cfg,
     if (!rc) rc = dmalloc(m, &m->x, x_floats);
     if (!rc) rc = cuda_status(cudaMemset(m->x, 0, x_floats * 4));
     if (!rc) rc = flexllm_model_reset(m, nullptr);
+    if (!rc) rc = wait_cleared();
     if (rc) { flexllm_model_destroy(m); return rc; }
     *out = m;
     return FLEXLLM_OK;

@@ -217,7 +217,7 @@ FLEXLLM_API int flexllm_mha_i8xi8_prefill_online(const int8_t* q, const float* q
 /* ---------------------------------------------------------------------------------------------
  * Paged int8 KV cache (replaces dec_K_cache_manager / dec_V_cache_manager and their scale caches,
  * Modules/MHA.h:393-559, :713-851). One pool per layer set: pages of `page` tokens;
- * K,V pages [n_pages][HKV][page][64] s8, scale pages [n_pages][HKV][page] fp32, per layer.
+ * K,V pages [n_pages][HKV][page][64] s8, scale pages [n_pages][HKV][page] fp32, per layer. A cache is clear when its maker returns, on every stream.
  * ------------------------------------------------------------------------------------------- */
 typedef struct flexllm_kv_cache flexllm_kv_cache;
 FLEXLLM_API int flexllm_kv_cache_create(flexllm_kv_cache** out, int layers, int n_pages, int hkv, int page);
