@@ -79,6 +79,7 @@ __global__ void __launch_bounds__(256, RT * NV <= 256 ? 2 : 1) attn_paged_simt_k
             if (on) copy16(q_sm + row * DP + c, (const float*)a.q + (long)(s.row0 + i) * a.ldq + (long)(h0 + row % sa.RC) * a.dk + c);
             else store4(q_sm + row * DP + c, make_float4(0.0f, 0.0f, 0.0f, 0.0f));
     }
+    copies_commit();                      // also where this part has no page: the wait at the end covers what was committed
     // page ids are asked for a page ahead: the copies of a page would wait for its id
     int next_page = t_beg < t_end ? page_of(a.seq, b, t_beg) : 0;
     auto load_page = [&](int t) {
