@@ -1,16 +1,22 @@
 // Attention of packed rows over their sequences' pages in fp32, on the tensor cores (heads up to 128). A number is the sum of three bf16 parts of eight bits
 // each, which hold it to the last bit; a product is the six of nine products of parts that reach 2^-24 of it, summed in fp32. Six bf16 MMAs
 // are a quarter of what the same product takes the fp32 units.
+// An MMA cuts its fp32 sums instead of rounding them: half a step on average, for every 16 products. So the sums in TMEM are short, the small products
+// first and the large ones of one page last, and the pages' outputs are added up by fp32 units, rounded (all pages in one sum in TMEM:
+// 5e-5 low after 10,000 keys, 5e-4 after 80,000).
 // A tile is 128 rows (tokens x the query heads of one key/value head), walked page by page with the running softmax of the bf16 kernel:
-//   warp 12        brings K and V^T of a page in pieces of up to 4 KB, a lane for each cutting warp
+//   warps 12, 14   bring K and V^T of a page in pieces of up to 4 KB, a lane for each cutting warp (one warp for both would hold the one back for
+//                  the other: with two slots, heads of 128, a fifth slower)
 //   warps 4 .. 11  cut them into parts, in swizzled shared memory (Q at the start, into TMEM)
-//   warp 13        S = Q K^T of the next page, then O += P V of this one; Q and P come from TMEM
-//   warps 0 .. 3   one row per thread: maximum, weights 2^(S scale log2 e - m) in three parts, sum
+//   warp 13        S = Q K^T of the next page, then P V of this one; Q and P come from TMEM
+//   warps 0 .. 3   one row per thread: maximum, weights 2^(S scale log2 e - m) in three parts, sums of the weights and of the pages' outputs. The latter
+//                  are in TMEM, or in shared memory where the columns are taken (heads of more than 96). (Held in registers by the cutting warps,
+//                  whose code is left too few: 10 to 20 % slower)
 // Few tiles: a cluster of CTAs cuts the keys.
-// Shared memory bounds it: for a page of heads of 128, 512 clocks of copies, 512 of reads and 768 of writes to cut it, 1536 of reads by the MMAs, and the cutting
-// waits for its turn in between; the tensor cores run a fifth of the time. 66 tokens of four sequences over 1350 to 3000, 16 / 4 heads of 128: 40 us;
-// three prompts of 380 behind 700, 8 / 2 heads of 64: 30 us; one token over 84500, one head of 128: 270 us; 1500 tokens behind 1000, 32 / 8 heads of 128:
-// 282 us, 139 TFLOP/s, nearly twice what the fp32 units could.
+// Shared memory bounds it: for a page of heads of 128, 512 clocks of copies, 512 of reads and 768 of writes to cut it, 1536 of reads by the MMAs, 1024 for the
+// sums of a full tile, and the cutting waits for its turn in between; the tensor cores run a fifth of the time. 66 tokens of four sequences over 1350 to 3000,
+// 16 / 4 heads of 128: 46 us; three prompts of 380 behind 280 to 700, 8 / 2 heads of 64: 32 us; one token over 84500, one head of 128: 290 us; 1500 tokens
+// behind 1000, 32 / 8 heads of 128: 324 us, 130 TFLOP/s, nearly twice what the fp32 units could. The rounded sums cost 7 to 10 % of these times.
 #include "attention_join.cuh"
 
 namespace flexllm {
@@ -19,7 +25,7 @@ using namespace tc;
 
 namespace {
 
-constexpr int kF32Threads = 448, kMostSlots = 4;     // slots for pieces per cutting warp: 4 or 2
+constexpr int kF32Threads = 480, kMostSlots = 4;     // slots for pieces per cutting warp: 4 or 2
 constexpr uint32_t kPieceBytes = 4096;
 
 struct F32Args {
@@ -27,17 +33,24 @@ struct F32Args {
     int RC, HC, TQ, heads;                 // heads per tile, head chunks per group, tokens per tile, head chunks
     int kc, kq, vr, n_split;               // 128-byte blocks of a part's K row, 32-element chunks of a Q row, rows of a V^T part
     int v_rows, slots_log, two;            // rows of V^T of a cutting warp; its slots; K's and V's parts have two stages (1) or one (0)
+    int x_log, sum_at;                     // log2 of the buffers of a page's outputs in TMEM; column of the sums, 0: in shared memory
     float a2;                              // scale * log2 e
 };
-struct F32Smem { uint32_t v, raw, bars, total; };      // K's parts, V's, pieces
-__host__ __device__ inline F32Smem f32_smem(int kc, int vr, int slots_log, int two) {
+struct F32Smem { uint32_t v, raw, sums, bars, total; };      // K's parts, V's, pieces, the outputs' sums
+__host__ __device__ inline F32Smem f32_smem(int kc, int vr, int slots_log, int two, bool sums) {
     F32Smem o;
     o.v = (3u << two) * kc * 8192u;
     o.raw = o.v + (3u << two) * vr * 128u;
-    o.bars = o.raw + (8u << slots_log) * kPieceBytes;
+    o.sums = o.raw + (8u << slots_log) * kPieceBytes;
+    o.bars = o.sums + (sums ? (uint32_t)(vr + 31) / 32 * 32 * 512u : 0u);
     o.total = o.bars + 1024u + 1024u;
     return o;
 }
+
+// TMEM: S, P, then the outputs of a page (one or two buffers), their sums where there is room, Q at the end
+constexpr uint32_t kPCol = 64, kXCol = 160;
+__host__ __device__ inline uint32_t q_col(int kq) { return 512u - 48u * (uint32_t)kq; }
+__host__ __device__ inline uint32_t x_stride(int vr) { return (uint32_t)(vr + 31) / 32 * 32; }
 
 // Two numbers less what is nearest to them in bf16, which is `w`: exact
 __device__ __forceinline__ f32x2 rest2(f32x2 f, uint32_t w) { return fma2(pack2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)), pack2(-1.0f, -1.0f), f); }
@@ -81,17 +94,17 @@ __global__ void __launch_bounds__(kF32Threads, 1) attn_paged_f32_kernel(const __
     const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
     uint8_t* base_ptr = smem_raw + (base - raw);
     const PagedAttn& a = t.a;
-    const F32Smem o = f32_smem(t.kc, t.vr, t.slots_log, t.two);
+    const F32Smem o = f32_smem(t.kc, t.vr, t.slots_log, t.two, t.sum_at == 0);
     uint64_t* bars = reinterpret_cast<uint64_t*>(base_ptr + o.bars);
     const uint32_t bar_rf = smem_u32(bars), bar_re = bar_rf + 64 * kMostSlots, bar_q = bar_re + 64 * kMostSlots, bar_k = bar_q + 8, bar_ke = bar_k + 16, bar_v = bar_ke + 16,
-                   bar_ve = bar_v + 16, bar_s = bar_ve + 16, bar_r = bar_s + 8, bar_p = bar_r + 8, bar_o = bar_p + 8, bar_f = bar_o + 8;
+                   bar_ve = bar_v + 16, bar_s = bar_ve + 16, bar_r = bar_s + 8, bar_p = bar_r + 8, bar_o = bar_p + 8, bar_x = bar_o + 8;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 96);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (threadIdx.x == 0) {
         for (int i = 0; i < 8 * kMostSlots; i++) { mbar_init(bar_rf + 8 * i, 1); mbar_init(bar_re + 8 * i, 1); }
-        for (int i = 0; i < 2; i++) { mbar_init(bar_k + 8 * i, 4); mbar_init(bar_ke + 8 * i, 1); mbar_init(bar_v + 8 * i, 4); mbar_init(bar_ve + 8 * i, 1); }
-        mbar_init(bar_q, 8); mbar_init(bar_s, 1); mbar_init(bar_r, 4); mbar_init(bar_p, 4); mbar_init(bar_o, 1); mbar_init(bar_f, 1);
+        for (int i = 0; i < 2; i++) { mbar_init(bar_k + 8 * i, 4); mbar_init(bar_ke + 8 * i, 1); mbar_init(bar_v + 8 * i, 4); mbar_init(bar_ve + 8 * i, 1); mbar_init(bar_x + 8 * i, 4); }
+        mbar_init(bar_q, 8); mbar_init(bar_s, 1); mbar_init(bar_r, 4); mbar_init(bar_p, 4); mbar_init(bar_o, 1);
         *abort_flag = 0;
         fence_barrier_init();
     }
@@ -108,7 +121,7 @@ __global__ void __launch_bounds__(kF32Threads, 1) attn_paged_f32_kernel(const __
     __syncthreads();
     tc_fence_after();
     pdl_launch();                                         // behind the allocation: no later kernel may hold the TMEM that this one waits for
-    const uint32_t tmem = *tmem_slot, tP = tmem + 64, tO = tmem + 192, tQ = tmem + 320;      // S at the start
+    const uint32_t tmem = *tmem_slot, tP = tmem + kPCol, tX = tmem + kXCol, tQ = tmem + q_col(t.kq);      // S at the start
     const int b = unit_sm.b;
     const SeqRows s = unit_sm.s;
     const int R = a.H / a.G, g = hg / t.HC, h0 = g * R + (hg % t.HC) * t.RC, heads = min(t.RC, (g + 1) * R - h0);
@@ -117,12 +130,13 @@ __global__ void __launch_bounds__(kF32Threads, 1) attn_paged_f32_kernel(const __
     const int t0 = (int)((long)n_pg * split / t.n_split), t1 = (int)((long)n_pg * (split + 1) / t.n_split);
     auto wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_spin(bar, parity, abort_flag)) != 0; };
     if (b >= 0) {
-    if (warp == 12) {
-        // lane w brings what the cutting warp w has of a page, in two pieces
-        const int c = lane & 3, rows = lane < 4 ? 16 : lane < 8 ? max(min(t.v_rows, a.dv - c * t.v_rows), 0) : 0, half = lane < 4 ? 8 : t.v_rows / 2;
-        const int width = lane < 4 ? a.dk : kPage;
-        const float* from = lane < 4 ? (const float*)a.k + (long)c * 16 * a.dk : (const float*)a.v + (long)c * t.v_rows * kPage;
-        const long page_size = (long)a.G * kPage * (lane < 4 ? a.dk : a.dv), head = (long)g * kPage * (lane < 4 ? a.dk : a.dv);
+    if (warp == 12 || warp == 14) {
+        // lane w brings what the cutting warp w (K) or w + 4 (V) has of a page, in two pieces
+        const bool keys = warp == 12;
+        const int c = lane & 3, rows = lane >= 4 ? 0 : keys ? 16 : max(min(t.v_rows, a.dv - c * t.v_rows), 0), half = keys ? 8 : t.v_rows / 2;
+        const int width = keys ? a.dk : kPage;
+        const float* from = keys ? (const float*)a.k + (long)c * 16 * a.dk : (const float*)a.v + (long)c * t.v_rows * kPage;
+        const long page_size = (long)a.G * kPage * (keys ? a.dk : a.dv), head = (long)g * kPage * (keys ? a.dk : a.dv);
         bool ok = true;
         int ids = 0, u = 0;
         for (int j = t0; j < t1; j++) {
@@ -130,7 +144,7 @@ __global__ void __launch_bounds__(kF32Threads, 1) attn_paged_f32_kernel(const __
             if ((n & 31) == 0) ids = j + lane < t1 ? page_of(a.seq, b, j + lane) : 0;
             const float* src = from + __shfl_sync(0xffffffffu, ids, n & 31) * page_size + head;
             for (int r = 0; r < rows; r += half, u++) {
-                const int slot = (lane << t.slots_log) + (u & ((1 << t.slots_log) - 1));
+                const int slot = ((keys ? lane : lane + 4) << t.slots_log) + (u & ((1 << t.slots_log) - 1));
                 ok = ok && mbar_spin(bar_re + 8 * slot, (uint32_t)(u >> t.slots_log & 1) ^ 1u, abort_flag);
                 if (!ok) continue;
                 const uint32_t bytes = (uint32_t)(min(half, rows - r) * width) * 4u;
@@ -159,7 +173,7 @@ __global__ void __launch_bounds__(kF32Threads, 1) attn_paged_f32_kernel(const __
             for (int x = 0; x < 6; x++) {
                 uint32_t pa, pb;
                 parts(x, pa, pb);
-                const uint32_t qa = u_tmem + 320 + pa * (uint32_t)t.kq * 16u, ka = k_lo + (st * 3u + pb) * (uint32_t)t.kc * 512u;
+                const uint32_t qa = u_tmem + q_col(t.kq) + pa * (uint32_t)t.kq * 16u, ka = k_lo + (st * 3u + pb) * (uint32_t)t.kc * 512u;
                 for (int k = 0; k < ksteps; k++) umma_bf16_ts_lo(leader, u_tmem, qa + 8 * k, ka + (k >> 2) * 512u + 2 * (k & 3), idesc_qk, x > 0 || k > 0);
             }
             umma_commit_by(leader, bar_s);
@@ -169,9 +183,10 @@ __global__ void __launch_bounds__(kF32Threads, 1) attn_paged_f32_kernel(const __
         bool ok = u0 < u1 && wait(bar_q, 0) && qk(0);
         for (int j = u0; ok && j < u1; j++) {
             const int n = j - u0;
-            const uint32_t st = n & t.two;
+            const uint32_t st = n & t.two, xb = n & ((1 << t.x_log) - 1), before = n >> t.x_log;
             if (j + 1 < u1 && !qk(n + 1)) break;          // under this page's softmax
             ok = wait(bar_v + 8 * st, (uint32_t)(n >> t.two & 1)) && wait(bar_p, (uint32_t)(n & 1));
+            ok = ok && (before == 0 || wait(bar_x + 8 * xb, before - 1 & 1));      // the outputs that were in this buffer have been added up
             if (!ok) break;
             tc_fence_after();
 #pragma unroll
@@ -180,12 +195,12 @@ __global__ void __launch_bounds__(kF32Threads, 1) attn_paged_f32_kernel(const __
                 parts(x, pa, pb);
 #pragma unroll
                 for (uint32_t k = 0; k < 4; k++)
-                    umma_bf16_ts_lo(leader, u_tmem + 192, u_tmem + 64 + 32 * pa + 8 * k, v_lo + (st * 3u + pb) * (uint32_t)t.vr * 8u + 2 * k, idesc_pv, n > 0 || x > 0 || k > 0);
+                    umma_bf16_ts_lo(leader, u_tmem + kXCol + xb * x_stride(t.vr), u_tmem + kPCol + 32 * pa + 8 * k, v_lo + (st * 3u + pb) * (uint32_t)t.vr * 8u + 2 * k, idesc_pv, x > 0 || k > 0);
             }
-            umma_commit_by(leader, j + 1 < u1 ? bar_o : bar_f);           // the last one has a barrier of its own
+            umma_commit_by(leader, bar_o);
             umma_commit_by(leader, bar_ve + 8 * st);
         }
-    } else if (warp >= 4) {
+    } else if (warp >= 4 && warp < 12) {
         // ---- numbers into parts: 8 of them per thread and piece
         const int ct = threadIdx.x - 128, per = a.dk / 8;
         uint4 part[3];
@@ -267,7 +282,7 @@ __global__ void __launch_bounds__(kF32Threads, 1) attn_paged_f32_kernel(const __
             __syncwarp();
             if (lane == 0) mbar_arrive(full + 8 * st);
         }
-    } else {
+    } else if (warp < 4) {
         // ---- one row per thread
         const int row = threadIdx.x;
         const uint32_t lane_addr = (uint32_t)(warp * 32) << 16;
@@ -275,7 +290,40 @@ __global__ void __launch_bounds__(kF32Threads, 1) attn_paged_f32_kernel(const __
         const bool live = row < t.TQ * t.RC && i < s.n && hr < heads;
         const int sure = live ? sure_keys(a, s, i) : 0x40000000;
         const unsigned long long bits = live ? mask_bits(a, s, i) : 0ull;
-        float m = kNoScore, l = 0.0f;
+        const bool busy = __any_sync(0xffffffffu, live);                                  // other warps' rows are nowhere read
+        float m = kNoScore, l = 0.0f, al = 0.0f;
+        // sums in shared memory: rows of whole 128 bytes, their 16-byte pieces turned by the row, so that eight lanes meet all banks once
+        float* const sums = reinterpret_cast<float*>(base_ptr + o.sums) + (uint32_t)row * x_stride(t.vr);
+        auto piece = [&](int d) { return sums + ((((uint32_t)d >> 2) ^ ((uint32_t)row & 7u)) << 2); };
+        const uint32_t tSum = tmem + t.sum_at + lane_addr;
+        // sums = sums * f + outputs of page n
+        auto add_page = [&](int n, float f) {
+            const int xb = n & ((1 << t.x_log) - 1);
+            if (busy) {
+                for (int d = 0; d < t.vr; d += 16) {
+                    uint32_t u[16], v[16];
+                    tmem_ld_32x16(tX + xb * x_stride(t.vr) + d + lane_addr, u);
+                    if (n > 0) {
+                        if (t.sum_at) tmem_ld_32x16(tSum + d, v);
+                        else
+#pragma unroll
+                            for (int x = 0; x < 16; x += 4) *reinterpret_cast<uint4*>(v + x) = *reinterpret_cast<const uint4*>(piece(d + x));
+                    }
+                    tmem_ld_wait();
+                    if (n > 0)
+#pragma unroll
+                        for (int x = 0; x < 16; x++) u[x] = __float_as_uint(__fmaf_rn(__uint_as_float(v[x]), f, __uint_as_float(u[x])));
+                    if (t.sum_at) tmem_st_32x16(tSum + d, u);
+                    else
+#pragma unroll
+                        for (int x = 0; x < 16; x += 4) *reinterpret_cast<uint4*>(piece(d + x)) = *reinterpret_cast<const uint4*>(u + x);
+                }
+                tmem_st_wait();
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_x + 8 * xb);
+        };
         bool ok = true;
         for (int j = t0; j < t1; j++) {
             const int n = j - t0;
@@ -302,25 +350,9 @@ __global__ void __launch_bounds__(kF32Threads, 1) attn_paged_f32_kernel(const __
                 mx = max3(mx, __uint_as_float(v[0][x]), __uint_as_float(v[1][x]));
                 my = max3(my, __uint_as_float(v[0][x + 1]), __uint_as_float(v[1][x + 1]));
             }
-            const float top = fmaxf(mx, my) * t.a2;
-            const bool grow = top > m + kSlack;
-            if (__any_sync(0xffffffffu, grow)) {
-                const float m_new = grow ? top : m, al = ex2_fast(m - m_new);
-                m = m_new;
-                l *= al;
-                if (n > 0) {
-                    if (!wait(bar_o, (uint32_t)((n - 1) & 1))) { ok = false; break; }
-                    tc_fence_after();
-                    for (int d = 0; d < t.vr; d += 16) {
-                        uint32_t u[16];
-                        tmem_ld_32x16(tO + d + lane_addr, u);
-                        tmem_ld_wait();
-#pragma unroll
-                        for (int x = 0; x < 16; x++) u[x] = __float_as_uint(__uint_as_float(u[x]) * al);
-                        tmem_st_32x16(tO + d + lane_addr, u);
-                    }
-                }
-            }
+            const float top = fmaxf(mx, my) * t.a2, m_new = top > m + kSlack ? top : m, al_n = ex2_fast(m - m_new);
+            m = m_new;
+            l *= al_n;
             f32x2 sum = pack2(0.0f, 0.0f);
 #pragma unroll
             for (int c = 0; c < 2; c++) {
@@ -351,11 +383,14 @@ __global__ void __launch_bounds__(kF32Threads, 1) attn_paged_f32_kernel(const __
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(bar_p);
+            if (n > 0) add_page(n - 1, al);               // under the products with this page
+            al = al_n;
         }
         const bool any = t0 < t1;
-        if (ok && any) ok = wait(bar_f, 0);
+        if (ok && any) ok = wait(bar_o, (uint32_t)((t1 - t0 - 1) & 1));
         if (ok) {
             tc_fence_after();
+            if (any) add_page(t1 - t0 - 1, al);
             const float rl = t.n_split > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
             bool odd = false;
             float* orow = reinterpret_cast<float*>(base_ptr) + (long)row * (a.dv + 4);
@@ -363,9 +398,12 @@ __global__ void __launch_bounds__(kF32Threads, 1) attn_paged_f32_kernel(const __
             const bool vec = whole_stores<float>(a);
             for (int d0 = 0; d0 < t.vr; d0 += 16) {
                 uint32_t u[16];
-                if (any) {
-                    tmem_ld_32x16(tO + d0 + lane_addr, u);
+                if (any && t.sum_at) {
+                    tmem_ld_32x16(tSum + d0, u);
                     tmem_ld_wait();
+                } else if (any) {
+#pragma unroll
+                    for (int x = 0; x < 16; x += 4) *reinterpret_cast<uint4*>(u + x) = *reinterpret_cast<const uint4*>(piece(d0 + x));
                 } else {
 #pragma unroll
                     for (int x = 0; x < 16; x++) u[x] = 0;
@@ -431,13 +469,16 @@ int attn_paged_f32(const PagedAttn& a, cudaStream_t st) {
     if (ones * 16 * heads > 0x7fffffffL) return FLEXLLM_ENOTSUP;
     const long tiles = ((a.seq.T + seqs - 1) / seqs + t.TQ - 1) / t.TQ * seqs * heads;
     t.n_split = key_splits(tiles, false, (a.seq.max_ctx + kPage) / kPage, 2, 16);
-    // two stages while four slots fit beside them, or two; heads of more than 96: one stage, and four slots, since what is on its way counts more
-    // (32 single tokens over 2000, heads of 128: 201 us against 211 with two stages and one slot)
-    auto fits = [&](int slots_log, int two) { return f32_smem(t.kc, t.vr, slots_log, two).total <= 226u * 1024u; };
+    // the sums of the outputs in TMEM where a page's outputs leave room, twice, so that the next page's products need not wait for the addition, or once
+    const uint32_t xs = x_stride(t.vr), room = q_col(t.kq) - kXCol;
+    t.x_log = 2 * xs + t.vr <= room;
+    t.sum_at = (1u << t.x_log) * xs + t.vr <= room ? kXCol + (xs << t.x_log) : 0;
+    // two stages while two slots fit beside them; four slots where they fit
+    auto fits = [&](int slots_log, int two) { return f32_smem(t.kc, t.vr, slots_log, two, t.sum_at == 0).total <= 226u * 1024u; };
     t.two = fits(1, 1);
     t.slots_log = fits(2, t.two) ? 2 : 1;
-    const F32Smem o = f32_smem(t.kc, t.vr, t.slots_log, t.two);
-    if (o.total > 226u * 1024u || (128u * (a.dv + 4) + 256u + kJoinRows) * 4u > o.bars) return FLEXLLM_ENOTSUP;
+    const F32Smem o = f32_smem(t.kc, t.vr, t.slots_log, t.two, t.sum_at == 0);
+    if (o.total > 226u * 1024u || (128u * (a.dv + 4) + 256u + kJoinRows) * 4u > o.sums) return FLEXLLM_ENOTSUP;
     TRY_RC(allow_shared(attn_paged_f32_kernel, o.total));
     TRY_RC(allow_cluster(attn_paged_f32_kernel, t.n_split));
     launch_cluster(attn_paged_f32_kernel, dim3((unsigned)(ones * t.n_split * heads)), dim3(kF32Threads), t.n_split, o.total, st, t);
