@@ -5,7 +5,7 @@
 // of them per thread, two partial sums each (even and odd elements) in packed fp32 pairs. A row's 16 threads are half a warp, so that its weights
 // change hands without a barrier; the next page comes in under this one's products where shared memory holds two.
 // Few tiles: a cluster of CTAs cuts the keys, and its partial maxima, sums and outputs meet in shared memory.
-// Bound by the fp32 units and the reads of shared memory that feed them: 8 / 2 heads of 256, two prompts of 750 behind 500: 399 us, 26 TFLOP/s; four trees
+// Bound by the fp32 units and the reads of shared memory that feed them: 8 / 2 heads of 256, two prompts of 750 behind 500: 422 us, 25 TFLOP/s; four trees
 // of 25 over 3000: 153 us.
 #include "attention_paged.cuh"
 #include "tc_common.cuh"
@@ -172,22 +172,35 @@ __global__ void __launch_bounds__(256, RT * NV <= 256 ? 2 : 1) attn_paged_simt_k
             for (int j = 0; j < NV; j++) acc[r][j] = mul2(acc[r][j], al2);
         }
         __syncwarp();                                     // a row's weights are read by the half warp that wrote them
+        // a page's keys in sums of their own: thousands of terms one after the other in one sum would cost it digits
         by_rows([&](auto rows) {
-            constexpr int L = decltype(rows)::value;
+            constexpr int L = decltype(rows)::value, NJ = NV > 8 ? 8 : NV;
+#pragma unroll
+            for (int j0 = 0; j0 < NV; j0 += NJ) {
+                f32x2 part[L][NJ];
+#pragma unroll
+                for (int r = 0; r < L; r++)
+#pragma unroll
+                    for (int j = 0; j < NJ; j++) part[r][j] = pack2(0.0f, 0.0f);
 #pragma unroll 4
-            for (int c = 0; c < kPage; c += 4) {
-                float4 pv[L];
+                for (int c = 0; c < kPage; c += 4) {
+                    float4 pv[L];
 #pragma unroll
-                for (int r = 0; r < L; r++) pv[r] = load4(p_sm + (ty + 16 * r) * PPITCH + c);
+                    for (int r = 0; r < L; r++) pv[r] = load4(p_sm + (ty + 16 * r) * PPITCH + c);
 #pragma unroll
-                for (int j = 0; j < NV; j++) {
-                    const float4 vv = load4(v_sm + (tx + 16 * j) * PPITCH + c);
+                    for (int j = 0; j < NJ; j++) {
+                        const float4 vv = load4(v_sm + (tx + 16 * (j0 + j)) * PPITCH + c);
 #pragma unroll
-                    for (int r = 0; r < L; r++) {
-                        acc[r][j] = fma2(pack2(pv[r].x, pv[r].y), pack2(vv.x, vv.y), acc[r][j]);
-                        acc[r][j] = fma2(pack2(pv[r].z, pv[r].w), pack2(vv.z, vv.w), acc[r][j]);
+                        for (int r = 0; r < L; r++) {
+                            part[r][j] = fma2(pack2(pv[r].x, pv[r].y), pack2(vv.x, vv.y), part[r][j]);
+                            part[r][j] = fma2(pack2(pv[r].z, pv[r].w), pack2(vv.z, vv.w), part[r][j]);
+                        }
                     }
                 }
+#pragma unroll
+                for (int r = 0; r < L; r++)
+#pragma unroll
+                    for (int j = 0; j < NJ; j++) acc[r][j0 + j] = add2(acc[r][j0 + j], part[r][j]);
             }
         });
         __syncwarp();

@@ -16,7 +16,7 @@
 // Shared memory bounds it: for a page of heads of 128, 512 clocks of copies, 512 of reads and 768 of writes to cut it, 1536 of reads by the MMAs, 1024 for the
 // sums of a full tile, and the cutting waits for its turn in between; the tensor cores run a fifth of the time. 66 tokens of four sequences over 1350 to 3000,
 // 16 / 4 heads of 128: 46 us; three prompts of 380 behind 280 to 700, 8 / 2 heads of 64: 32 us; one token over 84500, one head of 128: 290 us; 1500 tokens
-// behind 1000, 32 / 8 heads of 128: 324 us, 130 TFLOP/s, nearly twice what the fp32 units could. The rounded sums cost 7 to 10 % of these times.
+// behind 1000, 32 / 8 heads of 128: 324 us, 133 TFLOP/s, nearly twice what the fp32 units could. The rounded sums cost 7 to 10 % of these times.
 #include "attention_join.cuh"
 
 namespace flexllm {

@@ -24,7 +24,7 @@ def test_keys_cut_over_the_device(ops, keys, dim, vdim, mean, sharp):
     check(ops, q[None], k[:, None], v[:, None], [0])
 
 
-@pytest.mark.parametrize("dim,vdim", [(64, 64), (128, 128), (96, 40)])
+@pytest.mark.parametrize("dim,vdim", [(64, 64), (128, 128), (96, 40), (200, 64), (136, 136)])
 @pytest.mark.parametrize("keys,mean,sharp", [(1000, 1.0, False), (10000, 1.0, False), (10000, 1.0, True), (10000, 0.0, False)])
 def test_keys_of_many_heads_in_one_part(ops, dim, vdim, keys, mean, sharp):
     """More heads than SMs: nobody cuts their keys."""
