@@ -6,7 +6,7 @@
 namespace flexllm {
 
 constexpr float kSlack = 8.0f;             // log2 units by which a score may exceed its row's shift
-constexpr float kNoScore = -1e30f;
+constexpr float kNoScore = -1e30f;         // where a row's shift starts: weights of scores below it are zero, and a row of such scores is computed key by key
 
 __device__ __forceinline__ void store8f(bf16* p, const float (&f)[8], bool vec) {
     if (vec) *reinterpret_cast<uint4*>(p) = make_uint4(bf_pack(f[0], f[1]), bf_pack(f[2], f[3]), bf_pack(f[4], f[5]), bf_pack(f[6], f[7]));
@@ -54,6 +54,7 @@ __device__ __forceinline__ void join_parts(const PagedAttn& a, const SeqRows& s,
                 if (p0 + p < parts) { sum = __fmaf_rn(lk[p], ex2_fast(mk[p] - top), sum); w_sm[(p0 + p) * mine + e] = mk[p]; }
         }
         const float r = sum == 0.0f ? 0.0f : 1.0f / sum;
+        if (sum == 0.0f && row % RC < heads && sees_any(a, s, i0 + row / RC)) atomicOr(&redo_sm[row >> 5], 1u << (row & 31));
         for (int p = 0; p < parts; p++) w_sm[p * mine + e] = sum == 0.0f ? 0.0f : ex2_fast(w_sm[p * mine + e] - top) * r;
     }
     __syncthreads();

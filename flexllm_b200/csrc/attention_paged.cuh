@@ -29,8 +29,10 @@ __device__ __forceinline__ bool sees_key(int key, int sure, unsigned long long b
     return key < sure || (unsigned)(key - ctx) < 64u && ((bits >> (key - ctx)) & 1u);
 }
 
+__device__ __forceinline__ bool sees_any(const PagedAttn& a, const SeqRows& s, int i) { return sure_keys(a, s, i) > 0 || mask_bits(a, s, i) != 0; }
 // One row, key by key, by a whole warp. Rows come here whose result was not finite: a product of a weight of zero and an infinity or
-// NaN in a value that the row does not see must not reach it (and a result that is truly not finite comes out again).
+// NaN in a value that the row does not see must not reach it (and a result that is truly not finite comes out again). And rows that see a key, but whose
+// weights were all zero: scores below where the running maximum starts, or so large that their exponents in one rounding and in two are far apart.
 template <class T> __device__ __noinline__ void attn_row_by_key(const PagedAttn& a, int b, const SeqRows& s, int i, int h) {
     const int lane = threadIdx.x & 31, g = h / (a.H / a.G);
     const T* q = (const T*)a.q + (long)(s.row0 + i) * a.ldq + (long)h * a.dk;

@@ -392,7 +392,7 @@ __global__ void __launch_bounds__(kF32Threads, 1) attn_paged_f32_kernel(const __
             tc_fence_after();
             if (any) add_page(t1 - t0 - 1, al);
             const float rl = t.n_split > 1 ? 1.0f : l == 0.0f ? 0.0f : 1.0f / l;
-            bool odd = false;
+            bool odd = live && t.n_split == 1 && l == 0.0f && (sure > 0 || bits != 0);
             float* orow = reinterpret_cast<float*>(base_ptr) + (long)row * (a.dv + 4);
             float* out = (float*)a.out + (long)(s.row0 + i) * a.ldo + (long)(h0 + hr) * a.dv;
             const bool vec = whole_stores<float>(a);

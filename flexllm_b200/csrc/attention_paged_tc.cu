@@ -15,7 +15,8 @@
 // between sequences (16 of 25 tokens over 8000: 89 us, 4.2 TB/s); single tokens by the products, which take 128 rows for a few (one over 84500: 81 us,
 // 4.3 TB/s, the tensor cores busy 73 % on 80 SMs); short calls by latency (26 tokens over 1000: 14 us, eight prompts of 143: 11.6 us).
 // Keys behind a sequence's last one were never written: their scores are replaced, their values zeroed in shared memory. Any other value
-// that a row does not see meets a weight of zero; a row whose result is not finite is computed again, key by key.
+// that a row does not see meets a weight of zero; a row whose result is not finite, or whose weights are all zero
+// although it sees a key, is computed again, key by key.
 #include "attention_join.cuh"
 
 namespace flexllm {
@@ -321,7 +322,7 @@ __global__ void __launch_bounds__(MODE == kOne ? 192 : 320, MODE == kOne ? 2 : 1
             tc_fence_after();
             if (MODE == kPair || (MODE == kOne && t.n_split == 1)) {
                 const float rl = l == 0.0f ? 0.0f : 1.0f / l;
-                bool odd = false;
+                bool odd = live && l == 0.0f && (sure > 0 || bits != 0);
                 bf16* out = (bf16*)a.out + (long)(s.row0 + i) * a.ldo + (long)(h0 + hr) * a.dv;
                 const bool vec = (a.ldo & 7) == 0 && aligned16(a.out);
                 for (int d0 = 0; d0 < t.vr; d0 += 32) {

@@ -55,3 +55,67 @@ def test_parts_without_keys_beside_long_sequences_with_wide_heads(ops, dim, vdim
     top = (q[3].double() @ pc.gather(k, v, table, 2, 0, 71)[0].T).argmax(-1)
     vals = pc.gather(k, v, table, 2, 0, 71)[1]
     assert torch.equal(first[3].view(3, vdim).double(), vals[top])
+
+
+SEQUENCES = [([1], [3000]), ([40, 3], [90, 0]), ([1] * 9, [700] * 9), ([300, 500], [0, 64])]
+
+
+def pages(k, v, new, ctx, seed=0):
+    """k [keys,G,dim] and v [keys,G,vdim] of all sequences, one behind the other, as pages; table, start, ctx."""
+    table, start, cx, n_pages = pc.layout(new, ctx, seed)
+    kp = torch.zeros((n_pages, 64) + k.shape[1:], dtype=k.dtype, device="cuda")
+    vp = torch.zeros((n_pages, 64) + v.shape[1:], dtype=v.dtype, device="cuda")
+    at = 0
+    for b, (n, c) in enumerate(zip(new, ctx)):
+        for p in range((n + c + 63) // 64):
+            m = min(64, n + c - 64 * p)
+            kp[table[b, p], :m], vp[table[b, p], :m] = k[at:at + m], v[at:at + m]
+            at += m
+    return kp.transpose(1, 2).contiguous(), vp.permute(0, 2, 3, 1).contiguous(), table.cuda(), start.cuda(), cx.cuda()
+
+
+def means(v, new, ctx, H, tree):
+    """The mean of the values that each row sees, in 64 bits; of a tree the cached ones and the row itself."""
+    out, at = [], 0
+    for n, c in zip(new, ctx):
+        for i in range(n):
+            seen = torch.cat([v[at:at + c], v[at + c + i:at + c + i + 1]]) if tree else v[at:at + c + i + 1]
+            out.append(seen.double().mean(0).repeat_interleave(H // v.shape[1], 0).reshape(-1))
+        at += n + c
+    return torch.stack(out)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF], ids=["f32", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("new,ctx", SEQUENCES, ids=lambda v: "%d.%s" % (len(v), v[0]))
+def test_finite_scores_below_every_start_of_a_maximum(ops, dtype, dim, new, ctx):
+    """Scores of -7e31 and more: all alike, so that a row is the mean of the values it sees; and one of them higher, which has all the weight. Weights are
+    one: the sums of up to 3001 values are off by as many half steps of 2^-24, a result by its rounding."""
+    H, G, keys = 4, 2, sum(new) + sum(ctx)
+    g = torch.Generator(device="cuda").manual_seed(dim)
+    v = torch.randn((keys, G, dim), generator=g, device="cuda").to(dtype)
+    k = torch.full((keys, G, dim), -3e15, device="cuda").to(dtype)
+    q = torch.full((sum(new), H, dim), 3e15, device="cuda").to(dtype)
+    eye = torch.cat([1 << torch.arange(min(n, 63), dtype=torch.int64) for n in new]).cuda() if max(new) < 63 else None
+    for tree in (False, True):
+        if tree and eye is None:
+            continue
+        args = pages(k, v, new, ctx)
+        got = ops.attn_tree(q, eye, *args) if tree else ops.attn_packed(q, *args)
+        want = means(v, new, ctx, H, tree)
+        far = max(n + c for n, c in zip(new, ctx)) * 2.0 ** -24 * v.double().abs().amax() + (want.abs() * 2.0 ** -8 if dtype == BF else 0)
+        assert ((got.double() - want).abs() <= far).all(), (got.double() - want).abs().max()
+    up = k.clone()
+    up[0] = torch.tensor(-2e15).to(dtype)                       # the first key of the first sequence
+    got = ops.attn_packed(q[:new[0]], *pages(up[:new[0] + ctx[0]], v[:new[0] + ctx[0]], new[:1], ctx[:1]))
+    assert torch.equal(got, v[0].repeat_interleave(H // G, 0).reshape(1, -1).expand_as(got))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF], ids=["f32", "bf16"])
+def test_rows_that_see_nothing_stay_zero(ops, dtype):
+    v = torch.randn((50, 2, 64), device="cuda").to(dtype)
+    q = torch.full((50, 4, 64), 3e15, device="cuda").to(dtype)
+    mask = torch.zeros(50, dtype=torch.int64, device="cuda")
+    mask[7] = 1 << 3
+    got = ops.attn_tree(q, mask, *pages(torch.full_like(v, -3e15), v, [50], [0]))
+    assert torch.equal(got[7], v[3].repeat_interleave(2, 0).reshape(-1)) and not got[:7].any() and not got[8:].any()
