@@ -24,6 +24,12 @@ template <class T> __device__ __forceinline__ bool whole_stores(const PagedAttn&
 
 constexpr int kJoinRows = 144;             // rows of a tile and 16 CTAs, a multiple of their number: up to 15 more
 
+// scale * log2 e; for a scale of 0 the smallest number, so that masked scores of -infinity stay that: 3.4e38 becomes 4.8e-7, a weight of 1 but for the last bits
+inline float score_factor(const PagedAttn& a) {
+    const float f = a.scale * kLog2e;
+    return f > 1.401298464e-45f ? f : 1.401298464e-45f;
+}
+
 // The parts of a tile of 128 rows, STEP of them in each of the n_split CTAs of a cluster, joined by all nt threads of every CTA: maxima (log2 units) and
 // sums at m_at and l_at, [STEP][128], outputs at o_at, [STEP][128][dv + 4], at the same addresses in every CTA and fenced. CTA r of the
 // cluster has rows r, r + n_split, ..: first the parts' weights (over the sums; parts x rows of a CTA are kJoinRows STEP at most), then the outputs.

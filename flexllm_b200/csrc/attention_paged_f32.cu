@@ -462,8 +462,7 @@ int attn_paged_f32(const PagedAttn& a, cudaStream_t st) {
     t.RC = R < 128 ? R : 128; t.HC = (R + t.RC - 1) / t.RC; t.TQ = 128 / t.RC;
     t.kc = (a.dk + 63) / 64; t.kq = (a.dk + 31) / 32; t.vr = (a.dv + 15) / 16 * 16;
     t.v_rows = (a.dv + 31) / 32 * 8;
-    t.a2 = a.scale * kLog2e;
-    if (t.a2 < 1e-30f) t.a2 = 1e-30f;                     // scale 0: weights all alike, and no infinity times zero
+    t.a2 = score_factor(a);
     const long heads = (long)a.G * t.HC, seqs = a.seq.B < a.seq.T ? a.seq.B : a.seq.T, ones = most_units(a.seq, t.TQ);
     t.heads = (int)heads;
     if (ones * 16 * heads > 0x7fffffffL) return FLEXLLM_ENOTSUP;

@@ -450,8 +450,7 @@ int attn_paged_tc(const PagedAttn& a, cudaStream_t st) {
     t.a = a;
     t.RC = R < 128 ? R : 128; t.HC = (R + t.RC - 1) / t.RC;
     t.kc = (a.dk + 63) / 64; t.vr = (a.dv + 15) / 16 * 16; t.o_stride = (t.vr + 31) / 32 * 32;
-    t.a2 = a.scale * kLog2e;
-    if (t.a2 < 1e-30f) t.a2 = 1e-30f;                     // scale 0: weights all alike, and no infinity times zero
+    t.a2 = score_factor(a);
     const long heads = (long)a.G * t.HC, seqs = a.seq.B < a.seq.T ? a.seq.B : a.seq.T, each = (a.seq.T + seqs - 1) / seqs;
     // short tiles where two of them would hold what sequences have on average: shared memory for Q becomes stages (one token over 84500, 8 key/value
     // heads: 105 us and 81)

@@ -119,3 +119,21 @@ def test_rows_that_see_nothing_stay_zero(ops, dtype):
     mask[7] = 1 << 3
     got = ops.attn_tree(q, mask, *pages(torch.full_like(v, -3e15), v, [50], [0]))
     assert torch.equal(got[7], v[3].repeat_interleave(2, 0).reshape(-1)) and not got[:7].any() and not got[8:].any()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF], ids=["f32", "bf16"])
+@pytest.mark.parametrize("dim", [64, 256])
+@pytest.mark.parametrize("scale", [0.0, 1e-38, 1e-44])
+def test_scales_that_leave_all_weights_alike(ops, dtype, dim, scale):
+    """Products of q and k from -1e38 to 1e38: a scale of 0 makes them alike, and one of 1e-38 is no other."""
+    new, ctx = [70, 2], [30, 500]
+    g = torch.Generator(device="cuda").manual_seed(dim)
+    keys = sum(new) + sum(ctx)
+    v = torch.randn((keys, 2, dim), generator=g, device="cuda").to(dtype)
+    size = torch.linspace(-1.0, 1.0, keys, device="cuda")[torch.randperm(keys, generator=g, device="cuda")]
+    k = (size[:, None, None] * (1e19 / dim)).expand(keys, 2, dim).to(dtype)
+    q = torch.full((72, 4, dim), 1e19, device="cuda").to(dtype)
+    args = pages(k, v, new, ctx)
+    got = ops.attn_packed(q, *args, scale=scale)
+    want, far = pc.attention(q, args[0], args[1], args[2].cpu(), args[3].cpu(), args[4].cpu(), scale)
+    assert ((got.double() - want).abs() <= far).all(), ((got.double() - want).abs() / far).max()
