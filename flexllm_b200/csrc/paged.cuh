@@ -1,7 +1,7 @@
 // What the operators over packed sequences and the floating-point paged cache share: sequence b of a call has the packed rows
 // cu[b] .. cu[b+1] - 1, at cache positions ctx[b] .., in pages of 64 tokens, K [page][G][64][dk], V transposed [page][G][dv][64].
-// cu, ctx and the page table are device memory that the host never sees: values out of range are clamped (a page id: page 0; entries
-// that no position needs are not looked at) and reported through the device's error word, so that no access leaves its buffer.
+// cu, ctx and the page table are device memory that the host never sees: values out of range are clamped (a page id: reads take page 0, writes are
+// left out; entries that no position needs are not looked at) and reported through the device's error word, so that no access leaves its buffer.
 #pragma once
 #include "float_common.cuh"
 
@@ -29,12 +29,15 @@ __device__ __forceinline__ SeqRows seq_rows(const PackedSeqs& p, int b) {
     if (s.row0 != c0 || s.n != c1 - c0 || (s.n > 0 && s.ctx != x0)) data_error(p.error_flag);
     return s;
 }
-__device__ __forceinline__ int page_of(const PackedSeqs& p, int b, int i) {
+// Page i of sequence b, or -1. Nothing is written for a page that the table does not name: page 0 may be another sequence's.
+__device__ __forceinline__ int page_or_none(const PackedSeqs& p, int b, int i) {
     const int page = p.page_table[(long)b * p.max_pages + i];
     if ((unsigned)page < (unsigned)p.n_pages) return page;
     data_error(p.error_flag);
-    return 0;
+    return -1;
 }
+// The same for reads: page 0 in its place.
+__device__ __forceinline__ int page_of(const PackedSeqs& p, int b, int i) { return max(page_or_none(p, b, i), 0); }
 
 // How many of `n` are below a border, where below(i) holds up to it; 32 looks at a time. One whole warp.
 template <class Below> __device__ __forceinline__ int count_below(int n, Below below) {

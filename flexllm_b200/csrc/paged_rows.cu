@@ -102,7 +102,7 @@ template <class T, int L> __device__ __forceinline__ void rope_warp(const RopeAr
     if (t < s.row0 || t >= s.row0 + s.n) return;
     if (outside) data_error(a.seq.error_flag);
     const int at = s.ctx + t - s.row0;
-    const long page = h1 > a.H ? page_of(a.seq, b, at / kPage) : 0;
+    const long page = h1 > a.H ? page_or_none(a.seq, b, at / kPage) : 0;
     const float inv_dk = 1.0f / (float)a.dk;
     for (int h = h0; h < h1; h += kRounds * (32 / L)) {
         if (h > h0) load(h);
@@ -125,8 +125,10 @@ template <class T, int L> __device__ __forceinline__ void rope_warp(const RopeAr
             }
             T* dst = hj < a.H ? (T*)a.q + (long)t * a.ldq + (long)hj * a.dk
                               : (T*)a.k + ((page * a.G + (hj - a.H)) * kPage + (at & (kPage - 1))) * a.dk;
-            store_four(dst + e0, times_plus(v, minus_si, times(u, co)));
-            store_four(dst + e1, times_plus(u, si, times(v, co)));
+            const Four lo = times_plus(v, minus_si, times(u, co)), hi = times_plus(u, si, times(v, co));
+            if (hj >= a.H && page < 0) continue;           // looked at here and no earlier: the page's id is on its way until now
+            store_four(dst + e0, lo);
+            store_four(dst + e1, hi);
         }
     }
 }
@@ -167,8 +169,9 @@ template <class T, int L> __global__ void __launch_bounds__(256, 4) qk_norm_rope
         uint32_t* dst = reinterpret_cast<uint32_t*>(tile + (long)t * pitch + d);
         dst[0] = w.x; dst[1] = w.y; dst[2] = w.z; dst[3] = w.w;
     }
-    const long page = page_of(a.seq, unit_sm.b, pg);
+    const long page = page_or_none(a.seq, unit_sm.b, pg);
     __syncthreads();
+    if (page < 0) return;
     T* vp = (T*)a.v + (page * a.G + g) * (long)a.dv * kPage;
     constexpr int PIECES = kPage / N;
     for (int e = tid; e < a.dv * PIECES; e += 256) {
@@ -237,9 +240,12 @@ template <class T> __global__ void __launch_bounds__(256) kv_keep_kernel(const _
         if (ctx < 0 || from < 0 || from >= 64 || max(from, tid) > a.seq.max_ctx - ctx) data_error(a.seq.error_flag);      // such an entry is not moved
         else if (from != tid) {
             const int s = ctx + from, d = ctx + tid;
-            const int sp = page_of(p, b, s / kPage), dp = page_of(p, b, d / kPage), m = atomicAdd(&n_moves, 1);
-            src_page[m] = sp; src_slot[m] = s & (kPage - 1);
-            dst_page[m] = dp; dst_slot[m] = d & (kPage - 1);
+            const int sp = page_or_none(p, b, s / kPage), dp = page_or_none(p, b, d / kPage);
+            if (sp >= 0 && dp >= 0) {
+                const int m = atomicAdd(&n_moves, 1);
+                src_page[m] = sp; src_slot[m] = s & (kPage - 1);
+                dst_page[m] = dp; dst_slot[m] = d & (kPage - 1);
+            }
         }
     }
     __syncthreads();

@@ -460,8 +460,8 @@ FLEXLLM_API int flexllm_attn_window(int dtype, flexllm_kv_cache* c, int layer, c
  * A call has T packed rows; sequence b < B has the rows cu[b] .. cu[b+1] - 1 (cu [B+1], cu[0] = 0; a sequence may have none, rows from cu[B] on are
  * left alone) at the cache positions ctx[b] .. of its pages page_table[b][0 ..] (max_pages per sequence; entries behind its last position are
  * not looked at). max_ctx: largest position of the call, < 64 * max_pages and < 2^30. cu, ctx, page_table, pos, keep and count are device memory;
- * values out of range are clamped and reported by flexllm_device_status() (FLEXLLM_EDEVDATA). Element type FLEXLLM_BF16 or FLEXLLM_F32 for
- * rows and pages alike; scores, norms, weights and sums are fp32. kdim and vdim multiples of 8 up to 256 (else FLEXLLM_ENOTSUP).
+ * values out of range are clamped and reported by flexllm_device_status() (FLEXLLM_EDEVDATA); where the table names no page nothing is written. Element type
+ * FLEXLLM_BF16 or FLEXLLM_F32 for rows and pages alike; scores, norms, weights and sums are fp32. kdim and vdim multiples of 8 up to 256 (else FLEXLLM_ENOTSUP).
  * ------------------------------------------------------------------------------------------- */
 /* One layer's pages of 64 tokens, K [n_pages][hkv][64][kdim] and V [n_pages][hkv][vdim][64], 16-byte aligned: memory of the caller, or a layer of a
  * cache made by flexllm_kv_cache_create_float, which flexllm_kv_cache_pages describes. */
@@ -493,7 +493,8 @@ FLEXLLM_API int flexllm_attn_tree(int dtype, const flexllm_kv_pages* kv, int hea
                                   const int32_t* cu, const int32_t* ctx, const int32_t* page_table, int max_pages, int max_ctx, int B, int T, void* out,
                                   long ldo, void* stream);
 /* The accepted tokens of every tree moved together, in all `layers` layers: the entries at ctx[b] + keep[b][i] become those at ctx[b] + i,
- * i < count[b] <= most <= 64, keep [B][most] in [0, 64) in any order. An entry out of range stays where it is and is reported. */
+ * i < count[b] <= most <= 64, keep [B][most] in [0, 64) in any order. An entry out of range, or from or to a page that the table does not name, stays where
+ * it is and is reported. */
 FLEXLLM_API int flexllm_kv_keep(int dtype, const flexllm_kv_pages* layers_host, int layers, const int32_t* page_table, int max_pages, const int32_t* ctx,
                                 int max_ctx, const int32_t* keep, const int32_t* count, int most, int B, void* stream);
 

@@ -137,3 +137,52 @@ def test_scales_that_leave_all_weights_alike(ops, dtype, dim, scale):
     got = ops.attn_packed(q, *args, scale=scale)
     want, far = pc.attention(q, args[0], args[1], args[2].cpu(), args[3].cpu(), args[4].cpu(), scale)
     assert ((got.double() - want).abs() <= far).all(), ((got.double() - want).abs() / far).max()
+
+
+def status():
+    from flexllm_b200 import lib
+    return lib().flexllm_device_status()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF], ids=["f32", "bf16"])
+@pytest.mark.parametrize("bad", [-1, 6, 2 ** 31 - 1, -2 ** 31])
+@pytest.mark.parametrize("many", [False, True], ids=["few", "many"])
+def test_nothing_is_appended_where_the_table_names_no_page(ops, dtype, bad, many):
+    """Positions 60 .. 79 of a sequence whose second page is bad: the first four are written, nothing else is, page 0 least of all."""
+    H, G, dim, n = 4, 2, 64, 20
+    g = torch.Generator(device="cuda").manual_seed(3)
+    r = lambda *s: torch.randn(s, generator=g, device="cuda").to(dtype)
+    k, v, proj = r(6, G, 64, dim), r(6, G, dim, 64), r(n + 3, (H + 2 * G) * dim)
+    table, cu, ctx = [[5, bad], [2, 4]], [0, n, n + 3], [60, 62]
+    if many:                                                    # sequences that are searched, not looked through
+        table, cu, ctx = table + [[1, 1]] * 80, cu + [n + 3] * 80, ctx + [0] * 80
+    cos, sin = torch.ones((1, 32), device="cuda"), torch.zeros((1, 32), device="cuda")
+    k1, v1, x = k.clone(), v.clone(), proj.view(n + 3, -1, dim)
+    k1[5, :, 60:], v1[5, :, :, 60:] = x[:4, H:H + G].transpose(0, 1), x[:4, H + G:].permute(1, 2, 0)
+    for i, (page, slot) in enumerate([(2, 62), (2, 63), (4, 0)]):
+        k1[page, :, slot], v1[page, :, :, slot] = x[n + i, H:H + G], x[n + i, H + G:]
+    assert status() == 0
+    q = ops.qk_norm_rope(proj, H, torch.zeros(n + 3, dtype=torch.int32, device="cuda"), cos, sin, k, v, torch.tensor(table, dtype=torch.int32, device="cuda"), i32(*cu), i32(*ctx))
+    assert status() == -7
+    assert torch.equal(k, k1) and torch.equal(v, v1) and torch.equal(q.view(n + 3, H, dim), x[:, :H])
+
+
+@pytest.mark.parametrize("dtype", [F32, BF], ids=["f32", "bf16"])
+@pytest.mark.parametrize("bad", [-1, 6, 2 ** 31 - 1])
+def test_no_entry_moves_from_or_to_a_page_that_the_table_does_not_name(ops, dtype, bad):
+    g = torch.Generator(device="cuda").manual_seed(4)
+    r = lambda *s: torch.randn(s, generator=g, device="cuda").to(dtype)
+    layers = [(r(6, 2, 64, 64), r(6, 2, 64, 64)) for _ in range(3)]
+    table = torch.tensor([[3, bad], [bad, 4], [1, 5]], dtype=torch.int32, device="cuda")
+    # positions 60 + keep: over the border from the bad page, over it to the bad page and within the good one, good
+    ctx, keep, count = i32(60, 60, 60), torch.tensor([[2, 9], [7, 1], [9, 8]], dtype=torch.int32, device="cuda"), i32(2, 2, 2)
+    want = [(k.clone(), v.clone()) for k, v in layers]
+    for (k, v), (k0, v0) in zip(layers, want):
+        k0[3, :, 60], v0[3, :, :, 60] = k[3, :, 62], v[3, :, :, 62]             # 62 to 60; 69 is on the bad page
+        for i, s in enumerate((69, 68)):
+            k0[1, :, 60 + i], v0[1, :, :, 60 + i] = k[5, :, s - 64], v[5, :, :, s - 64]
+    assert status() == 0
+    ops.kv_keep(layers, table, ctx, keep, count)
+    assert status() == -7
+    for (k, v), (k0, v0) in zip(layers, want):
+        assert torch.equal(k, k0) and torch.equal(v, v0)
