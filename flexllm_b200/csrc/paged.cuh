@@ -1,7 +1,8 @@
 // What the operators over packed sequences and the floating-point paged cache share: sequence b of a call has the packed rows
 // cu[b] .. cu[b+1] - 1, at cache positions ctx[b] .., in pages of 64 tokens, K [page][G][64][dk], V transposed [page][G][dv][64].
-// cu, ctx and the page table are device memory that the host never sees: values out of range are clamped (a page id: reads take page 0, writes are
-// left out; entries that no position needs are not looked at) and reported through the device's error word, so that no access leaves its buffer.
+// cu, ctx and the page table are device memory that the host never sees: values out of range are clamped (a page id: reads take page 0; entries that no
+// position needs are not looked at) and reported through the device's error word, so that no access leaves its buffer. What a sequence with such
+// values, or a page that the table does not name, would receive is left out.
 #pragma once
 #include "float_common.cuh"
 
@@ -15,7 +16,7 @@ struct PackedSeqs {
     int max_new;                           // most rows of one sequence
     int* error_flag;
 };
-struct SeqRows { int row0, n, ctx; };      // first packed row, rows, tokens already in the cache
+struct SeqRows { int row0, n, ctx; bool sound; };      // first packed row, rows, tokens already in the cache; as the call says, not clamped
 
 __device__ __forceinline__ void data_error(int* flag) { if (flag) atomicOr(flag, 2); }
 
@@ -26,7 +27,8 @@ __device__ __forceinline__ SeqRows seq_rows(const PackedSeqs& p, int b) {
     s.n = min(max(c1, s.row0), p.T) - s.row0;
     s.n = min(min(s.n, p.max_new), p.max_ctx + 1);
     s.ctx = min(max(x0, 0), p.max_ctx + 1 - s.n);
-    if (s.row0 != c0 || s.n != c1 - c0 || (s.n > 0 && s.ctx != x0)) data_error(p.error_flag);
+    s.sound = s.row0 == c0 && s.n == c1 - c0 && (s.n == 0 || s.ctx == x0);
+    if (!s.sound) data_error(p.error_flag);
     return s;
 }
 // Page i of sequence b, or -1. Nothing is written for a page that the table does not name: page 0 may be another sequence's.
@@ -61,7 +63,7 @@ constexpr int kLookThrough = 64;
 template <class Count> __device__ __forceinline__ Unit find_unit(const PackedSeqs& p, int u, int per, int extra, Count count) {
     const int lane = threadIdx.x & 31;
     Unit r;
-    r.b = -1; r.i = 0; r.s.row0 = r.s.n = r.s.ctx = 0;
+    r.b = -1; r.i = 0; r.s.row0 = r.s.n = r.s.ctx = 0; r.s.sound = true;
     if (p.B > kLookThrough) {
         if ((long)u * 32 + lane < p.B) seq_rows(p, u * 32 + lane);        // for what it reports
         const int id = p.T / per + extra * p.B - 1 - u;
@@ -76,7 +78,7 @@ template <class Count> __device__ __forceinline__ Unit find_unit(const PackedSeq
     int base = 0;
     for (int b0 = 0; b0 < p.B; b0 += 32) {
         const int b = p.B - 1 - b0 - lane;
-        SeqRows s = {0, 0, 0};
+        SeqRows s = {0, 0, 0, true};
         if (b >= 0) s = seq_rows(p, b);
         const int c = s.n > 0 ? count(s) : 0;
         int incl = c;
@@ -93,6 +95,7 @@ template <class Count> __device__ __forceinline__ Unit find_unit(const PackedSeq
             r.s.row0 = __shfl_sync(0xffffffffu, s.row0, src);
             r.s.n = __shfl_sync(0xffffffffu, s.n, src);
             r.s.ctx = __shfl_sync(0xffffffffu, s.ctx, src);
+            r.s.sound = __shfl_sync(0xffffffffu, (int)s.sound, src);
             return r;
         }
         base += __shfl_sync(0xffffffffu, incl, 31);

@@ -102,7 +102,7 @@ template <class T, int L> __device__ __forceinline__ void rope_warp(const RopeAr
     if (t < s.row0 || t >= s.row0 + s.n) return;
     if (outside) data_error(a.seq.error_flag);
     const int at = s.ctx + t - s.row0;
-    const long page = h1 > a.H ? page_or_none(a.seq, b, at / kPage) : 0;
+    const long page = h1 <= a.H ? 0 : s.sound ? page_or_none(a.seq, b, at / kPage) : -1;
     const float inv_dk = 1.0f / (float)a.dk;
     for (int h = h0; h < h1; h += kRounds * (32 / L)) {
         if (h > h0) load(h);
@@ -154,7 +154,7 @@ template <class T, int L> __global__ void __launch_bounds__(256, 4) qk_norm_rope
         if (tid == 0) unit_sm = u;
     }
     __syncthreads();
-    if (unit_sm.b < 0) return;
+    if (unit_sm.b < 0 || !unit_sm.s.sound) return;
     const SeqRows s = unit_sm.s;
     const int pg = s.ctx / kPage + unit_sm.i;
     const int lo = max(s.ctx, pg * kPage) - pg * kPage, hi = min(s.ctx + s.n - pg * kPage, kPage);      // slots [lo, hi)

@@ -186,3 +186,31 @@ def test_no_entry_moves_from_or_to_a_page_that_the_table_does_not_name(ops, dtyp
     assert status() == -7
     for (k, v), (k0, v0) in zip(layers, want):
         assert torch.equal(k, k0) and torch.equal(v, v0)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF], ids=["f32", "bf16"])
+@pytest.mark.parametrize("cu,ctx,sound", [((0, 10, 23), (-1, 3), (1,)), ((0, 10, 23), (119, 3), (1,)), ((0, 10, 23), (5, 2 ** 31 - 1), (0,)), ((0, 10, 400), (5, 3), (0,)),
+                                          ((-3, 10, 23), (5, 3), (1,)), ((0, 30, 20), (5, 3), ()), ((0, 10, 5), (5, 3), (0,))], ids=str)
+@pytest.mark.parametrize("many", [False, True], ids=["few", "many"])
+def test_nothing_is_appended_for_a_sequence_whose_values_are_out_of_range(ops, dtype, cu, ctx, sound, many):
+    """Contexts before the first position and behind the last one (128 positions), row starts that leave the 23 rows or fall: the other sequence is appended,
+    nothing of the bad one is, not even at clamped positions."""
+    H, G, dim, T = 4, 2, 64, 23
+    g = torch.Generator(device="cuda").manual_seed(5)
+    r = lambda *s: torch.randn(s, generator=g, device="cuda").to(dtype)
+    k, v, proj = r(5, G, 64, dim), r(5, G, dim, 64), r(T, (H + 2 * G) * dim)
+    table = [[1, 2], [3, 4]]
+    k0, v0, k1, v1, x = k.clone(), v.clone(), k.clone(), v.clone(), proj.view(T, -1, dim)
+    for b in sound:
+        for t in range(cu[b], cu[b + 1]):
+            at = ctx[b] + t - cu[b]
+            k1[table[b][at // 64], :, at % 64], v1[table[b][at // 64], :, :, at % 64] = x[t, H:H + G], x[t, H + G:]
+    if many:
+        table, ctx, cu = table + [[1, 2]] * 70, list(ctx) + [0] * 70, list(cu) + [cu[2]] * 70
+    cos, sin = torch.ones((1, 32), device="cuda"), torch.zeros((1, 32), device="cuda")
+    assert status() == 0
+    ops.qk_norm_rope(proj, H, torch.zeros(T, dtype=torch.int32, device="cuda"), cos, sin, k, v, torch.tensor(table, dtype=torch.int32, device="cuda"), i32(*cu), i32(*ctx))
+    assert status() == -7
+    if min(b - a for a, b in zip(cu, cu[1:])) < 0:              # where starts fall, two sequences claim a row: it may be left out
+        k1, v1 = torch.where(k == k0, k0, k1), torch.where(v == v0, v0, v1)
+    assert torch.equal(k, k1) and torch.equal(v, v1)
