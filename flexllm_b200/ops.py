@@ -580,8 +580,8 @@ def linear_w4(x, w, scale, zero=None, bias=None, out_f32=False, out=None):
     _same(x, scale.dtype, scale)
     _same(x, torch.float32, bias)
     y = torch.empty((M, N), dtype=torch.float32 if out_f32 else x.dtype, device=x.device) if out is None else out
-    if y.dim() != 2 or y.shape[0] != M or y.shape[1] != N or y.dtype is not (torch.float32 if out_f32 else x.dtype):
-        raise ValueError("flexllm_b200: linear_w4: out has to be [%d,%d] %s" % (M, N, torch.float32 if out_f32 else x.dtype))
+    if y.dim() != 2 or y.shape[0] != M or y.shape[1] != N or y.dtype is not (torch.float32 if out_f32 else x.dtype) or y.device != x.device:
+        raise ValueError("flexllm_b200: linear_w4: out has to be [%d,%d] %s on %s" % (M, N, torch.float32 if out_f32 else x.dtype, x.device))
     yp, ldy = _rows(y)
     _call_on(x.device, "flexllm_linear_w4", _DTYPE[x.dtype], p, lda, w.data_ptr(), scale.data_ptr(), _DTYPE[scale.dtype], _ptr(zero), K // scale.shape[1],
              _ptr(bias), M, N, K, yp, ldy, 1 if out_f32 else 0)
