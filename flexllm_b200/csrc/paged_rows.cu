@@ -320,7 +320,7 @@ extern "C" int flexllm_qk_norm_rope(int dtype, const flexllm_kv_pages* kv, int h
     if (!dims_ok(kv) || rot % 8) return FLEXLLM_ENOTSUP;
     int end = 0;
     for (int i = 0; i < axes; i++) {
-        const int n = axes == 1 ? rot / 2 : sections_host[i];
+        const int n = sections_host ? sections_host[i] : rot / 2;
         FLEXLLM_REQUIRE(n >= 0 && n <= rot / 2 - end);
         end += n;
         a.sec_end[i] = end;

@@ -473,7 +473,7 @@ FLEXLLM_API int flexllm_kv_cache_pages(flexllm_kv_cache* c, int layer, flexllm_k
  *   y = x / sqrt(mean x^2 + eps) * gain  (q_gain, k_gain [kdim] fp32, either NULL: no norm for that side)
  *   pair p < rot/2 turns y[p] and y[p + rot/2] by the angle with cosine cos_t[pos_a][p] and sine sin_t[pos_a][p], a the axis of the pair
  * proj [T][ldp]: q heads | k heads | v heads. pos [axes][T]: positions of the rows (time, height, width, ...), 1 to 4 axes; sections_host[axes]: pairs
- * that follow each axis, in order, adding up to rot/2 (NULL with one axis). cos_t, sin_t [table_len][rot/2] fp32; rot a multiple of 8 up to
+ * that follow each axis, in order, adding up to rot/2 (one axis: may be NULL). cos_t, sin_t [table_len][rot/2] fp32; rot a multiple of 8 up to
  * kdim (0: no rotation), the elements behind it only normed. q [T][ldq] receives the q heads, the pages the keys and values. Row strides are
  * multiples of 16 bytes, pointers 16-byte aligned. */
 FLEXLLM_API int flexllm_qk_norm_rope(int dtype, const flexllm_kv_pages* kv, int heads, const void* proj, long ldp, const float* q_gain, const float* k_gain,

@@ -58,3 +58,13 @@ def test_four_bit_products_want_their_output_on_their_inputs_device(ops, called)
         with pytest.raises(ValueError):
             ops.linear_w4(x, w, s, out_f32=out_f32, out=OnDevice((2, 8), dtype, 1))
     assert len(called) == 2
+
+
+def test_sections_of_one_axis_have_to_add_up():
+    import test_paged_cpu as c
+    from flexllm_b200 import build
+    build.build()
+    lib = _lib.load()
+    assert c.rope(lib, sec=[32]) == _lib.OK and c.rope(lib) == _lib.OK
+    for bad in (31, 33, 0, -32):
+        assert c.rope(lib, sec=[bad]) == _lib.EINVAL
