@@ -420,7 +420,15 @@ def _packed(like, page_table, cu, ctx, max_ctx):
     B, max_pages = page_table.shape
     if cu.numel() != B + 1 or ctx.numel() != B:
         raise ValueError("flexllm_b200: %d sequences in the page table, cu has %d and ctx %d entries" % (B, cu.numel(), ctx.numel()))
-    return max_pages, max_pages * 64 - 1 if max_ctx is None else max_ctx, B
+    return max_pages, _last_position(max_pages, max_ctx), B
+
+
+def _last_position(max_pages, max_ctx):
+    if max_ctx is None:
+        return max_pages * 64 - 1
+    if not -1 << 31 <= max_ctx < 1 << 31:                # the call takes 32 bits
+        raise ValueError("flexllm_b200: max_ctx %d" % max_ctx)
+    return max_ctx
 
 
 class PagedKV:
@@ -483,7 +491,8 @@ def qk_norm_rope(proj, heads, pos, cos_t, sin_t, k_pages, v_pages, page_table, c
     _same(proj, torch.float32, cos_t, sin_t, q_gain, k_gain)
     _same(proj, torch.int32, pos)
     axes = pos.shape[0] if pos.dim() == 2 else 1
-    if proj.shape[1] != (heads + kv.hkv) * kv.kdim + kv.hkv * kv.vdim or pos.numel() != axes * T or (axes > 1 and (sections is None or len(sections) != axes)):
+    if proj.shape[1] != (heads + kv.hkv) * kv.kdim + kv.hkv * kv.vdim or pos.numel() != axes * T or (
+            axes > 1 if sections is None else len(sections) != axes or any(not 0 <= n <= cos_t.shape[-1] for n in sections)):
         raise ValueError("flexllm_b200: qk_norm_rope: the widths of proj, pos and sections do not fit %d heads" % heads)
     if cos_t.dim() != 2 or cos_t.shape != sin_t.shape or any(x is not None and x.numel() != kv.kdim for x in (q_gain, k_gain)):
         raise ValueError("flexllm_b200: qk_norm_rope: tables are [P, rot/2], gains [dim]")
@@ -560,7 +569,7 @@ def kv_keep(layers, page_table, ctx, keep, count, max_ctx=None):
     if ctx.numel() != B or count.numel() != B or keep.dim() != 2 or keep.shape[0] != B:
         raise ValueError("flexllm_b200: kv_keep: page_table, ctx, keep and count are for different numbers of sequences")
     _call_on(k0.device, "flexllm_kv_keep", _DTYPE[k0.dtype], kv, len(layers), page_table.data_ptr(), max_pages, ctx.data_ptr(),
-             max_pages * 64 - 1 if max_ctx is None else max_ctx, keep.data_ptr(), count.data_ptr(), keep.shape[1], B)
+             _last_position(max_pages, max_ctx), keep.data_ptr(), count.data_ptr(), keep.shape[1], B)
 
 
 def linear_w4(x, w, scale, zero=None, bias=None, out_f32=False, out=None):

@@ -60,6 +60,27 @@ def test_four_bit_products_want_their_output_on_their_inputs_device(ops, called)
     assert len(called) == 2
 
 
+def test_positions_and_sections_of_more_than_32_bits(ops, called):
+    """ctypes passes the low 32 bits on; sections of one axis were not looked at."""
+    I32, F32 = torch.int32, torch.float32
+    k, v, q = OnDevice((2, 2, 64, 64), F32), OnDevice((2, 2, 64, 64), F32), OnDevice((3, 4, 64), F32)
+    table, cu, ctx, mask = OnDevice((1, 2), I32), OnDevice((2,), I32), OnDevice((1,), I32), OnDevice((3,), torch.int64)
+    keep, count, out = OnDevice((1, 4), I32), OnDevice((1,), I32), OnDevice((3, 256), F32)
+    proj, pos, cos = OnDevice((3, 512), F32), OnDevice((3,), I32), OnDevice((9, 32), F32)
+    rope = lambda **a: ops.qk_norm_rope(proj, 4, pos, cos, cos, k, v, table, cu, ctx, out=out, **a)
+    ops.attn_packed(q, k, v, table, cu, ctx, max_ctx=127, out=out), ops.kv_keep([(k, v)], table, ctx, keep, count, max_ctx=127), rope(max_ctx=127, sections=[32])
+    assert len(called) == 3
+    for wide in ((1 << 32) + 127, 1 << 31, -(1 << 32) + 100):
+        for call in (lambda: ops.attn_packed(q, k, v, table, cu, ctx, max_ctx=wide, out=out), lambda: ops.attn_tree(q, mask, k, v, table, cu, ctx, max_ctx=wide, out=out),
+                     lambda: ops.kv_keep([(k, v)], table, ctx, keep, count, max_ctx=wide), lambda: rope(max_ctx=wide)):
+            with pytest.raises(ValueError):
+                call()
+    for sections in ([16, 16], [], [(1 << 32) + 32], [-1], [33]):
+        with pytest.raises(ValueError):
+            rope(sections=sections)
+    assert len(called) == 3
+
+
 def test_sections_of_one_axis_have_to_add_up():
     import test_paged_cpu as c
     from flexllm_b200 import build
