@@ -317,7 +317,8 @@ extern "C" int flexllm_linear_w4(int dtype, const void* a, long lda, const uint8
                                  const float* bias, int M, int N, int K, void* y, long ldy, int y_f32, void* stream) {
     FLEXLLM_REQUIRE((dtype == FLEXLLM_F32 || dtype == FLEXLLM_BF16) && (scale_dtype == FLEXLLM_F32 || scale_dtype == FLEXLLM_BF16));
     FLEXLLM_REQUIRE(M >= 0 && N > 0 && K > 0 && group > 0 && group % 32 == 0 && K % group == 0 && lda >= K && lda % 8 == 0 && ldy >= N);
-    if ((M + 31) / 32 > 65535 || K > 1 << 20) return FLEXLLM_ENOTSUP;
+    // tiles of up to 512 rows are counted a grid beyond the last one, in 31 bits
+    if (M > 32 * 65535 || N > 1 << 30 || K > 1 << 20) return FLEXLLM_ENOTSUP;
     if (M == 0) return FLEXLLM_OK;
     FLEXLLM_REQUIRE(a && w && scale && y && aligned(a, 16) && aligned(w, 16) && aligned(scale, scale_dtype == FLEXLLM_F32 ? 4 : 2) && aligned(bias, 4) &&
                     aligned(y, y_f32 || dtype == FLEXLLM_F32 ? 4 : 2));

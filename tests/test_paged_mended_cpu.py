@@ -89,3 +89,14 @@ def test_sections_of_one_axis_have_to_add_up():
     assert c.rope(lib, sec=[32]) == _lib.OK and c.rope(lib) == _lib.OK
     for bad in (31, 33, 0, -32):
         assert c.rope(lib, sec=[bad]) == _lib.EINVAL
+
+
+def test_four_bit_products_count_rows_in_31_bits():
+    """The row numbers behind the last tile of 2^31 - 1 rows would wrap and be read."""
+    from flexllm_b200 import build
+    build.build()
+    lib, P = _lib.load(), 1 << 20
+    call = lambda M, N: lib.flexllm_linear_w4(_lib.BF16, P, 32, P, P, _lib.BF16, None, 32, None, M, N, 32, P, N, 0, None)
+    assert call(0, 1 << 30) == _lib.OK
+    for M, N in ((0, (1 << 30) + 1), (0, (1 << 31) - 1), (0, (1 << 31) - 500)):
+        assert call(M, N) == _lib.ENOTSUP
