@@ -13,7 +13,10 @@ struct W4Call {
     const float* bias;
     int M, N, K;
     void* y; long ldy; int y_f32;
+    int* error_flag;
 };
+// Zero points of more than four bits (`seen`: those of a thread, one on top of the other) are used without the upper ones, and reported.
+__device__ __forceinline__ void check_zeros(uint32_t seen, int* flag) { if ((seen & 0xf0f0f0f0u) && flag) atomicOr(flag, 2); }
 int linear_w4_tc(const W4Call& c, bool f32, cudaStream_t st);
 
 // 8 fp32 activations as the pairs (0,4) (1,5) (2,6) (3,7) of their three bf16 parts

@@ -501,7 +501,8 @@ FLEXLLM_API int flexllm_kv_keep(int dtype, const flexllm_kv_pages* layers_host, 
 
 /* Product with 4-bit weights: y[m][n] = sum_k a[m][k] (q[n][k] - z[n][k/group]) s[n][k/group] (+ bias[n]).
  * a [M][lda] of type dtype, lda a multiple of 8 and >= K; w [N][K/2]: element k of a row in the low (k even) or high nibble of byte k/2; scale [N][K/group]
- * of type scale_dtype (FLEXLLM_BF16 or FLEXLLM_F32); zero [N][K/group] one value of 0 .. 15 per byte, NULL: 8 throughout; bias [N] fp32 or NULL.
+ * of type scale_dtype (FLEXLLM_BF16 or FLEXLLM_F32); zero [N][K/group] one value of 0 .. 15 per byte (larger ones lose
+ * their upper bits and are reported by flexllm_device_status(), FLEXLLM_EDEVDATA), NULL: 8 throughout; bias [N] fp32 or NULL.
  * group a multiple of 32 that divides K <= 2^20; N <= 2^30. y [M][ldy] of type dtype, or fp32 (y_f32). Made for few tokens, where the weights' bytes are the cost;
  * M up to 2,097,120 is taken, 64 tokens at a time (fp32: 32). Nothing is rounded to fewer than 32 bits but y. */
 FLEXLLM_API int flexllm_linear_w4(int dtype, const void* a, long lda, const uint8_t* w, const void* scale, int scale_dtype, const uint8_t* zero, int group,

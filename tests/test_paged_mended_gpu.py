@@ -214,3 +214,24 @@ def test_nothing_is_appended_for_a_sequence_whose_values_are_out_of_range(ops, d
     if min(b - a for a, b in zip(cu, cu[1:])) < 0:              # where starts fall, two sequences claim a row: it may be left out
         k1, v1 = torch.where(k == k0, k0, k1), torch.where(v == v0, v0, v1)
     assert torch.equal(k, k1) and torch.equal(v, v1)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF], ids=["f32", "bf16"])
+@pytest.mark.parametrize("M,N,K,group", [(1, 300, 512, 128), (2, 300, 512, 64), (8, 300, 512, 32), (3, 40, 480, 96), (30, 300, 512, 128), (64, 300, 512, 64), (100, 300, 512, 32), (3, 40, 8192, 256)])
+def test_zero_points_of_more_than_four_bits_are_reported(ops, dtype, M, N, K, group):
+    g = torch.Generator(device="cuda").manual_seed(M)
+    x = torch.randn((M, K), generator=g, device="cuda").to(dtype)
+    w = torch.randint(0, 256, (N, K // 2), generator=g, device="cuda", dtype=torch.uint8)
+    scale = (torch.rand((N, K // group), generator=g, device="cuda") + 0.1).to(BF)
+    zero = torch.randint(0, 16, scale.shape, generator=g, device="cuda", dtype=torch.uint8)
+    assert status() == 0
+    want = ops.linear_w4(x, w, scale, zero=zero)
+    assert status() == 0
+    for n, k, add in ((N - 1, 0, 16), (0, K // group - 1, 128), (N // 2, (K // group) // 2, 240)):
+        bad = zero.clone()
+        bad[n, k] += add
+        got = ops.linear_w4(x, w, scale, zero=bad)
+        assert status() == -7, (n, k)
+        assert torch.equal(got, want)                           # the upper bits count for nothing
+    ops.linear_w4(x, w, scale)
+    assert status() == 0
