@@ -19,20 +19,26 @@ struct W4Call {
 __device__ __forceinline__ void check_zeros(uint32_t seen, int* flag) { if ((seen & 0xf0f0f0f0u) && flag) atomicOr(flag, 2); }
 int linear_w4_tc(const W4Call& c, bool f32, cudaStream_t st);
 
-// 8 fp32 activations as the pairs (0,4) (1,5) (2,6) (3,7) of their three bf16 parts
+__device__ __forceinline__ uint32_t pick(uint32_t a, uint32_t b, uint32_t sel) {
+    uint32_t r;
+    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(sel));
+    return r;
+}
+// 8 fp32 activations as the pairs (0,4) (1,5) (2,6) (3,7) of their three bf16 parts: the upper 16 bits of a number, of what they leave, and of what that
+// leaves, eight significant bits each. (Cut, since the nearest bf16 of a number above 3.39e38 is an infinity.) An infinity leaves nothing, a NaN a NaN.
 struct Eight { uint4 part[3]; };
 __device__ __forceinline__ Eight eight(float (&f)[8]) {
     Eight r;
 #pragma unroll
     for (int k = 0; k < 3; k++) {
-        r.part[k] = make_uint4(bf_pack(f[0], f[4]), bf_pack(f[1], f[5]), bf_pack(f[2], f[6]), bf_pack(f[3], f[7]));
-        const uint32_t w[4] = {r.part[k].x, r.part[k].y, r.part[k].z, r.part[k].w};
+        uint32_t w[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            // what the part leaves; nothing of an infinity or NaN (the first part carries it)
-            f[j] = fabsf(f[j]) <= 3.0e38f ? f[j] - bf_lo(w[j]) : 0.0f;
-            f[j + 4] = fabsf(f[j + 4]) <= 3.0e38f ? f[j + 4] - bf_hi(w[j]) : 0.0f;
+            w[j] = pick(__float_as_uint(f[j]), __float_as_uint(f[j + 4]), 0x7632);
+            f[j] = fabsf(f[j]) == INFINITY ? 0.0f : f[j] - bf_lo(w[j]);
+            f[j + 4] = fabsf(f[j + 4]) == INFINITY ? 0.0f : f[j + 4] - bf_hi(w[j]);
         }
+        r.part[k] = make_uint4(w[0], w[1], w[2], w[3]);
     }
     return r;
 }
@@ -45,11 +51,6 @@ __device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t mask, uint32_t b
 __device__ __forceinline__ uint32_t sub_bf2(uint32_t a, uint32_t b) {
     uint32_t r;
     asm("sub.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
-}
-__device__ __forceinline__ uint32_t pick(uint32_t a, uint32_t b, uint32_t sel) {
-    uint32_t r;
-    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(sel));
     return r;
 }
 // Nibbles i and i + 4 of a word as bf16, less the zero point: 0x4300 | q is 128 + q, and z2 holds 128 + z twice.

@@ -504,7 +504,8 @@ FLEXLLM_API int flexllm_kv_keep(int dtype, const flexllm_kv_pages* layers_host, 
  * of type scale_dtype (FLEXLLM_BF16 or FLEXLLM_F32); zero [N][K/group] one value of 0 .. 15 per byte (larger ones lose
  * their upper bits and are reported by flexllm_device_status(), FLEXLLM_EDEVDATA), NULL: 8 throughout; bias [N] fp32 or NULL.
  * group a multiple of 32 that divides K <= 2^20; N <= 2^30. y [M][ldy] of type dtype, or fp32 (y_f32). Made for few tokens, where the weights' bytes are the cost;
- * M up to 2,097,120 is taken, 64 tokens at a time (fp32: 32). Nothing is rounded to fewer than 32 bits but y. */
+ * M up to 2,097,120 is taken, 64 tokens at a time (fp32: 32). Nothing is rounded to fewer than 32 bits but y; a group's
+ * sum of a (q - z), which its scale then multiplies, has to be in fp32's range. */
 FLEXLLM_API int flexllm_linear_w4(int dtype, const void* a, long lda, const uint8_t* w, const void* scale, int scale_dtype, const uint8_t* zero, int group,
                                   const float* bias, int M, int N, int K, void* y, long ldy, int y_f32, void* stream);
 

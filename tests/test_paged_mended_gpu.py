@@ -235,3 +235,32 @@ def test_zero_points_of_more_than_four_bits_are_reported(ops, dtype, M, N, K, gr
         assert torch.equal(got, want)                           # the upper bits count for nothing
     ops.linear_w4(x, w, scale)
     assert status() == 0
+
+
+@pytest.mark.parametrize("M,N,K,group", [(1, 70, 256, 128), (4, 70, 128, 32), (20, 140, 256, 64), (3, 40, 4096, 128)])
+def test_activations_at_the_ends_of_32_bits(ops, M, N, K, group):
+    """fp32 activations up to the largest number, weights of -1, 0 and 1 and scales of 2^-60: every product and sum is in range. The error is that of sums in
+    fp32 (paged_cases.linear_w4); a row with one number is exact."""
+    g = torch.Generator(device="cuda").manual_seed(K)
+    big = torch.finfo(F32).max
+    q = torch.randint(7, 10, (N, K), generator=g, device="cuda", dtype=torch.uint8)
+    w = (q[:, 0::2] | q[:, 1::2] << 4).contiguous()
+    scale = torch.full((N, K // group), 2.0 ** -60, device="cuda")
+    for value in (big, -big, 3.39e38, -3.395e38, 3.0e38, 2.99e38, 1e-30, 2.0 ** -100):
+        x = torch.zeros((M, K), device="cuda")
+        at = torch.randint(0, K, (M,), generator=g, device="cuda")
+        x[torch.arange(M), at] = value
+        want = (q.double() - 8)[:, at].T * x.double().amax(1, keepdim=True).where(torch.tensor(value > 0), x.double().amin(1, keepdim=True)) * 2.0 ** -60
+        got = ops.linear_w4(x, w, scale)
+        assert torch.equal(got, want.float()), value            # (1e-30 2^-60 is below half the smallest fp32 number)
+    x = torch.randn((M, K), generator=g, device="cuda") * 2.0 ** 110
+    want, far = pc.linear_w4(x, w, scale, None)
+    assert ((ops.linear_w4(x, w, scale).double() - want).abs() <= far).all()
+    for value in (float("inf"), -float("inf"), float("nan")):
+        x[0, 5] = value
+        got = ops.linear_w4(x, w, scale)
+        odd = q[:, 5] != 8
+        assert not torch.isfinite(got[0][odd]).any() and (torch.isnan(got[0]) if value != value else torch.isinf(got[0]) | torch.isnan(got[0])).all()
+        assert torch.isfinite(got[1:]).all()
+        if value == value:
+            assert torch.equal(got[0][odd], (q[:, 5][odd].float() - 8) * value)
