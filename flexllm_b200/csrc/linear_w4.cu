@@ -175,7 +175,8 @@ __global__ void __launch_bounds__(kWarps * 32, 1) linear_w4_kernel(const __grid_
 #pragma unroll
         for (int u = 0; u < U; u++) {
             if (!PACKED && k0 + u * BK >= p.K) break;
-            float sc[4], part[2][4];
+            // an MMA cuts its fp32 sums instead of rounding them: the small parts' products have sums of their own, and do not cut the large ones
+            float sc[4], part[PL == 3 ? 2 : 1][2][4];
             uint32_t z[4];
 #pragma unroll
             for (int r = 0; r < 4; r++) { z[r] = zero_of(cur.z[r], u); sc[r] = scale_of(cur.s[r], u); }
@@ -191,17 +192,17 @@ __global__ void __launch_bounds__(kWarps * 32, 1) linear_w4_kernel(const __grid_
                     const uint4 x = *reinterpret_cast<const uint4*>(xb + q * plane + (u * VW + j) * XC);
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
-                        if (j == 0 && q == 0) mma_bf16_first(part[h], a[2 * h][0], a[2 * h + 1][0], a[2 * h][1], a[2 * h + 1][1], x.x, x.y);
-                        else mma_bf16(part[h], a[2 * h][0], a[2 * h + 1][0], a[2 * h][1], a[2 * h + 1][1], x.x, x.y);
+                        if (j == 0 && q < 2) mma_bf16_first(part[q > 0][h], a[2 * h][0], a[2 * h + 1][0], a[2 * h][1], a[2 * h + 1][1], x.x, x.y);
+                        else mma_bf16(part[q > 0][h], a[2 * h][0], a[2 * h + 1][0], a[2 * h][1], a[2 * h + 1][1], x.x, x.y);
                     }
 #pragma unroll
-                    for (int h = 0; h < 2; h++) mma_bf16(part[h], a[2 * h][2], a[2 * h + 1][2], a[2 * h][3], a[2 * h + 1][3], x.z, x.w);
+                    for (int h = 0; h < 2; h++) mma_bf16(part[q > 0][h], a[2 * h][2], a[2 * h + 1][2], a[2 * h][3], a[2 * h + 1][3], x.z, x.w);
                 }
             }
 #pragma unroll
             for (int h = 0; h < 2; h++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) acc[h][i] = __fmaf_rn(part[h][i], sc[2 * h + (i >> 1)], acc[h][i]);
+                for (int i = 0; i < 4; i++) acc[h][i] = __fmaf_rn(PL == 3 ? part[0][h][i] + part[PL == 3][h][i] : part[0][h][i], sc[2 * h + (i >> 1)], acc[h][i]);
         }
     };
     // the warps' parts of K, joined in their order; [ks][tokens][rows of the CTA + 4], behind the activations when these are needed again

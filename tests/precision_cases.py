@@ -57,3 +57,12 @@ def within(got, q, k, v):
     bound = 4 * (plain(q, k, v).double() - want).abs().max().item() + 2.0 ** -22 * want.abs().max().item()
     over = (got.double() - want).abs().max().item() / bound
     return over <= 1.0, over
+
+
+def linear_within(got, x, w):
+    """The same for products got = x w^T of fp32 x with weights w in 64 bits; the plain form has the weights in fp32. A tensor core cuts the large sum of a group 8
+    times at most, by half a step, 2^-24 of a sum that is half grown on average: 2^-22 of the largest result is granted."""
+    want = x.double() @ w.T
+    bound = 4 * ((x @ w.float().T).double() - want).abs().max().item() + 2.0 ** -22 * want.abs().max().item()
+    over = (got.double() - want).abs().max().item() / bound
+    return over <= 1.0, over

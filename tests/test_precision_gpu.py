@@ -49,3 +49,17 @@ def check(ops, q, k, v, heads):
         for g in heads:
             ok, over = pc.within(out[g * R:(g + 1) * R], q[0, g * R:(g + 1) * R], k[:, g], v[:, g])
             assert ok, (g, over)
+
+
+@pytest.mark.parametrize("M", [1, 4, 8, 16, 64])
+@pytest.mark.parametrize("K,group", [(256, 128), (2048, 128), (2048, 64), (2048, 32), (8192, 256)])
+@pytest.mark.parametrize("mean", [0.0, 1.0], ids=["centred", "offset"])
+def test_four_bit_products(ops, M, K, group, mean):
+    N, g = 200, torch.Generator(device="cuda").manual_seed(M + K + group)
+    x = torch.randn((M, K), generator=g, device="cuda") + mean
+    q = torch.randint(0, 16, (N, K), generator=g, device="cuda", dtype=torch.uint8)
+    scale = torch.rand((N, K // group), generator=g, device="cuda") + 0.1
+    for z in (0, 8):
+        zero = torch.full(scale.shape, z, dtype=torch.uint8, device="cuda")
+        ok, over = pc.linear_within(ops.linear_w4(x, (q[:, 0::2] | q[:, 1::2] << 4).contiguous(), scale, zero=zero), x, (q.double() - z) * scale.double().repeat_interleave(group, 1))
+        assert ok, (z, over)
