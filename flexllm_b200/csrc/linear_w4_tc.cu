@@ -164,7 +164,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_w4_tc_kernel(const __gri
         };
         // zero points of step n into a slot that the conversion of step n - kZeros has left: its products are among the sums
         struct Zeros { uint32_t v[U]; } zero;
-        uint32_t zeros = 0;
         auto fetch_zero = [&](int n) {
             Zeros z;
 #pragma unroll
@@ -172,8 +171,10 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_w4_tc_kernel(const __gri
             return z;
         };
         auto hand_zero = [&](int n, const Zeros& z) {
+            uint32_t seen = 0;
 #pragma unroll
-            for (int u = 0; u < U; u++) { base_ptr[S::z + n % kZeros * 512 + u * 128 + rr] = (uint8_t)z.v[u]; zeros |= z.v[u]; }
+            for (int u = 0; u < U; u++) { base_ptr[S::z + n % kZeros * 512 + u * 128 + rr] = (uint8_t)z.v[u]; seen |= z.v[u]; }
+            check_zeros(seen, c.error_flag);
             __syncwarp();
             if (lane == 0) mbar_arrive(bar_z + 8 * (n % kZeros));
         };
@@ -249,7 +250,6 @@ __global__ void __launch_bounds__(kTcThreads, 1) linear_w4_tc_kernel(const __gri
                 zero = fetch_zero(n + kZerosAhead + 1);
             }
         }
-        check_zeros(zeros, c.error_flag);
     }
     // the sums into shared memory (every product has been waited for), [token][132]; the CTAs of the cluster join the tokens in turn
     float* red = reinterpret_cast<float*>(base_ptr);
