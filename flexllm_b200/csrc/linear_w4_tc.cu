@@ -10,8 +10,8 @@
 //   warps 0 .. 3   take a step's sums out of TMEM and add them up in fp32 registers, times the groups' scales: no weight is ever rounded;
 //                  they also hand the zero points to the converting warps, six steps ahead, and cut fp32 activations into their parts
 // Few rows: the CTAs of a cluster cut K, and their sums meet in shared memory, in a fixed order.
-// Bound by the chain of a step: words from shared memory, unpacked and put back (about 600 clocks), their fence, eight MMAs. 48 tokens, 16384 x 2048: 11.8 us;
-// 64 tokens, 8192 x 8192: 21.7 us, 396 TFLOP/s, 1.5 TB/s; 64 tokens, 128256 x 2048: 83 us; fp32, 64 tokens, 8192 x 2048: 21.5 us (warp MMAs, 68).
+// Bound by the chain of a step: words from shared memory, unpacked and put back (about 600 clocks), their fence, eight MMAs. 48 tokens, 16384 x 2048: 12.1 us;
+// 64 tokens, 8192 x 8192: 22.4 us, 383 TFLOP/s, 1.5 TB/s; 64 tokens, 128256 x 2048: 88 us; fp32, 64 tokens, 8192 x 2048: 23 us (warp MMAs, 68).
 #include "linear_w4.h"
 #include "tc_common.cuh"
 

@@ -462,7 +462,8 @@ FLEXLLM_API int flexllm_attn_window(int dtype, flexllm_kv_cache* c, int layer, c
  * not looked at). max_ctx: largest position of the call, < 64 * max_pages and < 2^30. cu, ctx, page_table, pos, keep and count are device memory;
  * values out of range are clamped and reported by flexllm_device_status() (FLEXLLM_EDEVDATA); nothing is appended for a sequence whose values are, or where
  * the table names no page (where cu falls, rows that two sequences claim may be left out too). Element type FLEXLLM_BF16 or FLEXLLM_F32 for rows and
- * pages alike; scores, norms, weights and sums are fp32. kdim and vdim multiples of 8 up to 256 (else FLEXLLM_ENOTSUP).
+ * pages alike; scores, norms, maxima and sums are fp32. In bf16 attention's weights are rounded to bf16 before they multiply the values, as results
+ * are; in fp32 nothing is. kdim and vdim multiples of 8 up to 256 (else FLEXLLM_ENOTSUP).
  * ------------------------------------------------------------------------------------------- */
 /* One layer's pages of 64 tokens, K [n_pages][hkv][64][kdim] and V [n_pages][hkv][vdim][64], 16-byte aligned: memory of the caller, or a layer of a
  * cache made by flexllm_kv_cache_create_float, which flexllm_kv_cache_pages describes. */
