@@ -460,7 +460,7 @@ FLEXLLM_API int flexllm_attn_window(int dtype, flexllm_kv_cache* c, int layer, c
  * A call has T packed rows; sequence b < B has the rows cu[b] .. cu[b+1] - 1 (cu [B+1], cu[0] = 0; a sequence may have none, rows from cu[B] on are
  * left alone) at the cache positions ctx[b] .. of its pages page_table[b][0 ..] (max_pages per sequence; entries behind its last position are
  * not looked at). max_ctx: largest position of the call, < 64 * max_pages and < 2^30. cu, ctx, page_table, pos, keep and count are device memory;
- * values out of range are clamped and reported by flexllm_device_status() (FLEXLLM_EDEVDATA); nothing is appended for a sequence whose values are, or where
+ * values out of range are clamped and reported by flexllm_device_status() (FLEXLLM_EDEVDATA); nothing is appended for a sequence whose cu or ctx are, or where
  * the table names no page (where cu falls, rows that two sequences claim may be left out too). Element type FLEXLLM_BF16 or FLEXLLM_F32 for rows and
  * pages alike; scores, norms, maxima and sums are fp32. In bf16 attention's weights are rounded to bf16 before they multiply the values, as results
  * are; in fp32 nothing is. kdim and vdim multiples of 8 up to 256 (else FLEXLLM_ENOTSUP).
