@@ -6,7 +6,7 @@
 // m is lazy: only a row whose maximum exceeds it by more than kSlack moves it and rescales its O in TMEM.
 // P is rounded to bf16 since both operands of an MMA have one type, and a second part would double the products with V: results are off by 1.9e-3 to 2.3e-3
 // (root of the mean square, relative), where rounding the result alone leaves 1.6e-3. The weights' sum is of the unrounded ones, in fp32. O is the
-// tensor core's fp32 sum, which it cuts instead of rounding: 5e-4 low after 80,000 keys in one part, when half a step of the result is 2e-3 to 3.9e-3.
+// tensor core's fp32 sum, which it cuts instead of rounding: 5e-4 low after 80,000 keys in one part and 2.5e-3 after a million, when half a step of the result is 2e-3 to 3.9e-3.
 //   kPair   two tiles per CTA, so that one tile's softmax runs under the other's products: prompts
 //   kOne    one tile per CTA, two CTAs per SM: more tiles than SMs; and heads of more than 128
 //   kTurns  one tile per CTA with two sets of scores, outputs and softmax warps that take the key tiles in turn: fewer tiles than SMs (trees,
